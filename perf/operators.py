@@ -2,7 +2,7 @@
 
 Keys and values of G heads of D values lie in pages [pages, 2, G, page, D] (keys, then values), in eight bits as codes of
 float8_e4m3fn with one exponent a token, head and plane: a value is code * 2^(exponent - 127).  The exponent of a row of D values
-is 127 + n with the smallest n for which max |x| <= 448 * 2^n, n in -100 .. 119 (127 for a row of zeros); codes are x * 2^-n rounded
+is 127 + n with the smallest n for which max |x| <= 448 * 2^n, n in -60 .. 60 (127 for a row of zeros); codes are x * 2^-n rounded
 to the nearest, ties to even.
 
   write    keys and values of new tokens, as float32 columns of a wider product or as bfloat16 rows, go into their slots
@@ -24,7 +24,7 @@ import torch
 own = False
 
 DEVICE = "cuda:0"
-LOWEST, HIGHEST = -100, 119
+LOWEST, HIGHEST = -60, 60
 
 
 def _attend(name, **kw):
