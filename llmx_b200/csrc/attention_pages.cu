@@ -1,0 +1,160 @@
+// Softmax attention of requests' new rows over pages, in any of the cache's types, under a window or a tree's bits.
+//
+// Request r brings row_count[r] rows, row_start[r] the first, after history[r] keys that the cache holds already; the rows' own keys
+// and values follow them there.  Row i sees the keys t with
+//     t <= history + i,  t > history + i - window (window > 0)         or, with a tree,
+//     t < history  or  bit (t - history) of its words is set (t < history + row_count)
+// and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key.
+// Query head h reads key/value head h / (heads / kv_heads).  A page that is not in the cache reads as zeros.
+//
+// The general form: one block a (row, head), any width to 256, any page size.  Each warp walks every fourth key in increasing order
+// with a running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone.
+#include "e4m3.cuh"
+#include <cuda_fp16.h>
+#include <math.h>
+
+namespace {
+constexpr int WARPS = 4;
+constexpr int MAX_PER_LANE = 8;     // widths up to 256
+
+struct Rows {                       // whose rows these are and where their keys lie
+    const int* row_start;
+    const int* row_count;
+    const int* history;
+    const int* tables;              // [requests, table_stride]
+    int table_stride, total_rows, pages, page_size, window;
+    const unsigned* tree;           // [rows, tree_words] or null
+    int tree_words;
+};
+
+struct E4m3 {};                     // the cache's type: codes, exponents beside them
+
+__device__ __forceinline__ float read_value(const float* p) { return *p; }
+__device__ __forceinline__ float read_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float read_value(const uint8_t* p) { return __half2float(__ushort_as_half((unsigned short)(e4m3::halves(*p) & 0xffffu))); }
+
+template <typename T> struct Stored { typedef T type; };
+template <> struct Stored<E4m3> { typedef uint8_t type; };
+
+template <typename QT, typename KVT>
+__global__ void __launch_bounds__(WARPS * 32)
+attention_pages_kernel(const QT* __restrict__ q, const void* __restrict__ cache, const uint8_t* __restrict__ exponents, QT* __restrict__ out, Rows a,
+                       int heads, int kv_heads, int head_dim, float scale) {
+    pdl_trigger();
+    pdl_wait();
+    typedef typename Stored<KVT>::type S;
+    constexpr bool eight = sizeof(S) == 1;
+    extern __shared__ float smem[];  // WARPS * (head_dim + 2)
+    const int i = blockIdx.x, h = blockIdx.y, r = blockIdx.z;
+    const int count = a.row_count[r], history = max(a.history[r], 0);
+    const int row = a.row_start[r] + i;
+    if (i >= count || row < 0 || row >= a.total_rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = h / (heads / kv_heads);
+    const long long pos = (long long)history + i;
+    const long long reach = (long long)a.table_stride * a.page_size;
+    const long long end = min(a.tree ? (long long)history + min(count, 32 * a.tree_words) : pos + 1, reach);
+    const long long lo = a.window > 0 ? max(0ll, pos - a.window + 1) : 0;
+    const int* table = a.tables + (size_t)r * a.table_stride;
+    const unsigned* bits = a.tree ? a.tree + (size_t)row * a.tree_words : nullptr;
+
+    float qv[MAX_PER_LANE], acc[MAX_PER_LANE];
+    const QT* qrow = q + ((size_t)row * heads + h) * head_dim;
+#pragma unroll
+    for (int j = 0; j < MAX_PER_LANE; ++j) {
+        const int d = lane + 32 * j;
+        qv[j] = d < head_dim ? to_float(qrow[d]) : 0.0f;
+        acc[j] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (long long t = lo + warp; t < end; t += WARPS) {
+        if (bits && t >= history && !(bits[(t - history) >> 5] >> ((t - history) & 31) & 1u)) continue;
+        const int page = table[t / a.page_size];
+        const bool there = page >= 0 && page < a.pages;
+        const size_t slot = (((size_t)max(page, 0) * 2) * kv_heads + g) * a.page_size + t % a.page_size;
+        const size_t v_slot = slot + (size_t)kv_heads * a.page_size;
+        const S* kp = (const S*)cache + slot * head_dim;
+        const S* vp = (const S*)cache + v_slot * head_dim;
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < MAX_PER_LANE; ++j) {
+            const int d = lane + 32 * j;
+            if (there && d < head_dim) s = fmaf(qv[j], read_value(kp + d), s);
+        }
+        s = warp_sum(s);
+        float vf = 1.0f;
+        if (eight && there) {
+            s *= e4m3::up(exponents[slot]);
+            vf = e4m3::up(exponents[v_slot]);
+        }
+        s *= scale;
+        const float m_new = fmaxf(m, s);
+        const float corr = expf(m - m_new);  // exp(-inf) = 0 on the first key
+        const float e = expf(s - m_new);
+        l = l * corr + e;
+#pragma unroll
+        for (int j = 0; j < MAX_PER_LANE; ++j) {
+            const int d = lane + 32 * j;
+            acc[j] = fmaf(e, there && d < head_dim ? read_value(vp + d) * vf : 0.0f, acc[j] * corr);
+        }
+        m = m_new;
+    }
+    float* mine = smem + warp * (head_dim + 2);
+#pragma unroll
+    for (int j = 0; j < MAX_PER_LANE; ++j) {
+        const int d = lane + 32 * j;
+        if (d < head_dim) mine[d] = acc[j];
+    }
+    if (lane == 0) {
+        mine[head_dim] = m;
+        mine[head_dim + 1] = l;
+    }
+    __syncthreads();
+    if (warp) return;
+    float mm = -INFINITY, ll = 0.0f, f[WARPS];
+    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, smem[w * (head_dim + 2) + head_dim]);
+    for (int w = 0; w < WARPS; ++w) {
+        // A warp without keys has a sum of zero and says nothing; one whose scores are NaN has a NaN there.
+        const float lw = smem[w * (head_dim + 2) + head_dim + 1], mw = smem[w * (head_dim + 2) + head_dim];
+        f[w] = lw == 0.0f ? 0.0f : expf(mw - mm);
+        ll = fmaf(lw, f[w], ll);
+    }
+    QT* orow = out + ((size_t)row * heads + h) * head_dim;
+    for (int d = lane; d < head_dim; d += 32) {
+        float o = 0.0f;
+        for (int w = 0; w < WARPS; ++w) o = fmaf(smem[w * (head_dim + 2) + d], f[w], o);
+        orow[d] = from_float<QT>(ll == 0.0f ? 0.0f : o / ll);
+    }
+}
+}  // namespace
+
+// q/out [total_rows, heads, head_dim] of `q_dtype`; the cache [pages, 2, kv_heads, page_size, head_dim] of `cache_dtype`, with `exponents`
+// [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  No request brings more than `max_rows` rows.  Rows that no request names
+// are left as they are.
+LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cache, const void* exponents, int cache_dtype, void* out,
+                                     const int* row_start, const int* row_count, const int* history, const int* tables, int table_stride,
+                                     const void* tree, int tree_words, int requests, int total_rows, int max_rows, int pages, int heads,
+                                     int kv_heads, int head_dim, int page_size, int window, float scale, cudaStream_t stream) {
+    if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
+    if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
+        return LLMX_ERR_UNSUPPORTED;
+    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words};
+    const size_t shmem = (size_t)WARPS * (head_dim + 2) * sizeof(float);
+    const dim3 grid((unsigned)max_rows, (unsigned)heads, (unsigned)requests);
+#define LLMX_PAGES(QT, KVT)                                                                                                               \
+    launch_kernel(attention_pages_kernel<QT, KVT>, grid, dim3(WARPS * 32), shmem, stream, (const QT*)q, cache, (const uint8_t*)exponents, (QT*)out, \
+                  a, heads, kv_heads, head_dim, scale)
+#define LLMX_PAGES_Q(KVT)                                    \
+    do {                                                     \
+        if (q_dtype == LLMX_BF16) LLMX_PAGES(__nv_bfloat16, KVT); \
+        else if (q_dtype == LLMX_F32) LLMX_PAGES(float, KVT); \
+        else return LLMX_ERR_BAD_ARGUMENT;                   \
+    } while (0)
+    if (cache_dtype == LLMX_E4M3) LLMX_PAGES_Q(E4m3);
+    else if (cache_dtype == LLMX_BF16) LLMX_PAGES_Q(__nv_bfloat16);
+    else if (cache_dtype == LLMX_F32) LLMX_PAGES_Q(float);
+    else return LLMX_ERR_BAD_ARGUMENT;
+#undef LLMX_PAGES_Q
+#undef LLMX_PAGES
+    return launch_status();
+}

@@ -50,6 +50,8 @@ LIBRARIES: Dict[str, List[str]] = {
     "moe": ["moe.cu"],                        # experts chosen by a table: routing on the device, grouped products
     "latent_attention": ["latent_attention.cu"],   # attention over a cache of latents
     "latent_prompt_tc": ["latent_prompt_tc.cu"],    # the same for requests of many rows: keys and values made once a step
+    "cache_e4m3": ["cache_e4m3.cu"],          # keys and values into a cache of eight bits, and back
+    "attention_pages": ["attention_pages.cu"],     # attention over pages of any type, that one's among them, under a window or a tree's bits
     "selftest": ["selftest.cu"],              # the bounded wait made to run out on purpose (tests)
     "runtime": ["runtime/runtime.cpp", "runtime/engine.cpp", "runtime/loader.cpp"],       # host code: the parts' forward passes (no kernels of its own)
 }

@@ -12,13 +12,14 @@ these functions raise.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from .csrc import build as _build
 
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2            # E4M3: of a cache alone (`QuantizedPages`)
 _CODE = {torch.float32: F32, torch.bfloat16: BF16}
 
 
@@ -151,6 +152,9 @@ _SIGNATURES = {
     ("latent_prompt_tc", "llmx_latent_expand"): [_p, ctypes.c_longlong, _p, _p, _i, _p, _p, _i, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i,
                                                  _i, _p, _p],
     ("latent_prompt_tc", "llmx_latent_prompt"): [_p, _i, _p, _i, _p, _p, _i, _p, _i, _i, _f, _p, _i, _i, _i, _i, _i, _f, _p, _p],
+    ("cache_e4m3", "llmx_quantize_kv"): [_p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    ("cache_e4m3", "llmx_dequantize_pages"): [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+    ("attention_pages", "llmx_attention_pages"): [_p, _i, _p, _p, _i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p],
     ("gemm_plain", "llmx_gemm_plain"): [_p, _i, _p, _i, _p, _i, _i, _i, _i, _p],
     ("attention_plain", "llmx_attention_plain"): [_p, _i, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _p],
 }
@@ -1286,3 +1290,143 @@ def latent_attention_prompt(q: torch.Tensor, cache: torch.Tensor, w_uk: torch.Te
             freq.numel(), 1 if halves else 0, float(magnitude), _ptr(positions), heads, h, n, rot, int(window or 0), float(scale), err,
             _stream()), "latent_prompt")
     return out
+
+
+# ---- a cache in eight bits, and attention for trees of drafted tokens -----------------------------------------------------------------
+class QuantizedPages:
+    """Keys and values in eight bits: `codes` float8_e4m3fn [pages, 2, kv_heads, page_size, head_dim] (keys, then values) and
+    `exponents` uint8 [pages, 2, kv_heads, page_size].  A value is code * 2^(exponent - 127); the exponent of a row of head_dim values
+    is 127 + n with the smallest n for which max |x| <= 448 * 2^n, n in -60 .. 60 (127 for a row of zeros), its codes are
+    x * 2^-n rounded to the nearest, ties to even (to 448 where the limits of n leave more).  A row that holds an infinity or a
+    NaN has the exponent 255 and reads as NaN throughout."""
+    __slots__ = ("codes", "exponents", "pages", "kv_heads", "page_size", "head_dim")
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
+        _need(codes.dtype is torch.float8_e4m3fn and exponents.dtype is torch.uint8 and codes.dim() == 5 and codes.shape[1] == 2
+              and codes.shape[:4] == exponents.shape and codes.is_contiguous() and exponents.is_contiguous() and codes.device == exponents.device,
+              "quantized pages: codes float8_e4m3fn [pages, 2, kv_heads, page size, head width] and exponents uint8 without the last axis, contiguous")
+        self.codes, self.exponents = codes, exponents
+        self.pages, _, self.kv_heads, self.page_size, self.head_dim = codes.shape
+
+    @classmethod
+    def zeros(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device) -> "QuantizedPages":
+        """A cache whose every slot holds a row of zeros."""
+        return cls(torch.zeros((pages, 2, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.full((pages, 2, kv_heads, page_size), 127, dtype=torch.uint8, device=device))
+
+
+def _launched(device: torch.device, call):
+    """`call(stream)` with `device` the current one, on its current stream."""
+    _need(device.type == "cuda", "kernel arguments must be CUDA tensors (there is no CPU path)")
+    if device.index == torch.cuda.current_device():
+        return call(_stream())
+    with torch.cuda.device(device):
+        return call(_stream())
+
+
+def _same_device(what: str, device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        _need(t is None or t.device == device, f"{what}: tensors on different devices")
+
+
+def quantize_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: QuantizedPages) -> None:
+    """Row r of keys and values goes to slot slots[r] (page * page size + place) of a cache in eight bits; k, v float32 or bfloat16
+    [rows, kv_heads, head_dim], each row contiguous and rows at any distance (columns of a product's output); slots int32
+    [rows], each named once, negative ones (and ones beyond the cache) not kept."""
+    _need(k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype and tuple(k.shape[1:]) == (cache.kv_heads, cache.head_dim),
+          "quantize_kv: keys and values [rows, kv_heads, head_dim] of one type and of the cache's heads")
+    rows, heads, dim = k.shape
+    for t in (k, v):
+        _need(rows == 0 or ((dim == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == dim)), "quantize_kv: a row's heads must lie one after another")
+    _need(slots.dtype is torch.int32 and slots.numel() == rows and slots.is_contiguous(), "quantize_kv: an int32 slot per row")
+    _need(dim <= 256, "quantize_kv: heads of 256 values at most")
+    code = _code(k)
+    _same_device("quantize_kv", k.device, v, slots, cache.codes)
+    _check(_launched(k.device, lambda stream: _fn("cache_e4m3", "llmx_quantize_kv")(
+        _ptr(k), k.stride(0), _ptr(v), v.stride(0), code, _ptr(slots), _ptr(cache.codes), _ptr(cache.exponents), rows, heads, dim, cache.page_size,
+        cache.pages, stream)), "quantize_kv")
+
+
+def dequantize_pages(cache: QuantizedPages, pages: torch.Tensor, out: torch.Tensor, used: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[i] = page pages[i] of a cache in eight bits; out float32 or bfloat16 [n, 2, kv_heads, page_size, head_dim], pages int32 [n].
+    `used` int32 [n]: how many of each page's slots hold tokens; the others (and pages outside of the cache) come as zeros."""
+    n = pages.numel()
+    _need(pages.dtype is torch.int32 and pages.is_contiguous() and tuple(out.shape) == (n, *cache.codes.shape[1:]) and out.is_contiguous(),
+          "dequantize_pages: int32 page ids and an output [ids, 2, kv_heads, page size, head width], contiguous")
+    _need(used is None or (used.dtype is torch.int32 and used.numel() == n and used.is_contiguous()), "dequantize_pages: an int32 count per page id")
+    code = _code(out)
+    _same_device("dequantize_pages", out.device, pages, used, cache.codes)
+    _check(_launched(out.device, lambda stream: _fn("cache_e4m3", "llmx_dequantize_pages")(
+        _ptr(cache.codes), _ptr(cache.exponents), _ptr(pages), _ptr(used), _ptr(out), code, n, cache.kv_heads, cache.head_dim, cache.page_size, cache.pages,
+        stream)), "dequantize_pages")
+    return out
+
+
+def tree_bits(parents: Sequence[Sequence[int]]) -> np.ndarray:
+    """What `attention_tree` wants to know of drafted tokens, int32 [rows, words], from the token that each of a request's drafted
+    tokens continues (its place among them, less than the token's own; -1: the request's history): a token sees itself, what it
+    continues, and so on."""
+    words = max(1, -(-max((len(p) for p in parents), default=0) // 32))
+    bits = np.zeros((sum(len(p) for p in parents), words), dtype=np.uint32)
+    first = 0
+    for own in parents:
+        for i, parent in enumerate(own):
+            _need(-1 <= parent < i, f"tree_bits: token {i} continues {parent}, which is no earlier token")
+            if parent >= 0:
+                bits[first + i] = bits[first + parent]
+            bits[first + i, i // 32] |= np.uint32(1 << (i % 32))
+        first += len(own)
+    return bits.view(np.int32)
+
+
+def _attention_pages(what: str, q, cache, out, row_start, row_count, history, block_tables, tree, heads, kv_heads, head_dim, window, scale, max_rows,
+                     max_context):
+    eight = isinstance(cache, QuantizedPages)
+    stored = cache.codes if eight else cache
+    rows, requests = q.shape[0], row_start.numel()
+    _need(q.dim() == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and q.shape[1] == heads * head_dim and out.shape == q.shape
+          and out.dtype == q.dtype and q.is_contiguous() and out.is_contiguous(), f"{what}: q and out [rows, heads * head_dim] of one type, contiguous")
+    _need(stored.dim() == 5 and stored.shape[1] == 2 and stored.shape[2] == kv_heads and stored.shape[4] == head_dim and stored.is_contiguous(),
+          f"{what}: a cache [pages, 2, kv_heads, page size, head_dim]")
+    _need(head_dim <= 256, f"{what}: heads of 256 values at most")
+    for t in (row_start, row_count, history):
+        _need(t.dtype is torch.int32 and t.numel() == requests and t.is_contiguous(), f"{what}: int32 first rows, row counts and histories, one per request")
+    _need(block_tables.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests and block_tables.is_contiguous(),
+          f"{what}: int32 block tables [requests, pages]")
+    _need(tree is None or (tree.dtype is torch.int32 and tree.dim() == 2 and tree.shape[0] == rows and tree.is_contiguous()),
+          f"{what}: int32 words of bits, [rows, words]")
+    _need(max_rows >= 0 and max_context >= 0 and (window is None or window > 0), f"{what}: bounds of at least 0 and a window of at least 1")
+    q_code, code = _code(q), E4M3 if eight else _code(stored)
+    _same_device(what, q.device, out, stored, row_start, row_count, history, block_tables, tree)
+    _check(_launched(q.device, lambda stream: _fn("attention_pages", "llmx_attention_pages")(
+        _ptr(q), q_code, _ptr(stored), _ptr(cache.exponents if eight else None), code, _ptr(out), _ptr(row_start), _ptr(row_count), _ptr(history),
+        _ptr(block_tables), block_tables.shape[1], _ptr(tree), 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), stored.shape[0],
+        heads, kv_heads, head_dim, stored.shape[3], int(window or 0), float(scale), stream)), what)
+    return out
+
+
+def attention_quantized(q: torch.Tensor, cache: QuantizedPages, out: torch.Tensor, row_start: torch.Tensor, row_count: torch.Tensor,
+                        history: torch.Tensor, block_tables: torch.Tensor, heads: int, kv_heads: int, head_dim: int, window: Optional[int],
+                        scale: float, max_rows: int, max_context: int) -> torch.Tensor:
+    """out = softmax(scale q k^T) v over a cache in eight bits; q, out float32 or bfloat16 [rows, heads * head_dim].  Request r brings the
+    rows row_start[r] .. + row_count[r], whose keys and values the cache holds already behind the history[r] tokens before them;
+    its row i sees the keys up to history[r] + i (the last `window` of them); head h reads key/value head h // (heads // kv_heads).
+    Key t of a request lies in page block_tables[r, t // page size]; a page that is not in the cache reads as zeros.
+    row_start, row_count, history int32 [requests] and block_tables int32 [requests, pages] on the device, as a step's metadata
+    has them; `max_rows`, `max_context`: the most rows that a request brings and the most keys that one has, its own rows' among
+    them.  Rows of no request are left as they are."""
+    _need(isinstance(cache, QuantizedPages), "attention_quantized: a cache in eight bits (QuantizedPages)")
+    return _attention_pages("attention_quantized", q, cache, out, row_start, row_count, history, block_tables, None, heads, kv_heads, head_dim, window,
+                            scale, max_rows, max_context)
+
+
+def attention_tree(q: torch.Tensor, cache, out: torch.Tensor, row_start: torch.Tensor, row_count: torch.Tensor, history: torch.Tensor,
+                   block_tables: torch.Tensor, tree: torch.Tensor, heads: int, kv_heads: int, head_dim: int, scale: float, max_rows: int,
+                   max_context: int) -> torch.Tensor:
+    """`attention_quantized` for rows that are drafted tokens: a row sees its request's whole history, and key history[r] + j, that
+    of the request's j-th row, where bit j % 32 of word j // 32 of its words in `tree` (int32 [rows, words], `tree_bits`) is set:
+    rows may see rows behind them, and not themselves; one that sees no key is zeros.  `cache`: `QuantizedPages`, or bfloat16 or
+    float32 [pages, 2, kv_heads, page size, head_dim].  Where the drafted tokens' rotations stand is the queries' and keys' own
+    business."""
+    return _attention_pages("attention_tree", q, cache, out, row_start, row_count, history, block_tables, tree, heads, kv_heads, head_dim, None, scale,
+                            max_rows, max_context)
