@@ -7,25 +7,17 @@
 // and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key.
 // Query head h reads key/value head h / (heads / kv_heads).  A page that is not in the cache reads as zeros.
 //
-// The general form: one block a (row, head), any width to 256, any page size.  Each warp walks every fourth key in increasing order
+// Two forms.  Heads of 64 or 128 in pages of whole 16s run on the matrix instruction (attention_pages_mma.cuh): queries of either type
+// over eight bits, bfloat16 over bfloat16.  The general form takes any width to 256, any page size and any types, one block a
+// (row, head): each warp walks every fourth key in increasing order
 // with a running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone.
-#include "e4m3.cuh"
-#include <cuda_fp16.h>
-#include <math.h>
+#include "attention_pages_mma.cuh"
 
 namespace {
 constexpr int WARPS = 4;
 constexpr int MAX_PER_LANE = 8;     // widths up to 256
 
-struct Rows {                       // whose rows these are and where their keys lie
-    const int* row_start;
-    const int* row_count;
-    const int* history;
-    const int* tables;              // [requests, table_stride]
-    int table_stride, total_rows, pages, page_size, window;
-    const unsigned* tree;           // [rows, tree_words] or null
-    int tree_words;
-};
+using mma_pages::Rows;
 
 struct E4m3 {};                     // the cache's type: codes, exponents beside them
 
@@ -126,19 +118,105 @@ attention_pages_kernel(const QT* __restrict__ q, const void* __restrict__ cache,
         orow[d] = from_float<QT>(ll == 0.0f ? 0.0f : o / ll);
     }
 }
+
+int multiprocessors() {
+    static const int n = [] {
+        int dev = 0, v = 0;
+        return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+    }();
+    return n;
+}
+
+// How the form on the matrix instruction cuts a call up; `row_warps` 0: it does not take these sizes.
+struct FewPlan {
+    int row_warps = 0, row_tiles = 0, splits = 1;
+};
+
+FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads, int head_dim, int page_size,
+                 int window) {
+    FewPlan p;
+    const bool types = cache_dtype == LLMX_E4M3 || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
+    if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16) return p;
+    const long long pairs = (long long)max_rows * (heads / kv_heads);
+    p.row_warps = pairs <= 16 ? 1 : pairs <= 32 ? 2 : 4;
+    const long long tiles = (pairs + 16 * p.row_warps - 1) / (16 * p.row_warps);
+    // Enough ranges of keys that two blocks find an SM each, and no range of less than two tiles a warp.
+    const long long blocks = tiles * kv_heads * requests;
+    const int keys = window > 0 ? (int)min((long long)max_context, (long long)window + max_rows) : max_context;
+    const int runs = mma_pages::WARPS / p.row_warps;
+    const long long ranges = min(2ll * multiprocessors() / max(blocks, 1ll), (long long)(keys / (2 * mma_pages::TILE * runs)));
+    p.splits = (int)max(1ll, min(ranges, 64ll));
+    if (tiles * p.splits >= (1ll << 31)) p.row_warps = 0;
+    p.row_tiles = (int)tiles;
+    return p;
+}
+
+template <typename QT, bool EIGHT, int D, int RW>
+int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exponents, void* out, float* partial, const Rows& a, int requests,
+             int max_rows, int heads, int kv_heads, float scale, cudaStream_t stream) {
+    using namespace mma_pages;
+    auto kernel = few_rows_kernel<QT, EIGHT, D, RW>;
+    constexpr int ring = (WARPS / RW) * Shape<EIGHT, D>::STAGES * Shape<EIGHT, D>::STAGE, states = WARPS * 16 * (D + PART) * 4;
+    LLMX_ALLOW_SMEM(few_rows_kernel<QT, EIGHT, D, RW>);
+    launch_kernel(kernel, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)kv_heads, (unsigned)requests), dim3(WARPS * 32),
+                  (size_t)(ring > states ? ring : states), stream, (const QT*)q, (const uint8_t*)cache, (const uint8_t*)exponents, (QT*)out, partial, a, heads,
+                  kv_heads, p.splits, scale * 1.4426950408889634f);
+    if (const int e = launch_status()) return e;
+    if (p.splits > 1) {
+        const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
+        launch_kernel(few_rows_merge_kernel<QT, EIGHT, D>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, (const float*)partial,
+                      (QT*)out, a, heads, p.splits);
+    }
+    return launch_status();
+}
 }  // namespace
 
+// The bytes that `workspace` needs.
+LLMX_EXPORT long long llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int requests, int total_rows, int max_rows, int max_context,
+                                                     int heads, int kv_heads, int head_dim, int page_size, int window) {
+    if (requests <= 0 || total_rows <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
+    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
+    return p.splits > 1 ? (long long)total_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4 : 0;
+}
+
 // q/out [total_rows, heads, head_dim] of `q_dtype`; the cache [pages, 2, kv_heads, page_size, head_dim] of `cache_dtype`, with `exponents`
-// [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  No request brings more than `max_rows` rows.  Rows that no request names
-// are left as they are.
+// [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  No request brings more than `max_rows` rows, none has more than `max_context`
+// keys (those only choose the form).  Rows that no request names are left as they are.
 LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cache, const void* exponents, int cache_dtype, void* out,
                                      const int* row_start, const int* row_count, const int* history, const int* tables, int table_stride,
-                                     const void* tree, int tree_words, int requests, int total_rows, int max_rows, int pages, int heads,
-                                     int kv_heads, int head_dim, int page_size, int window, float scale, cudaStream_t stream) {
+                                     const void* tree, int tree_words, int requests, int total_rows, int max_rows, int max_context, int pages,
+                                     int heads, int kv_heads, int head_dim, int page_size, int window, float scale, void* workspace,
+                                     long long workspace_bytes, cudaStream_t stream) {
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
         return LLMX_ERR_UNSUPPORTED;
     const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words};
+    if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
+    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
+    if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) && kv_heads <= 65535) {
+        if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
+                             workspace_bytes < (long long)total_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4))
+            return LLMX_ERR_BAD_ARGUMENT;
+#define LLMX_FEW(QT, EIGHT, D, RW) \
+    return few_rows<QT, EIGHT, D, RW>(p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale, stream)
+#define LLMX_FEW_ROWS(QT, EIGHT, D)                        \
+    do {                                                   \
+        if (p.row_warps == 1) LLMX_FEW(QT, EIGHT, D, 1);   \
+        if (p.row_warps == 2) LLMX_FEW(QT, EIGHT, D, 2);   \
+        LLMX_FEW(QT, EIGHT, D, 4);                         \
+    } while (0)
+#define LLMX_FEW_WIDTH(QT, EIGHT)                          \
+    do {                                                   \
+        if (head_dim == 128) LLMX_FEW_ROWS(QT, EIGHT, 128); \
+        LLMX_FEW_ROWS(QT, EIGHT, 64);                      \
+    } while (0)
+        if (cache_dtype == LLMX_BF16) LLMX_FEW_WIDTH(__nv_bfloat16, false);
+        if (q_dtype == LLMX_BF16) LLMX_FEW_WIDTH(__nv_bfloat16, true);
+        LLMX_FEW_WIDTH(float, true);
+#undef LLMX_FEW
+#undef LLMX_FEW_ROWS
+#undef LLMX_FEW_WIDTH
+    }
     const size_t shmem = (size_t)WARPS * (head_dim + 2) * sizeof(float);
     const dim3 grid((unsigned)max_rows, (unsigned)heads, (unsigned)requests);
 #define LLMX_PAGES(QT, KVT)                                                                                                               \

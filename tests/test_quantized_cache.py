@@ -90,6 +90,10 @@ REFUSED = [
     ("block tables", dict(block_tables=torch.zeros(2, 3))),
     ("block tables", dict(block_tables=torch.zeros(3, 2, dtype=torch.int32).T)),
     ("bounds", dict(max_rows=-1)),
+    ("bounds", dict(max_context=-1)),
+    ("scale above 0", dict(scale=0.0)),
+    ("scale above 0", dict(scale=-1.0)),
+    ("scale above 0", dict(scale=float("nan"))),
     ("CUDA tensors", dict()),
 ]
 
