@@ -40,7 +40,7 @@ attention_pages_kernel(const QT* __restrict__ q, const void* __restrict__ cache,
     const int i = blockIdx.x, h = blockIdx.y, r = blockIdx.z;
     const int count = a.row_count[r], history = max(a.history[r], 0);
     const int row = a.row_start[r] + i;
-    if (i >= count || row < 0 || row >= a.total_rows) return;
+    if (i >= count || count > a.max_rows || row < 0 || row >= a.total_rows) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = h / (heads / kv_heads);
     const long long pos = (long long)history + i;
@@ -172,16 +172,18 @@ int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exp
 }  // namespace
 
 // The bytes that `workspace` needs.
-LLMX_EXPORT long long llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int requests, int total_rows, int max_rows, int max_context,
-                                                     int heads, int kv_heads, int head_dim, int page_size, int window) {
-    if (requests <= 0 || total_rows <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
+LLMX_EXPORT int llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads,
+                                               int head_dim, int page_size, int window, long long* bytes) {
+    *bytes = 0;
+    if (requests <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    return p.splits > 1 ? (long long)total_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4 : 0;
+    if (p.splits > 1) *bytes = (long long)requests * max_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4;
+    return 0;
 }
 
 // q/out [total_rows, heads, head_dim] of `q_dtype`; the cache [pages, 2, kv_heads, page_size, head_dim] of `cache_dtype`, with `exponents`
-// [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  No request brings more than `max_rows` rows, none has more than `max_context`
-// keys (those only choose the form).  Rows that no request names are left as they are.
+// [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  Requests of more than `max_rows` rows are left out; none has more than
+// `max_context` keys (which only chooses the form).  Rows that no request names are left as they are.
 LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cache, const void* exponents, int cache_dtype, void* out,
                                      const int* row_start, const int* row_count, const int* history, const int* tables, int table_stride,
                                      const void* tree, int tree_words, int requests, int total_rows, int max_rows, int max_context, int pages,
@@ -190,12 +192,12 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
         return LLMX_ERR_UNSUPPORTED;
-    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words};
+    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words, max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
     if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) && kv_heads <= 65535) {
         if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
-                             workspace_bytes < (long long)total_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4))
+                             workspace_bytes < (long long)requests * max_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4))
             return LLMX_ERR_BAD_ARGUMENT;
 #define LLMX_FEW(QT, EIGHT, D, RW) \
     return few_rows<QT, EIGHT, D, RW>(p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale, stream)

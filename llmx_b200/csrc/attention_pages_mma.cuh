@@ -36,6 +36,7 @@ struct Rows {                        // whose rows these are and where their key
     int table_stride, total_rows, pages, page_size, window;
     const unsigned* tree;            // [rows, tree_words] or null
     int tree_words;
+    int max_rows;                    // the most rows of a request of this call; one with more is another's
 };
 
 template <bool EIGHT, int D>
@@ -128,7 +129,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
     const int ratio = heads / kv_heads;
     const int count = a.row_count[r], history = min(max(a.history[r], 0), MOST_KEYS), start = a.row_start[r];
     const int first = row_tile * (16 * RW);                      // the tile's first (row, head) pair
-    if (start < 0 || start > a.total_rows) return;
+    if (count > a.max_rows || start < 0 || start > a.total_rows) return;
     const int pairs = min(count, a.total_rows - start) * ratio;
     if (first >= pairs) return;
     const int first_row = first / ratio, last_row = (min(first + 16 * RW, pairs) - 1) / ratio;
@@ -489,7 +490,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
         }
         const size_t at = (size_t)(start + pair / ratio) * heads + kv * ratio + pair % ratio;
         if (splits > 1) {
-            float* to_row = partial + (at * splits + split) * ROWF;
+            float* to_row = partial + ((((size_t)r * a.max_rows + pair / ratio) * heads + kv * ratio + pair % ratio) * splits + split) * ROWF;
             *reinterpret_cast<float4*>(to_row + d) = acc;
             if (d == 0) *reinterpret_cast<float4*>(to_row + D) = make_float4(t, p, l, 0.0f);
         } else {
@@ -509,9 +510,9 @@ few_rows_merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, R
     const int r = blockIdx.y, count = a.row_count[r], start = a.row_start[r];
     const long long item = (long long)blockIdx.x * EACH + threadIdx.x / LANES;
     const int row = (int)(item / heads), d = 4 * (threadIdx.x % LANES);
-    if (start < 0 || row >= count || start + (long long)row >= a.total_rows) return;
+    if (count > a.max_rows || start < 0 || row >= count || start + (long long)row >= a.total_rows) return;
     const size_t at = (size_t)(start + row) * heads + item % heads;
-    const float* base = partial + at * splits * ROWF;
+    const float* base = partial + (((size_t)r * a.max_rows + row) * heads + item % heads) * splits * ROWF;
     float t = -INFINITY, p = -INFINITY;
     for (int n = 0; n < splits; ++n) {
         t = fmaxf(t, base[n * ROWF + D]);

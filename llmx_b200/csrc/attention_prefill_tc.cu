@@ -530,7 +530,7 @@ attn_prefill_merge_kernel(const float* __restrict__ partial, __nv_bfloat16* __re
     float l = 0.0f;
     for (int s = 0; s < key_splits; ++s) {
         const float ls = base[s * PART + D + 1];
-        if (ls > 0.0f) {                      // a range none of whose keys reached the row left its output unwritten
+        if (ls != 0.0f) {                     // a range none of whose keys reached the row left its output unwritten
             const float w = exp2f(base[s * PART + D] - m);
             const float4 o = *reinterpret_cast<const float4*>(base + s * PART + 4 * lane);
             acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y);

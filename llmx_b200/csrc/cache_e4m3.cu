@@ -69,6 +69,92 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     }
 }
 
+constexpr int EXPANDED = 16;         // slots of an expanded page
+
+// Requests' keys and values as bfloat16 pages of 16 slots, for a kernel that reads those: the requests of more than `rows_over` rows, one
+// after another without gaps, a block a page.  `out_table` names a request's pages, `out_count` has its rows (none for the requests
+// that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value.
+// A value row that is no numbers comes as zeros with its key as NaN: the attention's mask then keeps it from the rows that do
+// not see it (a weight of zero would not), and makes NaN of those that do, as it has to.
+__global__ void __launch_bounds__(256)
+expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ row_count,
+              const int* __restrict__ history, const int* __restrict__ tables, int table_stride, int requests, int rows_over, int window, int pages,
+              int kv_heads, int head_dim, int page_size, __nv_bfloat16* __restrict__ out, int* __restrict__ out_table, int out_stride,
+              int* __restrict__ out_count, int* __restrict__ out_list) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ int owner, page_of_owner;
+    if (threadIdx.x == 0) owner = -1;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int r = threadIdx.x; r < requests; r += blockDim.x) {
+            out_list[r] = r;
+            out_count[r] = row_count[r] > rows_over ? row_count[r] : 0;
+        }
+    if (threadIdx.x < 32) {
+        const int f = blockIdx.x;
+        int before = 0;
+        for (int r0 = 0; r0 < requests && before <= f; r0 += 32) {
+            const int r = r0 + threadIdx.x;
+            int n = 0, first = 0;
+            if (r < requests && row_count[r] > rows_over) {
+                const int keys = history[r] + row_count[r];
+                // The reader starts at a whole stage of 128 keys.
+                first = window > 0 ? max(0, history[r] - window + 1) / 128 * (128 / EXPANDED) : 0;
+                n = max(0, min((keys + EXPANDED - 1) / EXPANDED, out_stride) - first);
+            }
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if ((int)threadIdx.x >= o) upto += x;
+            }
+            if (f >= before + upto - n && f < before + upto) owner = r, page_of_owner = first + f - (before + upto - n);
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    __syncthreads();
+    const int r = owner, j = page_of_owner;
+    if (r < 0) return;
+    if (threadIdx.x == 0) out_table[(size_t)r * out_stride + j] = blockIdx.x;
+    const int keys = min(history[r] + row_count[r], table_stride * page_size);
+    const int pieces = head_dim / 16;
+    const int* table = tables + (size_t)r * table_stride;
+    const size_t plane = (size_t)kv_heads * page_size;
+    for (int x = threadIdx.x; x < 2 * kv_heads * EXPANDED * pieces; x += blockDim.x) {
+        const int piece = x % pieces, slot = x / pieces % EXPANDED, head = x / (pieces * EXPANDED);      // head: plane * kv_heads + g
+        const int t = j * EXPANDED + slot;
+        const int page = t < keys ? table[t / page_size] : -1;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (page >= 0 && page < pages) {
+            const size_t at = ((size_t)page * 2 * kv_heads + head) * page_size + t % page_size;
+            const unsigned byte = exponents[at];
+            const bool key = head < kv_heads;
+            const bool bad = byte == e4m3::NOT_NUMBERS || (key && exponents[at + plane] == e4m3::NOT_NUMBERS);
+            if (bad) {
+                if (key) lo = hi = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u);
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4*>(codes + at * head_dim + piece * 16);
+                const float f = e4m3::up(byte);
+                auto four = [&](unsigned c, unsigned& a, unsigned& b) {
+                    const unsigned h0 = e4m3::halves((unsigned short)(c & 0xffffu)), h1 = e4m3::halves((unsigned short)(c >> 16));
+                    const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                    const __nv_bfloat162 y0 = __floats2bfloat162_rn(x0.x * f, x0.y * f), y1 = __floats2bfloat162_rn(x1.x * f, x1.y * f);
+                    a = *reinterpret_cast<const unsigned*>(&y0);
+                    b = *reinterpret_cast<const unsigned*>(&y1);
+                };
+                four(w.x, lo.x, lo.y);
+                four(w.y, lo.z, lo.w);
+                four(w.z, hi.x, hi.y);
+                four(w.w, hi.z, hi.w);
+            }
+        }
+        uint4* to = reinterpret_cast<uint4*>(out + (((size_t)blockIdx.x * 2 * kv_heads + head) * EXPANDED + slot) * head_dim + piece * 16);
+        to[0] = lo;
+        to[1] = hi;
+    }
+}
+
 }  // namespace
 
 // Row r's keys and values, [rows, kv_heads, head_dim] of `dtype` with rows `k_stride` and `v_stride` values apart, go to slots[r]
@@ -104,5 +190,18 @@ LLMX_EXPORT int llmx_dequantize_pages(const void* codes, const void* exponents, 
     else if (dtype == LLMX_F32) LLMX_DEQUANTIZE(float);
     else return LLMX_ERR_BAD_ARGUMENT;
 #undef LLMX_DEQUANTIZE
+    return launch_status();
+}
+
+// Requests of more than `rows_over` rows, their keys and values as bfloat16 pages out[0 .. capacity) of [2, kv_heads, 16, head_dim]: all of
+// them, or under a window those from the stage of 128 that the first row's window starts in.  `capacity` pages must hold them.
+LLMX_EXPORT int llmx_expand_requests(const void* codes, const void* exponents, const int* row_count, const int* history, const int* tables,
+                                     int table_stride, int requests, int rows_over, int window, int pages, int kv_heads, int head_dim, int page_size,
+                                     void* out, int capacity, int* out_table, int out_stride, int* out_count, int* out_list, cudaStream_t stream) {
+    if (requests <= 0 || capacity <= 0) return 0;
+    if (kv_heads <= 0 || head_dim <= 0 || head_dim % 16 || page_size <= 0 || (((uintptr_t)codes | (uintptr_t)out) & 15)) return LLMX_ERR_UNSUPPORTED;
+    launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(256), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_count, history,
+                  tables, table_stride, requests, rows_over, window, pages, kv_heads, head_dim, page_size, (__nv_bfloat16*)out, out_table, out_stride,
+                  out_count, out_list);
     return launch_status();
 }

@@ -29,7 +29,7 @@ extern "C" {
 #define LLMX_RT_VERSION 2
 #define LLMX_MAX_GROUPS 32
 
-enum { LLMX_DT_F32 = 0, LLMX_DT_BF16 = 1 };
+enum { LLMX_DT_F32 = 0, LLMX_DT_BF16 = 1, LLMX_DT_E4M3 = 2 };   // E4M3: of a cache alone
 enum { LLMX_RT_ERR_BAD_ARGUMENT = 10001, LLMX_RT_ERR_UNSUPPORTED = 10002, LLMX_RT_ERR_TOO_LARGE = 10004,
        LLMX_RT_ERR_UNBOUND = 10010, LLMX_RT_ERR_WORKSPACE = 10011, LLMX_RT_ERR_CALLBACK = 10012, LLMX_RT_ERR_INJECTED = 10013 };
 
@@ -206,6 +206,32 @@ size_t llmx_paged_attention_workspace(const llmx_step*, int entry, int heads, in
 int llmx_decode_from_qkv(const llmx_step*, const float* qkv, int entry, const float* q_weight, const float* k_weight,
                          float eps, const float* cos, const float* sin, int rot_half, void* out, int heads, int kv_heads,
                          int head_dim, int window, float scale);
+
+// Attention of requests' rows over pages of any cache type (llmx_attention_pages, attention_pages.cu, has the formulas): over keys and
+// values in eight bits, and for rows that are drafted tokens.  Requests of many rows over eight bits (heads of 128, bfloat16
+// queries, no tree) have their pages expanded and run the tcgen05 kernel.
+typedef struct llmx_pages_call {
+    const void* q;                    // [total_rows, heads, head_dim] of q_dtype, like out
+    void* out;
+    const void* cache;                // [pages, 2, kv_heads, page_size, head_dim]
+    const void* exponents;            // [pages, 2, kv_heads, page_size] beside codes
+    const int* row_start;             // [requests], on the device like all that follows
+    const int* row_count;
+    const int* history;
+    const int* tables;                // [requests, table_stride]
+    const void* tree;                 // [total_rows, tree_words] words of bits, or null
+    int q_dtype, cache_dtype, table_stride, tree_words, requests, total_rows;
+    int max_rows, max_context;        // the most rows a request brings, the most keys one has
+    long long total_context;          // the most keys of all requests together (0: requests * max_context)
+    int pages, heads, kv_heads, head_dim, page_size, window;
+    float scale;
+    void* workspace;                  // llmx_pages_workspace bytes, 256-byte aligned
+    size_t workspace_bytes;
+    int* error_word;
+    void* stream;
+} llmx_pages_call;
+int llmx_pages_attention(const llmx_pages_call*);
+size_t llmx_pages_workspace(const llmx_pages_call*);      // notes unbound kernels, as llmx_part_workspace does
 
 // ---- the model ------------------------------------------------------------------------------------------------
 typedef struct llmx_layer_step { int block, cache_entry, write_cache; } llmx_layer_step;   // cache_entry < 0: none

@@ -44,6 +44,11 @@ typedef cudaStream_t S;
     X(llmx_gemm_plain, (const void*, int, const void*, int, float*, int, int, int, int, S))                               \
     X(llmx_attention_plain, (const void*, int, const void*, int, void*, const int*, const int*, const int*, int, int,     \
                              int, int, int, int, int, float, S))                                                          \
+    X(llmx_attention_pages, (const void*, int, const void*, const void*, int, void*, const int*, const int*, const int*, const int*,  \
+                             int, const void*, int, int, int, int, int, int, int, int, int, int, int, float, void*, long long, S))    \
+    X(llmx_attention_pages_workspace, (int, int, int, int, int, int, int, int, int, int, long long*))                         \
+    X(llmx_expand_requests, (const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, int, int,    \
+                             void*, int, int*, int, int*, int*, S))                                                       \
     X(llmx_gemm_tc_weight_map, (void*, const void*, int, int))                                                            \
     X(llmx_gemm_tc_weight_map_box, (void*, const void*, int, int, int))                                                   \
     X(llmx_gemm_tc, (const void*, const void*, float*, int, int, int, int, int, int, int, int*, S))                       \
@@ -416,6 +421,70 @@ bool tensor_core_prefill(int heads, int kv_heads, int head_dim, int page_size) {
     return head_dim == 128 && page_size == ATTN_PAGE && heads % kv_heads == 0 && heads / kv_heads <= 16;
 }
 
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention over pages of any cache type.
+// ---------------------------------------------------------------------------------------------------------------
+namespace {
+constexpr int FEW_PAIRS = 64;             // (row, head) pairs of a group up to which a request's rows read the pages as they are
+constexpr int EXPANDED_PAGE = 16;
+
+int pages_attention(Ctx& c, const llmx_pages_call& p) {
+    if (p.requests <= 0 || p.total_rows <= 0 || p.max_rows <= 0) return 0;
+    const int ratio = p.heads / p.kv_heads;
+    auto few = [&](int max_rows) {
+        if (!kern.llmx_attention_pages_workspace) {
+            note_missing("llmx_attention_pages");
+            if (!c.dry) c.status = fail(LLMX_RT_ERR_UNBOUND, "kernel llmx_attention_pages is not bound (its library was not loaded)");
+            return;
+        }
+        long long room = 0;
+        kern.llmx_attention_pages_workspace(p.q_dtype, p.cache_dtype, p.requests, max_rows, p.max_context, p.heads, p.kv_heads, p.head_dim, p.page_size,
+                                            p.window, &room);
+        void* at = room ? c.alloc((size_t)room) : nullptr;
+        CALL(c, llmx_attention_pages, room ? 2 : 1, p.q, p.q_dtype, p.cache, p.exponents, p.cache_dtype, p.out, p.row_start, p.row_count, p.history,
+             p.tables, p.table_stride, p.tree, p.tree_words, p.requests, p.total_rows, max_rows, p.max_context, p.pages, p.heads, p.kv_heads,
+             p.head_dim, p.page_size, p.window, p.scale, at, room, c.stream);
+    };
+    // Many rows: their keys and values become bfloat16 once (exact), and the prompt kernel runs over them.  Its tiles of 128 pairs are
+    // half empty below FEW_PAIRS.
+    const bool many = p.cache_dtype == LLMX_DT_E4M3 && p.q_dtype == LLMX_DT_BF16 && !p.tree && (long long)p.max_rows * ratio > FEW_PAIRS &&
+                      tensor_core_prefill(p.heads, p.kv_heads, p.head_dim, ATTN_PAGE) &&
+                      !(((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.cache) & 15);
+    if (!many) {
+        few(p.max_rows);
+        return c.status;
+    }
+    const int rows_few = std::max(FEW_PAIRS / ratio, 0);
+    const long long most = p.window > 0 ? std::min((long long)p.max_context, (long long)p.window + p.max_rows + 128) : p.max_context;
+    long long capacity = (long long)p.requests * (most / EXPANDED_PAGE + 2);
+    if (p.total_context > 0) capacity = std::min(capacity, p.total_context / EXPANDED_PAGE + 2ll * p.requests);
+    if (capacity >= (1ll << 31)) return c.status = fail(LLMX_RT_ERR_BAD_ARGUMENT, "attention over pages: more keys than 2^31 pages hold");
+    const int stride = p.max_context / EXPANDED_PAGE + 9;
+    void* expanded = c.alloc((size_t)capacity * 2 * p.kv_heads * EXPANDED_PAGE * p.head_dim * 2);
+    int* table = c.alloc_n<int>((size_t)p.requests * stride);
+    int* count = c.alloc_n<int>(p.requests);
+    int* list = c.alloc_n<int>(p.requests);
+    CALL(c, llmx_expand_requests, 1, p.cache, p.exponents, p.row_count, p.history, p.tables, p.table_stride, p.requests, rows_few, p.window, p.pages,
+         p.kv_heads, p.head_dim, p.page_size, expanded, (int)capacity, table, stride, count, list, c.stream);
+    int tiles = 2, splits = 1;
+    prefill_shape(p.requests, p.kv_heads, ratio, p.max_rows, p.max_context, p.window, sms(), &tiles, &splits);
+    float* partial = splits > 1 ? c.alloc_n<float>((size_t)p.total_rows * p.heads * splits * PREFILL_PART) : nullptr;
+    alignas(64) unsigned char map[128];
+    if (c.dry) {
+        if (!kern.llmx_attn_prefill_tc_cache_map) note_missing("llmx_attn_prefill_tc_cache_map");
+    } else if (!c.status) {
+        if (!kern.llmx_attn_prefill_tc_cache_map) return c.status = fail(LLMX_RT_ERR_UNBOUND, "kernel llmx_attn_prefill_tc_cache_map is not bound");
+        if (int err = kern.llmx_attn_prefill_tc_cache_map(map, expanded, capacity, p.kv_heads, EXPANDED_PAGE, p.head_dim))
+            return c.status = fail(err, "attention over pages: the expanded pages' map could not be made");
+    }
+    CALL(c, llmx_attn_prefill_tc, splits > 1 ? 2 : 1, (const void*)map, p.q, p.out, p.total_rows, (const int*)list, p.requests, p.row_start,
+         (const int*)count, p.history, (const int*)table, stride, p.heads, p.kv_heads, p.head_dim, EXPANDED_PAGE, p.window, p.scale, p.max_rows, tiles,
+         splits, partial, p.error_word, c.stream);
+    if (p.requests > 1 && rows_few > 0) few(std::min(p.max_rows, rows_few));
+    return c.status;
+}
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1384,6 +1453,33 @@ LLMX_API int llmx_decode_from_qkv(const llmx_step* s, const float* qkv, int entr
     Ctx c(s, false);
     const bool ran = a.from_qkv(c, qkv, *e, out, s->rows, c.meta(s->slots[e->group]), e->group);
     return c.status ? c.status : ran ? 0 : -1;
+}
+
+// ---- attention over pages of any cache type ----
+namespace {
+bool good_call(const llmx_pages_call* p) {
+    return p && p->requests >= 0 && p->total_rows >= 0 && p->max_rows >= 0 && p->max_context >= 0 && p->heads > 0 && p->kv_heads > 0 &&
+           p->heads % p->kv_heads == 0 && p->head_dim > 0 && p->page_size > 0 && p->table_stride >= 0 && p->window >= 0 && p->scale > 0.0f;
+}
+llmx_step step_of(const llmx_pages_call& p) {
+    llmx_step s = {};
+    s.workspace = p.workspace, s.workspace_bytes = p.workspace_bytes, s.error_word = p.error_word, s.stream = p.stream;
+    return s;
+}
+}  // namespace
+LLMX_API size_t llmx_pages_workspace(const llmx_pages_call* p) {
+    if (!good_call(p)) return 0;
+    const llmx_step s = step_of(*p);
+    Ctx c(&s, true);
+    pages_attention(c, *p);
+    return c.peak ? c.peak + 256 : 0;
+}
+LLMX_API int llmx_pages_attention(const llmx_pages_call* p) {
+    if (!good_call(p)) return fail(LLMX_RT_ERR_BAD_ARGUMENT, "attention over pages: sizes that do not fit each other");
+    const llmx_step s = step_of(*p);
+    Ctx c(&s, false);
+    pages_attention(c, *p);
+    return c.status;
 }
 
 // ---- the model ----

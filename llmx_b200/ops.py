@@ -17,6 +17,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
+from . import runtime
 from .csrc import build as _build
 
 F32, BF16, E4M3 = 0, 1, 2            # E4M3: of a cache alone (`QuantizedPages`)
@@ -154,9 +155,6 @@ _SIGNATURES = {
     ("latent_prompt_tc", "llmx_latent_prompt"): [_p, _i, _p, _i, _p, _p, _i, _p, _i, _i, _f, _p, _i, _i, _i, _i, _i, _f, _p, _p],
     ("cache_e4m3", "llmx_quantize_kv"): [_p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
     ("cache_e4m3", "llmx_dequantize_pages"): [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
-    ("attention_pages", "llmx_attention_pages"): [_p, _i, _p, _p, _i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p,
-                                                  ctypes.c_longlong, _p],
-    ("attention_pages", "llmx_attention_pages_workspace"): [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i],
     ("gemm_plain", "llmx_gemm_plain"): [_p, _i, _p, _i, _p, _i, _i, _i, _i, _p],
     ("attention_plain", "llmx_attention_plain"): [_p, _i, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _p],
 }
@@ -179,7 +177,7 @@ def _fn(lib: str, name: str):
     if f is None:
         f = getattr(_build.load(lib), name)
         f.argtypes = _SIGNATURES[key]
-        f.restype = ctypes.c_longlong if name.endswith("_workspace") else ctypes.c_int
+        f.restype = ctypes.c_int
         _fns[key] = f
     if _timed_calls is None:
         return f
@@ -1401,22 +1399,23 @@ def _attention_pages(what: str, q, cache, out, row_start, row_count, history, bl
           f"{what}: bounds of at least 0, a window of at least 1, a scale above 0")
     q_code, code = _code(q), E4M3 if eight else _code(stored)
     _same_device(what, q.device, out, stored, row_start, row_count, history, block_tables, tree)
-    _launched(q.device, lambda stream: _run_attention_pages(what, stream, q, q_code, cache, stored, code, out, row_start, row_count, history, block_tables,
-                                                            tree, requests, int(max_rows), int(max_context), heads, kv_heads, head_dim, int(window or 0),
-                                                            float(scale)))
+    call = runtime.PagesCall(q.data_ptr(), out.data_ptr(), stored.data_ptr(), cache.exponents.data_ptr() if eight else None, row_start.data_ptr(),
+                             row_count.data_ptr(), history.data_ptr(), block_tables.data_ptr(), None if tree is None else tree.data_ptr(), q_code, code,
+                             block_tables.shape[1], 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), int(max_context), 0,
+                             stored.shape[0], heads, kv_heads, head_dim, stored.shape[3], int(window or 0), float(scale))
+    _launched(q.device, lambda stream: _pages_attention(what, call, q.device, stream))
     return out
 
 
-def _run_attention_pages(what, stream, q, q_code, cache, stored, code, out, row_start, row_count, history, block_tables, tree, requests, max_rows,
-                         max_context, heads, kv_heads, head_dim, window, scale):
-    rows, page_size = q.shape[0], stored.shape[3]
-    room = _fn("attention_pages", "llmx_attention_pages_workspace")(
-        q_code, code, requests, rows, max_rows, max_context, heads, kv_heads, head_dim, page_size, window)
-    workspace = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
-    _check(_fn("attention_pages", "llmx_attention_pages")(
-        _ptr(q), q_code, _ptr(stored), _ptr(cache.exponents if code == E4M3 else None), code, _ptr(out), _ptr(row_start), _ptr(row_count), _ptr(history),
-        _ptr(block_tables), block_tables.shape[1], _ptr(tree), 0 if tree is None else tree.shape[1], requests, rows, max_rows, max_context,
-        stored.shape[0], heads, kv_heads, head_dim, page_size, window, scale, _ptr(workspace), room, stream), what)
+def _pages_attention(what: str, call, device: torch.device, stream) -> None:
+    lib = runtime.lib()
+    room = lib.llmx_pages_workspace(call)
+    if runtime.bind_missing():
+        room = lib.llmx_pages_workspace(call)
+    workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    call.workspace, call.workspace_bytes = None if workspace is None else workspace.data_ptr(), room
+    call.error_word, call.stream = runtime.error_word(device).data_ptr(), stream
+    runtime.check(lib.llmx_pages_attention(call), what)
 
 
 def attention_quantized(q: torch.Tensor, cache: QuantizedPages, out: torch.Tensor, row_start: torch.Tensor, row_count: torch.Tensor,

@@ -21,7 +21,7 @@ import torch
 
 from .csrc import build as _build
 
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 MAX_GROUPS = 32
 COUNTERS = 65536
 FLAG_INVARIANT = 1
@@ -63,7 +63,15 @@ class LayerStepStruct(ctypes.Structure):
     _fields_ = [("block", _i), ("cache_entry", _i), ("write_cache", _i)]
 
 
+class PagesCall(ctypes.Structure):
+    _fields_ = [("q", _p), ("out", _p), ("cache", _p), ("exponents", _p), ("row_start", _p), ("row_count", _p), ("history", _p), ("tables", _p),
+                ("tree", _p), ("q_dtype", _i), ("cache_dtype", _i), ("table_stride", _i), ("tree_words", _i), ("requests", _i), ("total_rows", _i),
+                ("max_rows", _i), ("max_context", _i), ("total_context", _ll), ("pages", _i), ("heads", _i), ("kv_heads", _i), ("head_dim", _i),
+                ("page_size", _i), ("window", _i), ("scale", _f), ("workspace", _p), ("workspace_bytes", _sz), ("error_word", _p), ("stream", _p)]
+
+
 _SP = ctypes.POINTER(StepStruct)
+_PCP = ctypes.POINTER(PagesCall)
 _SIGNATURES = {
     "llmx_rt_version": (_i, []),
     "llmx_rt_bind": (_i, [ctypes.c_char_p, _p]),
@@ -120,6 +128,8 @@ _SIGNATURES = {
     "llmx_paged_attention": (_i, [_SP, _p, _i, _i, _p, _i, _i, _i, _i, _f]),
     "llmx_paged_attention_workspace": (_sz, [_SP, _i, _i, _i, _i, _i]),
     "llmx_decode_from_qkv": (_i, [_SP, _p, _i, _p, _p, _f, _p, _p, _i, _p, _i, _i, _i, _i, _f]),
+    "llmx_pages_attention": (_i, [_PCP]),
+    "llmx_pages_workspace": (_sz, [_PCP]),
     "llmx_model_create": (_p, [_p, _p, _i, _p, _i, _p, _i, _i]),
     "llmx_model_destroy": (None, [_p]),
     "llmx_model_workspace": (_sz, [_p, _SP]),
@@ -138,6 +148,8 @@ KERNEL_LIBS: Dict[str, str] = {
     "llmx_attn_decode_qkv": "attention_decode", "llmx_attn_decode_max_clusters": "attention_decode",
     "llmx_attn_prefill_tc_cache_map": "attention_prefill_tc", "llmx_attn_prefill_tc": "attention_prefill_tc",
     "llmx_attn_prefill": "attention_prefill",
+    "llmx_attention_pages": "attention_pages", "llmx_attention_pages_workspace": "attention_pages",
+    "llmx_expand_requests": "cache_e4m3",
     "llmx_sample": "sampling", "llmx_penalize": "sampling",
 }
 
