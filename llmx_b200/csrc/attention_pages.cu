@@ -7,7 +7,7 @@
 // and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key.
 // Query head h reads key/value head h / (heads / kv_heads).  A page that is not in the cache reads as zeros.
 //
-// Two forms.  Heads of 64 or 128 in pages of whole 16s run on the matrix instruction (attention_pages_mma.cuh): queries of either type
+// Two forms.  Heads of 64 or 128 in pages of 16 to 512 slots by 16 run on the matrix instruction (attention_pages_mma.cuh): queries of either type
 // over eight bits, bfloat16 over bfloat16.  The general form takes any width to 256, any page size and any types, one block a
 // (row, head): each warp walks every fourth key in increasing order
 // with a running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone.
@@ -136,7 +136,7 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
                  int window) {
     FewPlan p;
     const bool types = cache_dtype == LLMX_E4M3 || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
-    if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16) return p;
+    if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
     p.row_warps = pairs <= 16 ? 1 : pairs <= 32 ? 2 : 4;
     const long long tiles = (pairs + 16 * p.row_warps - 1) / (16 * p.row_warps);
@@ -192,7 +192,8 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
         return LLMX_ERR_UNSUPPORTED;
-    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words, max_rows};
+    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words,
+                    ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
     if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) && kv_heads <= 65535) {

@@ -14,8 +14,10 @@
 // 32 bits, and their weights, are two halves each.  Over bfloat16 pages queries, keys, values and weights are bfloat16.
 //
 // A row's head axis is walked in an order that lets a lane read its keys in 16-byte pieces: piece 4h + c of a row's bytes belongs to
-// lane c of four, and queries are laid out the same way.  Pieces of rows lie exchanged in shared memory (`place`) so that neither
-// these reads nor the transposing ones of values meet in a bank.
+// lane c of four, and queries are laid out the same way.  A tile's keys are walked in such an order too: column 2c + x of the
+// instruction's j-th eight is key 8c + 2j + x, so that a lane's eight scores a row are of eight keys that follow one another (their
+// exponents are one read).  Pieces of rows lie exchanged in shared memory (`place`) so that neither the reads of keys (rows 2j and
+// 2j + 1 at a time) nor the transposing ones of values (rows 2j, 2j + 1, 8 + 2j, ...) meet in a bank.
 #pragma once
 #include "e4m3.cuh"
 #include <cuda_fp16.h>
@@ -36,6 +38,7 @@ struct Rows {                        // whose rows these are and where their key
     int table_stride, total_rows, pages, page_size, window;
     const unsigned* tree;            // [rows, tree_words] or null
     int tree_words;
+    unsigned run_pages;              // 2^31 / (page_size / 16), rounded up: t / page_size = (t / 16) * run_pages >> 31 for t < 2^30
     int max_rows;                    // the most rows of a request of this call; one with more is another's
 };
 
@@ -53,11 +56,14 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint
 // Where piece `piece` of row `row` lies.  Rows of 64 bytes share a line of 128 by twos.
 template <int ROW>
 __device__ __forceinline__ uint32_t place(int row, int piece) {
-    if constexpr (ROW == 64) return (uint32_t)(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
-    else return (uint32_t)(row * ROW + ((piece ^ (((row & 1) << 2) | ((row >> 1) & 3))) << 4));
+    if constexpr (ROW == 64) return (uint32_t)(row * 64 + ((piece ^ (row >> 3)) << 4));
+    else return (uint32_t)(row * ROW + ((piece ^ (((row & 1) << 2) | (row >> 3))) << 4));
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real) {
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zeros(uint32_t to, const void* from, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -86,6 +92,11 @@ __device__ __forceinline__ float exp2_fast(float x) {        // -inf gives 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     uint32_t r;
@@ -146,35 +157,50 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
     uint8_t* ring = smem + run * (STAGES * S::STAGE);
     const uint32_t ring_at = shared_address(ring);
     // A tile's keys lie in two runs of 16, each within a page.  Lookups are made one tile ahead of the copies.
+    const int runs_a_page = a.page_size >> 4;
+    auto page_of = [&](int sixteenth) { return (int)(((uint64_t)(unsigned)sixteenth * a.run_pages) >> 31); };
     int page_a = -1, page_b = -1;
     auto look_up = [&](int i) {
-        const int t = (from + run + i * RUNS) * TILE;
-        page_a = i < mine ? table[t / a.page_size] : -1;
-        page_b = i < mine && t + 16 < end ? table[(t + 16) / a.page_size] : -1;
+        const int n = 2 * (from + run + i * RUNS);
+        page_a = i < mine ? table[page_of(n)] : -1;
+        page_b = i < mine && (n + 1) * 16 < end ? table[page_of(n + 1)] : -1;
     };
+    constexpr int EACH = TILE * S::PIECES / (32 * RW);           // pieces of a plane for a lane
     auto fetch = [&](int i) {
-        const int t = (from + run + i * RUNS) * TILE;
+        const int n = 2 * (from + run + i * RUNS), t = n * 16;
         const uint32_t stage = ring_at + (i % STAGES) * S::STAGE;
-        const int off_a = t % a.page_size, off_b = (t + 16) % a.page_size;
         const bool in_a = page_a >= 0 && page_a < a.pages, in_b = page_b >= 0 && page_b < a.pages;
-        const size_t row_a = ((size_t)(in_a ? page_a : 0) * 2 * kv_heads + kv) * a.page_size + off_a;
-        const size_t row_b = ((size_t)(in_b ? page_b : 0) * 2 * kv_heads + kv) * a.page_size + off_b;
+        const size_t row_a = ((size_t)(in_a ? page_a : 0) * 2 * kv_heads + kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+        const size_t row_b = ((size_t)(in_b ? page_b : 0) * 2 * kv_heads + kv) * a.page_size + (n + 1 - page_of(n + 1) * runs_a_page) * 16;
         const size_t plane = (size_t)kv_heads * a.page_size;
-        constexpr int EACH = TILE * S::PIECES / (32 * RW);
+        if (in_a && in_b && t >= low && t + TILE <= end) {
+            // A run's rows follow one another, and 512 bytes of them are one warp's copy.
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+            for (int p = 0; p < 2; ++p) {
+                const uint8_t* lower = cache + (row_a + p * plane) * S::ROW + lane * 16;
+                const uint8_t* upper = cache + (row_b + p * plane) * S::ROW + lane * 16 - 16 * S::ROW;
 #pragma unroll
-            for (int j = 0; j < EACH; ++j) {
-                const int piece = (j * RW + rw) * 32 + lane, row = piece / S::PIECES, col = piece % S::PIECES;
-                const bool upper = row >= 16;
-                const bool real = (upper ? in_b : in_a) && t + row < end && t + row >= low;
-                const size_t at = (upper ? row_b + (row - 16) : row_a + row) + p * plane;
-                copy16(stage + p * S::PLANE + place<S::ROW>(row, col), cache + (real ? at * S::ROW + col * 16 : 0), real);
+                for (int j = 0; j < EACH; ++j) {
+                    const int piece = (j * RW + rw) * 32;
+                    copy16(stage + p * S::PLANE + place<S::ROW>((piece + lane) / S::PIECES, (piece + lane) % S::PIECES),
+                           (piece >= 16 * S::PIECES ? upper : lower) + piece * 16);
+                }
             }
+        } else {
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) {
+                    const int piece = (j * RW + rw) * 32 + lane, row = piece / S::PIECES, col = piece % S::PIECES;
+                    const bool upper = row >= 16, real = (upper ? in_b : in_a) && t + row < end && t + row >= low;
+                    const size_t at = (upper ? row_b + (row - 16) : row_a + row) + p * plane;
+                    copy16_or_zeros(stage + p * S::PLANE + place<S::ROW>(row, col), cache + (real ? at * S::ROW + col * 16 : 0), real);
+                }
+        }
         if (EIGHT && rw == 0 && lane < 4) {                      // exponents: keys' 32, values' 32
             const bool upper = lane & 1, real = upper ? in_b : in_a;
             const size_t at = (upper ? row_b : row_a) + (lane >> 1) * plane;
-            copy16(stage + 2 * S::PLANE + (lane >> 1) * TILE + (lane & 1) * 16, exponents + (real ? at : 0), real);
+            copy16_or_zeros(stage + 2 * S::PLANE + (lane >> 1) * TILE + (lane & 1) * 16, exponents + (real ? at : 0), real);
         }
     };
     look_up(0);
@@ -263,7 +289,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
             for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
 #pragma unroll
             for (int h = 0; h < S::PIECES / 4; ++h) {
-                const uint4 k = read16(stage + place<S::ROW>(8 * j + g, 4 * h + c));
+                const uint4 k = read16(stage + place<S::ROW>(8 * (g >> 1) + 2 * j + (g & 1), 4 * h + c));
                 if constexpr (EIGHT) {
                     const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
@@ -278,24 +304,28 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
                 }
             }
         }
-        float2 vn[4];                                            // the values' exponents
+        float vn[8];                                             // the values' exponents; [2j + x]: key 8c + 2j + x
         if constexpr (EIGHT) {
+            uint32_t kb[2], vb[2];
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(kb[0]), "=r"(kb[1]) : "r"(stage + 2 * S::PLANE + 8 * c) : "memory");
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vb[0]), "=r"(vb[1]) : "r"(stage + 2 * S::PLANE + TILE + 8 * c) : "memory");
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                unsigned kb, vb;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=r"(kb) : "r"(stage + 2 * S::PLANE + 8 * j + 2 * c) : "memory");
-                asm volatile("ld.shared.u16 %0, [%1];" : "=r"(vb) : "r"(stage + 2 * S::PLANE + TILE + 8 * j + 2 * c) : "memory");
+            for (int n = 0; n < 8; ++n) {
                 // Keys' powers: 255 becomes an infinity, which makes NaN of its codes' zeros.
-                const float k0 = __uint_as_float((kb & 255u) << 23), k1 = __uint_as_float((kb >> 8) << 23);
-                s[j][0] *= k0; s[j][1] *= k1; s[j][2] *= k0; s[j][3] *= k1;
-                vn[j].x = (vb & 255u) == e4m3::NOT_NUMBERS ? NAN : (float)((int)(vb & 255u) - 127);
-                vn[j].y = (vb >> 8) == e4m3::NOT_NUMBERS ? NAN : (float)((int)(vb >> 8) - 127);
+                const float k = __uint_as_float(__byte_perm(kb[n >> 2], 0, 0x0444 | (n & 3) << 12) >> 1);
+                s[n >> 1][n & 1] *= k;
+                s[n >> 1][2 + (n & 1)] *= k;
+                vn[n] = __uint_as_float(__byte_perm(vb[n >> 2], 0x4B000000u, 0x7440 | (n & 3))) - (8388608.0f + 127.0f);
             }
+            if (__any_sync(0xffffffffu, __vcmpeq4(vb[0], 0xffffffffu) | __vcmpeq4(vb[1], 0xffffffffu)))
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+                    if ((vb[n >> 2] >> (8 * (n & 3)) & 255u) == e4m3::NOT_NUMBERS) vn[n] = NAN;
         }
         // Who sees what.  Tiles that all of the warp's rows see whole are not looked at one by one.
         const int sure = a.tree ? history : min(history + warp_row0 + 1, end);
         const bool whole = t0 + TILE <= sure && t0 + TILE <= end && t0 >= low && (a.window <= 0 || t0 > history + warp_row1 - a.window);
-        unsigned seen[2] = {0xffffu, 0xffffu};                   // bits 2j, 2j + 1: keys 8j + 2c, + 1
+        unsigned seen[2] = {0xffffu, 0xffffu};                   // bit 2j + x: key 8c + 2j + x
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -304,7 +334,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int t = t0 + 8 * j + 2 * c + x;
+                        const int t = t0 + 8 * c + 2 * j + x;
                         bool ok = position[u] >= 0 && t < end && t >= low;
                         if (a.tree) ok = ok && (t < history || (bits[u][(t - history) >> 5] >> ((t - history) & 31) & 1u));
                         else ok = ok && t <= position[u] && (a.window <= 0 || t > position[u] - a.window);
@@ -320,17 +350,17 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
         for (int u = 0; u < 2; ++u) {
             float p = -INFINITY, m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
+                p = max3(p, s[j][2 * u], s[j][2 * u + 1]);
+                if constexpr (EIGHT) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float& z = s[j][2 * u + x];
-                    p = fmaxf(p, z);
-                    if constexpr (EIGHT) {
-                        w[j][2 * u + x] = fmaf(z, factor[u], x ? vn[j].y : vn[j].x);
+                    for (int x = 0; x < 2; ++x) {
+                        w[j][2 * u + x] = fmaf(s[j][2 * u + x], factor[u], vn[2 * j + x]);
                         if (!whole && !(seen[u] >> (2 * j + x) & 1u)) w[j][2 * u + x] = -INFINITY;
-                        m = fmaxf(m, w[j][2 * u + x]);
                     }
+                    m = max3(m, w[j][2 * u], w[j][2 * u + 1]);
                 }
+            }
             p *= factor[u];
             p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 1));
             p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 2));
@@ -382,7 +412,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 #pragma unroll
         for (int piece = 0; piece < S::PIECES; ++piece) {
             uint32_t v[4];
-            read_transposed(v, stage + S::PLANE + place<S::ROW>(lane, piece));
+            read_transposed(v, stage + S::PLANE + place<S::ROW>(8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1), piece));
             if constexpr (EIGHT) {
                 // A register holds values 2g and 2g + 1 of two keys: to the pairs of keys of each.
                 uint32_t even[4], odd[4];
@@ -412,7 +442,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
                     if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            // This lane holds value g of keys 8x + 2c, + 1; outputs are of values 2c, + 1 and rows g, g + 8.
+                            // This lane holds value g of keys 8c + 2x, + 1; outputs are of values 2c, + 1 and rows g, g + 8.
 #pragma unroll
                             for (int y = 0; y < 2; ++y)
                                 for (int cc = 0; cc < 4; ++cc) {
