@@ -129,7 +129,8 @@ int multiprocessors() {
 
 // How the form on the matrix instruction cuts a call up; `row_warps` 0: it does not take these sizes.
 struct FewPlan {
-    int row_warps = 0, row_tiles = 0, splits = 1;
+    int row_warps = 0, blocks = 0;
+    long long bytes(int head_dim) const { return 2ll * blocks * 16 * row_warps * (head_dim + mma_pages::PART) * 4; }      // two states a block
 };
 
 FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads, int head_dim, int page_size,
@@ -139,15 +140,11 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
     p.row_warps = pairs <= 16 ? 1 : pairs <= 32 ? 2 : 4;
-    const long long tiles = (pairs + 16 * p.row_warps - 1) / (16 * p.row_warps);
-    // Enough ranges of keys that two blocks find an SM each, and no range of less than two tiles a warp.
-    const long long blocks = tiles * kv_heads * requests;
-    const int keys = window > 0 ? (int)min((long long)max_context, (long long)window + max_rows) : max_context;
-    const int runs = mma_pages::WARPS / p.row_warps;
-    const long long ranges = min(2ll * multiprocessors() / max(blocks, 1ll), (long long)(keys / (2 * mma_pages::TILE * runs)));
-    p.splits = (int)max(1ll, min(ranges, 64ll));
-    if (tiles * p.splits >= (1ll << 31)) p.row_warps = 0;
-    p.row_tiles = (int)tiles;
+    // Two blocks find an SM each.  The kernel leaves some of them without work where there is too little.
+    const long long items = (pairs + 16 * p.row_warps - 1) / (16 * p.row_warps) * kv_heads * requests;
+    const long long keys = window > 0 ? min((long long)max_context, (long long)window + max_rows) : max_context;
+    const long long tiles = items * (keys / mma_pages::TILE + 2);
+    p.blocks = (int)min(2ll * multiprocessors(), max(items, tiles / 2));
     return p;
 }
 
@@ -155,18 +152,15 @@ template <typename QT, bool EIGHT, int D, int RW>
 int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exponents, void* out, float* partial, const Rows& a, int requests,
              int max_rows, int heads, int kv_heads, float scale, cudaStream_t stream) {
     using namespace mma_pages;
-    auto kernel = few_rows_kernel<QT, EIGHT, D, RW>;
     constexpr int ring = (WARPS / RW) * Shape<EIGHT, D>::STAGES * Shape<EIGHT, D>::STAGE, states = WARPS * 16 * (D + PART) * 4;
     LLMX_ALLOW_SMEM(few_rows_kernel<QT, EIGHT, D, RW>);
-    launch_kernel(kernel, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)kv_heads, (unsigned)requests), dim3(WARPS * 32),
-                  (size_t)(ring > states ? ring : states), stream, (const QT*)q, (const uint8_t*)cache, (const uint8_t*)exponents, (QT*)out, partial, a, heads,
-                  kv_heads, p.splits, scale * 1.4426950408889634f);
+    launch_kernel(few_rows_kernel<QT, EIGHT, D, RW>, dim3((unsigned)p.blocks), dim3(WARPS * 32), (size_t)(ring > states ? ring : states), stream,
+                  (const QT*)q, (const uint8_t*)cache, (const uint8_t*)exponents, (QT*)out, partial, a, requests, heads, kv_heads,
+                  scale * 1.4426950408889634f);
     if (const int e = launch_status()) return e;
-    if (p.splits > 1) {
-        const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
-        launch_kernel(few_rows_merge_kernel<QT, EIGHT, D>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, (const float*)partial,
-                      (QT*)out, a, heads, p.splits);
-    }
+    const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
+    launch_kernel(few_rows_merge_kernel<QT, EIGHT, D, RW>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, (const float*)partial,
+                  (QT*)out, a, requests, heads, kv_heads, p.blocks);
     return launch_status();
 }
 }  // namespace
@@ -177,7 +171,7 @@ LLMX_EXPORT int llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int
     *bytes = 0;
     if (requests <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    if (p.splits > 1) *bytes = (long long)requests * max_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4;
+    if (p.row_warps) *bytes = p.bytes(head_dim);
     return 0;
 }
 
@@ -196,10 +190,9 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
                     ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) && kv_heads <= 65535) {
-        if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
-                             workspace_bytes < (long long)requests * max_rows * heads * p.splits * (head_dim + mma_pages::PART) * 4))
-            return LLMX_ERR_BAD_ARGUMENT;
+    if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
+        (long long)pages * 2 * kv_heads * page_size < (1ll << 31)) {
+        if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes(head_dim)) return LLMX_ERR_BAD_ARGUMENT;
 #define LLMX_FEW(QT, EIGHT, D, RW) \
     return few_rows<QT, EIGHT, D, RW>(p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale, stream)
 #define LLMX_FEW_ROWS(QT, EIGHT, D)                        \
