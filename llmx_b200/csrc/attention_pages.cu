@@ -12,6 +12,7 @@
 // (row, head): each warp walks every fourth key in increasing order
 // with a running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone.
 #include "attention_pages_mma.cuh"
+#include "attention_pages_tc.cuh"
 
 namespace {
 constexpr int WARPS = 4;
@@ -127,10 +128,11 @@ int multiprocessors() {
     return n;
 }
 
-// How the form on the matrix instruction cuts a call up; `row_warps` 0: it does not take these sizes.
+// How a call is cut up; `rows` 0: only the general form takes these sizes.
 struct FewPlan {
-    int row_warps = 0, blocks = 0;
-    long long bytes(int head_dim) const { return 2ll * blocks * 16 * row_warps * (head_dim + mma_pages::PART) * 4; }      // two states a block
+    bool tensor = false;                  // tcgen05, else the warps' instruction
+    int rows = 0, blocks = 0;             // (row, head) pairs of a tile
+    long long bytes(int head_dim) const { return 2ll * blocks * rows * (head_dim + mma_pages::PART) * 4; }      // two states a block
 };
 
 FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads, int head_dim, int page_size,
@@ -139,13 +141,22 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
     const bool types = cache_dtype == LLMX_E4M3 || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
-    p.row_warps = pairs <= 16 ? 1 : pairs <= 32 ? 2 : 4;
-    // Two blocks find an SM each.  The kernel leaves some of them without work where there is too little.
-    const long long items = (pairs + 16 * p.row_warps - 1) / (16 * p.row_warps) * kv_heads * requests;
+    p.tensor = head_dim == 128 && q_dtype == LLMX_BF16;
+    p.rows = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
+    // As many blocks as find an SM at one time.  The kernel leaves some of them without work where there is too little.
+    const long long items = (pairs + p.rows - 1) / p.rows * kv_heads * requests;
     const long long keys = window > 0 ? min((long long)max_context, (long long)window + max_rows) : max_context;
-    const long long tiles = items * (keys / mma_pages::TILE + 2);
-    p.blocks = (int)min(2ll * multiprocessors(), max(items, tiles / 2));
+    const long long tiles = items * (keys / (p.tensor ? tc_pages::KEYS : mma_pages::TILE) + 2);
+    p.blocks = (int)min((p.tensor ? 1ll : 2ll) * multiprocessors(), max(items, tiles / 2));
     return p;
+}
+
+template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int RUNS>
+int merge(const FewPlan& p, void* out, const float* partial, const Rows& a, int requests, int max_rows, int heads, int kv_heads, cudaStream_t stream) {
+    const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
+    launch_kernel(mma_pages::merge_kernel<QT, EIGHT, D, TILE_ROWS, KEYS, RUNS>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, partial,
+                  (QT*)out, a, requests, heads, kv_heads, p.blocks);
+    return launch_status();
 }
 
 template <typename QT, bool EIGHT, int D, int RW>
@@ -158,10 +169,34 @@ int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exp
                   (const QT*)q, (const uint8_t*)cache, (const uint8_t*)exponents, (QT*)out, partial, a, requests, heads, kv_heads,
                   scale * 1.4426950408889634f);
     if (const int e = launch_status()) return e;
-    const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
-    launch_kernel(few_rows_merge_kernel<QT, EIGHT, D, RW>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, (const float*)partial,
-                  (QT*)out, a, requests, heads, kv_heads, p.blocks);
-    return launch_status();
+    return merge<QT, EIGHT, D, 16 * RW, TILE, WARPS / RW>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
+}
+
+// The pages' rows of 128 values, 16 at a time (bfloat16: 64 values of them).
+int pages_map(CUtensorMap* map, const void* cache, bool eight, uint64_t rows) {
+    if (!eight) return llmx_make_map_bf16_2d(map, cache, rows, 128, 16, 64);
+    llmx_encode_tiled_fn enc = llmx_encode_tiled();
+    if (!enc) return 10003;
+    const cuuint64_t dims[2] = {128, rows}, strides[1] = {128};
+    const cuuint32_t box[2] = {128, 16}, elem[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : 10003;
+}
+
+template <bool EIGHT, int U, int R>
+int tensor_rows(const FewPlan& p, const void* q, const void* cache, const void* exponents, void* out, float* partial, const Rows& a, int requests,
+                int max_rows, int heads, int kv_heads, float scale, int* error_word, cudaStream_t stream) {
+    using namespace tc_pages;
+    CUtensorMap map;
+    if (const int e = pages_map(&map, cache, EIGHT, (uint64_t)a.pages * 2 * kv_heads * a.page_size)) return e;
+    LLMX_ALLOW_SMEM(pages_kernel<EIGHT, U, R>);
+    launch_kernel(pages_kernel<EIGHT, U, R>, dim3((unsigned)p.blocks), dim3(tc_pages::Shape<EIGHT, U, R>::THREADS),
+                  (size_t)tc_pages::Shape<EIGHT, U, R>::BYTES, stream, map, (const __nv_bfloat16*)q, (const uint8_t*)exponents, (__nv_bfloat16*)out, partial, a,
+                  requests, heads, kv_heads, scale * 1.4426950408889634f, error_word);
+    if (const int e = launch_status()) return e;
+    return merge<__nv_bfloat16, EIGHT, 128, U * R, KEYS, 1>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
 }
 }  // namespace
 
@@ -171,7 +206,7 @@ LLMX_EXPORT int llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int
     *bytes = 0;
     if (requests <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    if (p.row_warps) *bytes = p.bytes(head_dim);
+    if (p.rows) *bytes = p.bytes(head_dim);
     return 0;
 }
 
@@ -182,7 +217,7 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
                                      const int* row_start, const int* row_count, const int* history, const int* tables, int table_stride,
                                      const void* tree, int tree_words, int requests, int total_rows, int max_rows, int max_context, int pages,
                                      int heads, int kv_heads, int head_dim, int page_size, int window, float scale, void* workspace,
-                                     long long workspace_bytes, cudaStream_t stream) {
+                                     long long workspace_bytes, int* error_word, cudaStream_t stream) {
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
         return LLMX_ERR_UNSUPPORTED;
@@ -190,28 +225,32 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
                     ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    if (p.row_warps && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
+    if (p.rows && pages > 0 && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
         (long long)pages * 2 * kv_heads * page_size < (1ll << 31)) {
         if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes(head_dim)) return LLMX_ERR_BAD_ARGUMENT;
-#define LLMX_FEW(QT, EIGHT, D, RW) \
-    return few_rows<QT, EIGHT, D, RW>(p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale, stream)
-#define LLMX_FEW_ROWS(QT, EIGHT, D)                        \
-    do {                                                   \
-        if (p.row_warps == 1) LLMX_FEW(QT, EIGHT, D, 1);   \
-        if (p.row_warps == 2) LLMX_FEW(QT, EIGHT, D, 2);   \
-        LLMX_FEW(QT, EIGHT, D, 4);                         \
+#define LLMX_FEW_ARGS p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale
+        if (p.tensor) {
+            if (cache_dtype == LLMX_E4M3) {
+                if (p.rows == 16) return tensor_rows<true, 1, 16>(LLMX_FEW_ARGS, error_word, stream);
+                if (p.rows == 32) return tensor_rows<true, 2, 16>(LLMX_FEW_ARGS, error_word, stream);
+                return tensor_rows<true, 2, 32>(LLMX_FEW_ARGS, error_word, stream);
+            }
+            if (p.rows == 16) return tensor_rows<false, 1, 16>(LLMX_FEW_ARGS, error_word, stream);
+            if (p.rows == 32) return tensor_rows<false, 2, 16>(LLMX_FEW_ARGS, error_word, stream);
+            return tensor_rows<false, 2, 32>(LLMX_FEW_ARGS, error_word, stream);
+        }
+#define LLMX_FEW_ROWS(QT, EIGHT, D)                                                         \
+    do {                                                                                    \
+        if (p.rows == 16) return few_rows<QT, EIGHT, D, 1>(LLMX_FEW_ARGS, stream);          \
+        if (p.rows == 32) return few_rows<QT, EIGHT, D, 2>(LLMX_FEW_ARGS, stream);          \
+        return few_rows<QT, EIGHT, D, 4>(LLMX_FEW_ARGS, stream);                            \
     } while (0)
-#define LLMX_FEW_WIDTH(QT, EIGHT)                          \
-    do {                                                   \
-        if (head_dim == 128) LLMX_FEW_ROWS(QT, EIGHT, 128); \
-        LLMX_FEW_ROWS(QT, EIGHT, 64);                      \
-    } while (0)
-        if (cache_dtype == LLMX_BF16) LLMX_FEW_WIDTH(__nv_bfloat16, false);
-        if (q_dtype == LLMX_BF16) LLMX_FEW_WIDTH(__nv_bfloat16, true);
-        LLMX_FEW_WIDTH(float, true);
-#undef LLMX_FEW
+        if (cache_dtype == LLMX_BF16) LLMX_FEW_ROWS(__nv_bfloat16, false, 64);
+        if (q_dtype == LLMX_BF16) LLMX_FEW_ROWS(__nv_bfloat16, true, 64);
+        if (head_dim == 64) LLMX_FEW_ROWS(float, true, 64);
+        LLMX_FEW_ROWS(float, true, 128);
+#undef LLMX_FEW_ARGS
 #undef LLMX_FEW_ROWS
-#undef LLMX_FEW_WIDTH
     }
     const size_t shmem = (size_t)WARPS * (head_dim + 2) * sizeof(float);
     const dim3 grid((unsigned)max_rows, (unsigned)heads, (unsigned)requests);

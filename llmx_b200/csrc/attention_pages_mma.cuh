@@ -124,7 +124,7 @@ __device__ __forceinline__ float4 read4(const __nv_bfloat16* p) {
 __device__ __forceinline__ void write4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void write4(__nv_bfloat16* p, float4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)); }
 
-// The state of a row over some keys: o (the sum of weights and codes), relative to 2^(top - RAISED); the sum of 2^(s - peak).
+// The state of a row over some keys: o (the sum of weights and codes), relative to 2^top; the sum of 2^(s - peak).
 constexpr int PART = 4;              // floats beside a row's D: top, peak, sum, one unused (16-byte rows)
 // A state's weight in a state with the maximum `most`: none for one without keys; NaN stays.
 __device__ __forceinline__ float share(float mine, float most) { return mine == -INFINITY ? 0.0f : exp2_fast(mine - most); }
@@ -133,7 +133,7 @@ __device__ __forceinline__ float share(float mine, float most) { return mine == 
 template <bool EIGHT>
 __device__ __forceinline__ float4 finished(float4 acc, float top, float peak, float sum) {
     if (sum == 0.0f) return make_float4(0.f, 0.f, 0.f, 0.f);
-    const float f = (EIGHT ? exp2f(top - peak - RAISED) : 1.0f) / sum;
+    const float f = (EIGHT ? exp2f(top - peak) : 1.0f) / sum;
     return make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 }
 
@@ -173,10 +173,11 @@ __device__ __forceinline__ void add_no_numbers(float (&o)[4], uint32_t (&v)[4], 
     }
 }
 
-// A request's part of the work: tiles of keys (at least one, so that rows that see nothing are written too) and tiles of rows.
+// A request's part of the work: tiles of KEYS keys (at least one, so that rows that see nothing are written too) and tiles of rows.
 struct Request {
     int count, history, start, pairs, low, end, tile0, tiles, row_tiles;
 };
+template <int KEYS>
 __device__ __forceinline__ Request request_of(const Rows& a, int r, int ratio, int tile_rows) {
     Request q;
     q.count = a.row_count[r], q.history = min(max(a.history[r], 0), MOST_KEYS), q.start = a.row_start[r];
@@ -186,12 +187,13 @@ __device__ __forceinline__ Request request_of(const Rows& a, int r, int ratio, i
     const int reach = (int)min((long long)a.table_stride * a.page_size, (long long)MOST_KEYS);
     q.end = min(reach, q.history + (a.tree ? min(q.count, 32 * a.tree_words) : q.count));
     q.low = a.window > 0 ? max(0, q.history - a.window + 1) : 0;
-    q.tile0 = q.low / TILE;
-    q.tiles = ours ? max((q.end + TILE - 1) / TILE - q.tile0, 1) : 0;
+    q.tile0 = q.low / KEYS;
+    q.tiles = ours ? max((q.end + KEYS - 1) / KEYS - q.tile0, 1) : 0;
     q.row_tiles = (q.pairs + tile_rows - 1) / tile_rows;
     return q;
 }
 // Requests' tiles in a row, by whole warps: those of all, or those before the request that place `x` falls in (which `found` names).
+template <int KEYS>
 __device__ __forceinline__ long long tiles_before(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, long long x, int& found,
                                                   long long& items) {
     const int lane = threadIdx.x & 31;
@@ -201,7 +203,7 @@ __device__ __forceinline__ long long tiles_before(const Rows& a, int requests, i
     for (int r0 = 0; r0 < requests; r0 += 32) {
         long long n = 0, of = 0;
         if (r0 + lane < requests) {
-            const Request q = request_of(a, r0 + lane, ratio, tile_rows);
+            const Request q = request_of<KEYS>(a, r0 + lane, ratio, tile_rows);
             of = (long long)q.row_tiles * kv_heads;
             n = of * q.tiles;
         }
@@ -245,14 +247,14 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 
     int r;
     long long items;
-    const long long all = tiles_before(a, requests, ratio, TILE_ROWS, kv_heads, -1, r, items);
+    const long long all = tiles_before<TILE>(a, requests, ratio, TILE_ROWS, kv_heads, -1, r, items);
     const int blocks = working_blocks(all, items, gridDim.x, RUNS);
     if ((int)blockIdx.x >= blocks) return;
     long long at = all * blockIdx.x / blocks;
     const long long until = all * (blockIdx.x + 1) / blocks;
     if (at >= until) return;
     long long unused;
-    long long request_at = tiles_before(a, requests, ratio, TILE_ROWS, kv_heads, at, r, unused);
+    long long request_at = tiles_before<TILE>(a, requests, ratio, TILE_ROWS, kv_heads, at, r, unused);
 
     // Where this lane's pieces lie: what it copies, keys (by the two, or four, quarters of a row's bytes), values.
     const uint32_t ring_at = shared_address(smem) + run * (STAGES * S::STAGE);
@@ -266,10 +268,10 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 
     for (bool first_segment = true;; first_segment = false) {
         // The item at `at`, and the part of its tiles that is this block's.
-        Request rq = request_of(a, r, ratio, TILE_ROWS);
+        Request rq = request_of<TILE>(a, r, ratio, TILE_ROWS);
         while (at >= request_at + (long long)rq.row_tiles * kv_heads * rq.tiles) {
             request_at += (long long)rq.row_tiles * kv_heads * rq.tiles;
-            rq = request_of(a, ++r, ratio, TILE_ROWS);
+            rq = request_of<TILE>(a, ++r, ratio, TILE_ROWS);
         }
         const long long item = (at - request_at) / rq.tiles;
         const int kv = (int)(item % kv_heads), first = (int)(item / kv_heads) * TILE_ROWS;
@@ -570,7 +572,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float* row = states + ((size_t)run * TILE_ROWS + rw * 16 + g + 8 * u) * ROWF;
-            if (c == 0) row[D] = top[u], row[D + 1] = peak[u], row[D + 2] = sum[u];
+            if (c == 0) row[D] = EIGHT ? top[u] - RAISED : top[u], row[D + 1] = peak[u], row[D + 2] = sum[u];
             if constexpr (EIGHT) {
 #pragma unroll
                 for (int n = 0; n < S::PIECES; ++n)
@@ -616,22 +618,22 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 
 // Adds up the items that blocks share, one warp for 128 of a (row, head)'s values (two rows of 64).  Which blocks those are follows
 // from the same counts as in the kernel before.
-template <typename QT, bool EIGHT, int D, int RW>
+template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int RUNS>
 __global__ void __launch_bounds__(128)
-few_rows_merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, int requests, int heads, int kv_heads, int grid) {
+merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, int requests, int heads, int kv_heads, int grid) {
     pdl_trigger();
     pdl_wait();
-    constexpr int ROWF = D + PART, TILE_ROWS = 16 * RW, LANES = D / 4, EACH = 128 / LANES;
+    constexpr int ROWF = D + PART, LANES = D / 4, EACH = 128 / LANES;
     const int r = blockIdx.y, ratio = heads / kv_heads;
-    const Request rq = request_of(a, r, ratio, TILE_ROWS);
+    const Request rq = request_of<KEYS>(a, r, ratio, TILE_ROWS);
     const long long first_item = (long long)blockIdx.x * EACH;
     if (first_item >= (long long)rq.count * heads) return;
     int found;
     long long items, unused;
-    const long long all = tiles_before(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
-    const int blocks = working_blocks(all, items, grid, WARPS / RW);
+    const long long all = tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
+    const int blocks = working_blocks(all, items, grid, RUNS);
     // The place of this request's tiles: before it lie those of the requests 0 .. r - 1.
-    const long long request_at = tiles_before(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
+    const long long request_at = tiles_before<KEYS>(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
     const long long item = first_item + threadIdx.x / LANES;
     if (item >= (long long)rq.count * heads) return;
     const int row = (int)(item / heads), head = (int)(item % heads), kv = head / ratio, pair = row * ratio + head % ratio, d = 4 * (threadIdx.x % LANES);

@@ -1,0 +1,668 @@
+// Attention over pages on the tensor cores of tcgen05: few rows a request (decoding, drafts), heads of 128.
+//
+// The warp form (attention_pages_mma.cuh) spends its time on turning codes into halves and moving them through registers.  Here neither
+// keys nor values pass through registers at all: TMA brings 128 keys of a head to shared memory as they lie in their pages, and the
+// matrix instruction reads codes (kind::f8f6f4; bfloat16 pages: kind::f16) from there, keys and values on its 128-row side:
+//     S^T [128 keys, rows] = K Q^T           K as it lies, K-major
+//     O^T [128 values, rows] += V^T W^T      V as it lies, MN-major; W^T [keys, rows] written by the softmax warps, MN-major
+// A request's rows are the narrow side, 16 at a time: what is idle is not the instruction's 128 rows but its columns, which cost
+// nothing.  A softmax thread has one key and all rows, so that a key's power of two is its thread's own.
+//
+// Eight bits on both sides: a query is two codes that add up to it, q = (q1 + q2 / 32) 2^e (bfloat16 has 8 bits, a code 4: exact down
+// to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 16 + w3 / 256 (12 bits, down to 2^-26 of the largest): columns of their
+// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two joins its key's score.
+//
+//   warp 0          page lookups and copies, 16 keys (or their exponents) a lane, STAGES tiles ahead
+//   warp 1          matrix instructions: S^T of the next tile before O^T of this one
+//   warps 2 ..      units of four warps, each with R of the rows: exponentials, weights to shared memory
+// The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^4 of them has the unit
+// raise them, and its sums and outputs (in tensor memory) scaled.  Every wait is bounded; the softmax warps go on through their
+// barriers without waiting once one has run out.
+//
+// Work is cut evenly as in the warp form, one block an SM, tiles of 128 keys.
+#pragma once
+#include "attention_pages_mma.cuh"
+#include "attn_common.cuh"
+
+namespace tc_pages {
+
+using mma_pages::copy16;
+using mma_pages::exp2_fast;
+using mma_pages::max3;
+using mma_pages::PART;
+using mma_pages::Request;
+using mma_pages::request_of;
+using mma_pages::Rows;
+
+constexpr int KEYS = 128, D = 128;
+constexpr int UNIT_WARPS = 4;
+// The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
+// leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
+constexpr float RAISED = 4.0f, ROOM = 57.0f, LIMIT = 8.0f;
+constexpr float NONE = -1.0e30f;        // a maximum of no keys
+enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 503 };
+
+template <bool EIGHT, int U, int R>
+struct Shape {
+    static constexpr int THREADS = 64 + U * UNIT_WARPS * 32;
+    static constexpr int PLANE = KEYS * D * (EIGHT ? 1 : 2);
+    static constexpr int STAGE = 2 * PLANE;
+    static constexpr int STAGES = EIGHT ? 4 : 2;
+    static constexpr int WEIGHTS = KEYS * 128;                  // bytes of a unit's weights of a tile: rows of 128 bytes, the first ones used
+    static constexpr int BUFFERS = EIGHT ? 2 : 1;               // of weights
+    static constexpr int QUERIES = (EIGHT ? 2 * R * D : R * D * 2);
+    static constexpr int S_COLS = EIGHT ? 2 * R : R, O_COLS = EIGHT ? 3 * R : R, U_COLS = 2 * S_COLS + O_COLS;
+    static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
+    static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + U * BUFFERS * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
+    // What a unit's threads tell each other, in floats: factors, minus the two maxima, what raising scales the two by, positions [R];
+    // maxima and sums of warps [2][4][R].
+    static constexpr int UNIT_FLOATS = 6 * R + 2 * UNIT_WARPS * R;
+    static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
+    static constexpr int AT_STRAY = AT_FLOATS + U * UNIT_FLOATS * 4;                    // [rows][D] products with values that are no numbers
+    static constexpr int AT_BARRIERS = AT_STRAY + (EIGHT ? 0 : U * R * D * 4);
+    static constexpr int BYTES = AT_BARRIERS + 512 + 1024;                              // and to the next 1024
+};
+
+// MN-major operand of bytes or 16-bit values under the 128-byte swizzle: 128 bytes of the MN dimension in a row, rows of the K dimension 128
+// bytes apart (groups of eight 1024), the MN dimension's next 128 bytes `block` further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t block) {
+    return (uint64_t)((at & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+constexpr uint32_t TRANSPOSED = (1u << 15) | (1u << 16);
+// kind::f8f6f4, e4m3 on both sides, 32-bit sums.
+__host__ __device__ constexpr uint32_t instruction_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes),
+                 "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+// A barrier of a unit's threads; true for all if it is for one.
+__device__ __forceinline__ bool unit_any(int unit, bool mine) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)mine), "r"(1 + unit)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void unit_barrier(int unit) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + unit) : "memory"); }
+
+__device__ __forceinline__ float4 shared4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void to_shared4(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ unsigned shared_byte(uint32_t at) {
+    unsigned v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float at4(const float4& v, int k) { return k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w; }
+// Value d of a bfloat16 row of a stage, its two halves apart, pieces of 16 bytes exchanged by the row's place.
+template <int HALF>
+__device__ __forceinline__ unsigned short* value_in(uint8_t* row, int key, int d) {
+    return reinterpret_cast<unsigned short*>(row + (d >> 6) * HALF + (((d >> 3 & 7) ^ (key & 7)) << 4) + 2 * (d & 7));
+}
+
+// Two halves to two codes, the second value in the upper byte.
+__device__ __forceinline__ uint32_t codes2(uint32_t halves) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(halves));
+    return r;
+}
+// 16 halves (pairs) as 16 codes, and what is left of them times 32.
+__device__ __forceinline__ uint4 take_codes(uint32_t (&h)[8], bool more) {
+    uint32_t c[8];
+    const __half2 scale = __floats2half2_rn(32.0f, 32.0f);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        c[n] = codes2(h[n]);
+        if (more) {
+            const uint32_t back = e4m3::halves((unsigned short)c[n]);
+            const __half2 left = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&h[n]), *reinterpret_cast<const __half2*>(&back)), scale);
+            h[n] = *reinterpret_cast<const uint32_t*>(&left);
+        }
+    }
+    return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
+}
+
+template <bool EIGHT, int U, int R>
+__global__ void __launch_bounds__(Shape<EIGHT, U, R>::THREADS, 1)
+pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ exponents,
+             __nv_bfloat16* __restrict__ out, float* __restrict__ partial, Rows a, int requests, int heads, int kv_heads, float scale_log2,
+             int* error_word) {
+    using S = Shape<EIGHT, U, R>;
+    constexpr int TILE_ROWS = U * R, ROWF = D + PART, STAGES = S::STAGES, CHUNKS = R / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = (uint64_t*)(smem + S::AT_BARRIERS);        // [STAGES]
+    uint64_t* empty = full + STAGES;                            // [STAGES]
+    uint64_t* q_full = empty + STAGES;                          // [U]
+    uint64_t* s_full = q_full + U;                              // [U][2]
+    uint64_t* s_free = s_full + 2 * U;                          // [U][2]
+    uint64_t* w_full = s_free + 2 * U;                          // [U][BUFFERS]
+    uint64_t* o_done = w_full + 2 * U;                          // [U][BUFFERS]: O^T with that buffer's weights
+    uint32_t* tmem_slot = (uint32_t*)(o_done + 2 * U);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    volatile int* live = abort_flag + 1;                        // [STAGES]: which of the stage's runs of 16 keys are in the cache
+    volatile int* stray_flag = live + STAGES;                   // [U]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ratio = heads / kv_heads;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
+        for (int u = 0; u < U; ++u) {
+            tc::mbar_init(&q_full[u], UNIT_WARPS);
+            for (int i = 0; i < 2; ++i) {
+                tc::mbar_init(&s_full[2 * u + i], 1);
+                tc::mbar_init(&s_free[2 * u + i], UNIT_WARPS);
+                tc::mbar_init(&w_full[2 * u + i], UNIT_WARPS);
+                tc::mbar_init(&o_done[2 * u + i], 1);
+            }
+            stray_flag[u] = 0;
+        }
+        *abort_flag = 0;
+        tc::fence_barrier_init();
+        tc::tma_prefetch_desc(&map);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, S::TMEM);
+        tc::tmem_relinquish();
+    }
+    // Values that no copy has written yet are zeros, never what the memory held before: a weight of zero meets them.
+    for (int i = threadIdx.x; i < STAGES * S::PLANE / 16; i += S::THREADS)
+        *reinterpret_cast<uint4*>(smem + (i / (S::PLANE / 16)) * S::STAGE + S::PLANE + (i % (S::PLANE / 16)) * 16) = make_uint4(0, 0, 0, 0);
+    if constexpr (!EIGHT)
+        for (int i = threadIdx.x; i < U * R * D / 4; i += S::THREADS) reinterpret_cast<float4*>(smem + S::AT_STRAY)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    tc::fence_proxy_async();
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_trigger();                       // (only now: a dependent block must not take the tensor memory that this one waits for)
+    pdl_wait();
+
+    // ---- the work, which every role walks alike
+    int r0;
+    long long items;
+    const long long all = mma_pages::tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, -1, r0, items);
+    const int blocks = mma_pages::working_blocks(all, items, gridDim.x, 1);
+    long long at = (int)blockIdx.x < blocks ? all * blockIdx.x / blocks : 0;
+    const long long until = (int)blockIdx.x < blocks ? all * (blockIdx.x + 1) / blocks : 0;
+    long long unused;
+    long long request_at = mma_pages::tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, at, r0, unused);
+    const int runs_a_page = a.page_size >> 4;
+    auto page_of = [&](int sixteenth) { return (int)(((uint64_t)(unsigned)sixteenth * a.run_pages) >> 31); };
+    struct Segment {
+        Request rq;
+        int r, kv, first, from, tiles;
+        bool whole;
+    } sg;
+    sg.r = r0;
+    auto next_segment = [&]() -> bool {
+        if (at >= until) return false;
+        sg.rq = request_of<KEYS>(a, sg.r, ratio, TILE_ROWS);
+        while (at >= request_at + (long long)sg.rq.row_tiles * kv_heads * sg.rq.tiles) {
+            request_at += (long long)sg.rq.row_tiles * kv_heads * sg.rq.tiles;
+            sg.rq = request_of<KEYS>(a, ++sg.r, ratio, TILE_ROWS);
+        }
+        const long long item = (at - request_at) / sg.rq.tiles, item_at = request_at + item * sg.rq.tiles;
+        sg.kv = (int)(item % kv_heads), sg.first = (int)(item / kv_heads) * TILE_ROWS;
+        const int skipped = (int)(at - item_at);
+        sg.tiles = (int)(min(until, item_at + sg.rq.tiles) - at);
+        sg.whole = skipped == 0 && sg.tiles == sg.rq.tiles;
+        sg.from = sg.rq.tile0 + skipped;
+        at += sg.tiles;
+        return true;
+    };
+
+    if (warp == 0) {
+        // Lane: a run of 16 keys, keys or values, and codes or exponents (bfloat16: the row's first or second half).
+        const int p = lane & 7, plane = (lane >> 3) & 1, second = lane >> 4;
+        uint32_t use = 0;
+        bool ok = true;
+        while (ok && next_segment()) {
+            const int* table = a.tables + (size_t)sg.r * a.table_stride;
+            auto look_up = [&](int i) {
+                const int n = (sg.from + i) * (KEYS / 16) + p;
+                return i < sg.tiles && n * 16 < sg.rq.end && n * 16 + 16 > sg.rq.low ? table[page_of(n)] : -1;
+            };
+            int ahead = look_up(0);
+            for (int i = 0; i < sg.tiles; ++i, ++use) {
+                const int stage = use % STAGES, n = (sg.from + i) * (KEYS / 16) + p, page = ahead;
+                ahead = look_up(i + 1);
+                ok = tc::mbar_wait(&empty[stage], ((use / STAGES) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const bool real = (unsigned)page < (unsigned)a.pages;
+                const unsigned runs = __ballot_sync(0xffffffffu, real) & 0xffu;
+                if (lane == 0) {
+                    live[stage] = (int)runs;
+                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * (16 * D * (EIGHT ? 1 : 2) + (EIGHT ? 16 : 0)));
+                }
+                __syncwarp();
+                if (real) {
+                    const unsigned row = (((unsigned)page * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+                    uint8_t* to = smem + stage * S::STAGE + plane * S::PLANE;
+                    if constexpr (EIGHT) {
+                        if (second) copy_bulk(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16, exponents + row, 16, &full[stage]);
+                        else tc::tma_load_2d(to + p * 16 * 128, &map, 0, (int)row, &full[stage]);
+                    } else {
+                        tc::tma_load_2d(to + second * (S::PLANE / 2) + p * 16 * 128, &map, 64 * second, (int)row, &full[stage]);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (tc::elect_one()) {
+            uint32_t use = 0, segments = 0;
+            bool ok = true;
+            auto scores = [&](uint32_t n) -> bool {              // S^T of tile use n
+                const int stage = n % STAGES, buffer = n & 1;
+                if (!tc::mbar_wait(&full[stage], (n / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_MMA)) return false;
+                const uint32_t keys = tc::smem_u32(smem + stage * S::STAGE);
+                for (int u = 0; u < U; ++u) {
+                    if (!tc::mbar_wait(&s_free[2 * u + buffer], ((n >> 1) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_MMA)) return false;
+                    tc::tc_fence_after();
+                    const uint32_t queries = tc::smem_u32(smem + S::AT_QUERIES + u * S::QUERIES), d = tmem + u * S::U_COLS + buffer * S::S_COLS;
+                    if constexpr (EIGHT) {
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+                            mma_e4m3(d, tc::smem_desc_k_sw128(keys + k * 32), tc::smem_desc_k_sw128(queries + k * 32), instruction_e4m3(KEYS, 2 * R), k > 0);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+                            tc::mma_bf16_ss(d, tc::smem_desc_k_sw128(keys + (k >> 2) * (S::PLANE / 2) + (k & 3) * 32),
+                                            tc::smem_desc_k_sw128(queries + (k >> 2) * (R * 128) + (k & 3) * 32), tc::instr_desc_bf16(KEYS, R), k > 0);
+                    }
+                    tc::mma_commit(&s_full[2 * u + buffer]);
+                }
+                return true;
+            };
+            while (ok && next_segment()) {
+                for (int u = 0; u < U && ok; ++u) ok = tc::mbar_wait(&q_full[u], segments & 1u, abort_flag, error_word, ERR_PAGES_MMA);
+                ++segments;
+                tc::tc_fence_after();
+                if (ok) ok = scores(use);
+                for (int i = 0; i < sg.tiles && ok; ++i, ++use) {
+                    if (i + 1 < sg.tiles) ok = scores(use + 1);
+                    const int stage = use % STAGES, buffer = use % S::BUFFERS;
+                    for (int u = 0; u < U && ok; ++u) {
+                        ok = tc::mbar_wait(&w_full[2 * u + buffer], (use / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_MMA);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + S::PLANE), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
+                        const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + (u * S::BUFFERS + buffer) * S::WEIGHTS);
+                        if constexpr (EIGHT) {
+#pragma unroll
+                            for (int k = 0; k < KEYS / 32; ++k)
+                                mma_e4m3(d, desc_mn(values + k * 4096, S::PLANE), desc_mn(weights + k * 4096, S::WEIGHTS),
+                                         instruction_e4m3(D, 3 * R) | TRANSPOSED, i > 0 || k > 0);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < KEYS / 16; ++k)
+                                tc::mma_bf16_ss(d, desc_mn(values + k * 2048, S::PLANE / 2), desc_mn(weights + k * 2048, S::WEIGHTS),
+                                                tc::instr_desc_bf16(D, R) | TRANSPOSED, i > 0 || k > 0);
+                        }
+                        if (u == U - 1) tc::mma_commit(&empty[stage]);
+                        tc::mma_commit(&o_done[2 * u + buffer]);
+                    }
+                }
+            }
+        }
+    } else {
+        const int unit = (warp - 2) / UNIT_WARPS, quarter = warp & 3, key = quarter * 32 + lane;
+        const int thread = ((warp - 2) % UNIT_WARPS) * 32 + lane;               // of the unit, for what is shared out among its threads
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t s_at = tmem + unit * S::U_COLS + lanes, o_at = s_at + 2 * S::S_COLS;
+        float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
+        float *factor = shared, *minus_peak = shared + R, *minus_top = shared + 2 * R, *fade_sum = shared + 3 * R, *fade_o = shared + 4 * R;
+        int* position = reinterpret_cast<int*>(shared + 5 * R);
+        float *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
+        float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
+        const uint32_t rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
+        const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + unit * S::BUFFERS * S::WEIGHTS) + key * 128;
+        uint32_t use = 0;
+        bool ok = true, first_segment = true;
+        for (; next_segment(); first_segment = false) {
+            const int first = sg.first + unit * R, pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
+            // ---- the unit's queries: a row by 128 / R threads
+            {
+                constexpr int EACH = 128 / R, OWN = D / EACH;
+                const int row = thread / EACH, part = thread % EACH, pair = first + row;
+                const bool real = pair < pairs;
+                const int token = real ? pair / ratio : 0;
+                const __nv_bfloat16* src = q + ((size_t)(start + token) * heads + sg.kv * ratio + (real ? pair % ratio : 0)) * D + part * OWN;
+                uint4 x[OWN / 8];
+#pragma unroll
+                for (int n = 0; n < OWN / 8; ++n) x[n] = real ? reinterpret_cast<const uint4*>(src)[n] : make_uint4(0, 0, 0, 0);
+                uint8_t* queries = smem + S::AT_QUERIES + unit * S::QUERIES;
+                float f = scale_log2;
+                if constexpr (EIGHT) {
+                    unsigned most = 0;                           // magnitudes of bfloat16 compare as their bits do
+#pragma unroll
+                    for (int n = 0; n < OWN / 8; ++n) {
+                        const unsigned v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) most = max(most, max(v[k] & 0x7FFFu, v[k] >> 16 & 0x7FFFu));
+                    }
+#pragma unroll
+                    for (int o = 1; o < EACH; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int e = min(max((int)(most >> 7) - 127, -100), 127);     // the row's largest lies in 2^e .. 2^(e + 1): to 2^7 .. 2^8
+                    const float up = __int_as_float((127 + 7 - e) << 23);
+                    f = fmaxf(__int_as_float((127 - 7 + e) << 23) * scale_log2, 1.0e-44f);     // (not zero: a masked score stays -inf)
+                    const bool bad = most >= 0x7F80u;            // a row with an infinity or a NaN: codes that are NaN
+#pragma unroll
+                    for (int n = 0; n < OWN / 16; ++n) {
+                        uint32_t one[4], two[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const unsigned w0 = (&x[2 * n + (k >> 1)].x)[2 * (k & 1)], w1 = (&x[2 * n + (k >> 1)].x)[2 * (k & 1) + 1];
+                            const float v[4] = {__uint_as_float(w0 << 16) * up, __uint_as_float(w0 & 0xffff0000u) * up, __uint_as_float(w1 << 16) * up,
+                                                __uint_as_float(w1 & 0xffff0000u) * up};
+                            const unsigned c0 = e4m3::pack2(v[0], v[1]), c1 = e4m3::pack2(v[2], v[3]);
+                            const float2 b0 = mma_pages::from_halves(e4m3::halves((unsigned short)c0)), b1 = mma_pages::from_halves(e4m3::halves((unsigned short)c1));
+                            one[k] = bad ? 0x7F7F7F7Fu : c0 | c1 << 16;
+                            two[k] = e4m3::pack2((v[0] - b0.x) * 32.0f, (v[1] - b0.y) * 32.0f) | e4m3::pack2((v[2] - b1.x) * 32.0f, (v[3] - b1.y) * 32.0f) << 16;
+                        }
+                        const int piece = part * (OWN / 16) + n, r1 = (row >> 4) * 32 + (row & 15), r2 = r1 + 16;
+                        *reinterpret_cast<uint4*>(queries + r1 * 128 + ((piece ^ (r1 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
+                        *reinterpret_cast<uint4*>(queries + r2 * 128 + ((piece ^ (r2 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < OWN / 8; ++n) {
+                        const int piece = part * (OWN / 8) + n;
+                        *reinterpret_cast<uint4*>(queries + (piece >> 3) * (R * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = x[n];
+                    }
+                }
+                if (part == 0) {
+                    factor[row] = f;
+                    minus_peak[row] = minus_top[row] = -NONE;
+                    position[row] = real ? history + token : -1;
+                }
+                tc::fence_proxy_async();
+                unit_barrier(unit);
+                if (lane == 0) tc::mbar_arrive(&q_full[unit]);
+            }
+            const int row0 = first / ratio, row1 = max(row0, (min(first + R, pairs) - 1) / ratio);
+            const int all_to = a.tree ? min(history, sg.rq.end) : min(history + row0 + 1, sg.rq.end);
+            const int all_from = a.window > 0 ? max(history + row1 - a.window + 1, 0) : 0;
+
+            float sum[R];
+#pragma unroll
+            for (int n = 0; n < R; ++n) sum[n] = 0.0f;
+            for (int i = 0; i < sg.tiles; ++i, ++use) {
+                const int stage = use % STAGES, s_buffer = use & 1, w_buffer = use % S::BUFFERS;
+                const int t0 = (sg.from + i) * KEYS, t = t0 + key;
+                if (ok) ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                const int runs = live[stage];
+                const bool dead = !(runs >> (key >> 4) & 1);     // a page that is not in the cache: a key of zeros
+                float k_power = 1.0f, v_power = 0.0f;
+                if constexpr (EIGHT) {
+                    const uint32_t b = exponents_at + stage * 256 + key;
+                    const unsigned kb = shared_byte(b), vb = shared_byte(b + KEYS);
+                    // A value that is no number makes its key none: NaN for the rows that see it.
+                    k_power = dead ? 0.0f : vb == e4m3::NOT_NUMBERS ? NAN : e4m3::up(kb);
+                    v_power = dead || vb == e4m3::NOT_NUMBERS ? 0.0f : (float)((int)vb - 127);
+                }
+                const bool whole = t0 >= all_from && t0 + KEYS <= all_to && runs == 0xff;
+                const bool in_reach = t >= sg.rq.low && t < sg.rq.end;
+                uint8_t* value_row = smem + stage * S::STAGE + S::PLANE + key * 128;
+                bool stray = false;
+                unsigned hidden = 0;                             // rows that do not see this key
+                if (!whole) {
+                    if (dead || !in_reach) {
+                        // Values that nobody sees must be numbers, those of a page that is not there zeros.
+#pragma unroll
+                        for (int n = 0; n < (EIGHT ? 8 : 16); ++n)
+                            *reinterpret_cast<uint4*>(value_row + (n >> 3) * (S::PLANE / 2) + (n & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    } else if (!EIGHT && a.tree && t >= history) {
+                        // Values that are no numbers, of a key that not every row sees: their products are added up beside the others, for
+                        // the rows that do, and zeros take their place (a weight of zero times an infinity is no zero).
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(value_row + (n >> 3) * (S::PLANE / 2) + (n & 7) * 16);
+                            const unsigned x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) stray |= (x[k] & 0x7F80u) == 0x7F80u || (x[k] & 0x7F800000u) == 0x7F800000u;
+                        }
+                    }
+                    for (int n = 0; n < R; ++n) {
+                        const int pos = position[n];
+                        bool sees = in_reach && pos >= 0;
+                        if (a.tree) {
+                            if (sees && t >= history)
+                                sees = (a.tree[(size_t)(start + pos - history) * a.tree_words + ((t - history) >> 5)] >> ((t - history) & 31)) & 1u;
+                        } else {
+                            sees = sees && t <= pos && (a.window <= 0 || t > pos - a.window);
+                        }
+                        if (!sees) hidden |= 1u << n;
+                    }
+                }
+                if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (use >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                tc::tc_fence_after();
+                // ---- the exponents: x of the sum, y of the weights
+                float x[R], y[EIGHT ? R : 1];
+                auto scores = [&](auto&& take) {                 // score by score, without their rows' factors
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        float z[16];
+                        if constexpr (EIGHT) {
+                            uint32_t v[32];
+                            tc::tmem_ld_32x32(s_at + s_buffer * S::S_COLS + 32 * c, v);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) z[n] = fmaf(__uint_as_float(v[16 + n]), 1.0f / 32.0f, __uint_as_float(v[n])) * k_power;
+                        } else {
+                            uint32_t v[16];
+                            tc::tmem_ld_32x16(s_at + s_buffer * S::S_COLS + 16 * c, v);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) z[n] = __uint_as_float(v[n]);
+                        }
+                        if (!whole) {
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) z[n] = hidden >> (16 * c + n) & 1u ? -INFINITY : dead ? 0.0f : z[n];
+                        }
+#pragma unroll
+                        for (int n = 0; n < 16; n += 4) take(16 * c + n, z[n], z[n + 1], z[n + 2], z[n + 3]);
+                    }
+                };
+                for (int again = 0; again < 2; ++again) {
+                    float over = -INFINITY;
+                    scores([&](int n, float z0, float z1, float z2, float z3) {
+                        const float4 f = shared4(rows_at + 4 * n), mp = shared4(rows_at + 4 * (R + n));
+                        x[n] = fmaf(z0, f.x, mp.x), x[n + 1] = fmaf(z1, f.y, mp.y), x[n + 2] = fmaf(z2, f.z, mp.z), x[n + 3] = fmaf(z3, f.w, mp.w);
+                        if constexpr (EIGHT) {
+                            const float4 mt = shared4(rows_at + 4 * (2 * R + n));
+                            y[n] = fmaf(z0, f.x, mt.x + v_power), y[n + 1] = fmaf(z1, f.y, mt.y + v_power);
+                            y[n + 2] = fmaf(z2, f.z, mt.z + v_power), y[n + 3] = fmaf(z3, f.w, mt.w + v_power);
+                            over = max3(max3(over, x[n], y[n]), x[n + 1], y[n + 1]);
+                            over = max3(max3(over, x[n + 2], y[n + 2]), x[n + 3], y[n + 3]);
+                        } else {
+                            over = max3(max3(over, x[n], x[n + 1]), x[n + 2], x[n + 3]);
+                        }
+                    });
+                    if (!unit_any(unit, again == 0 && over > LIMIT)) break;
+                    // ---- the references rise to this tile's maxima
+                    scores([&](int n, float z0, float z1, float z2, float z3) {
+                        const float z[4] = {z0, z1, z2, z3};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float p = z[k] * factor[n + k], w = p + v_power;
+#pragma unroll
+                            for (int o = 16; o > 0; o >>= 1) {
+                                p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, o));
+                                if (EIGHT) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+                            }
+                            if (lane == 0) warp_peak[quarter * R + n + k] = p, warp_top[quarter * R + n + k] = w;
+                        }
+                    });
+                    unit_barrier(unit);
+                    if (thread < R) {
+                        const int n = thread;
+                        float p = NONE, w = NONE;
+#pragma unroll
+                        for (int k = 0; k < UNIT_WARPS; ++k) p = fmaxf(p, warp_peak[k * R + n]), w = fmaxf(w, warp_top[k * R + n]);
+                        const float before = -minus_peak[n], now = fmaxf(before, p == NONE ? NONE : EIGHT ? p + ROOM : p);
+                        const float top_before = -minus_top[n], top_now = EIGHT ? fmaxf(top_before, w == NONE ? NONE : w - RAISED) : now;
+                        fade_sum[n] = exp2_fast(before - now);
+                        fade_o[n] = EIGHT ? exp2_fast(top_before - top_now) : fade_sum[n];
+                        minus_peak[n] = -now, minus_top[n] = -top_now;
+                    }
+                    unit_barrier(unit);
+#pragma unroll
+                    for (int n = 0; n < R; ++n) sum[n] *= fade_sum[n];
+                    if (i > 0) {
+                        // Every O^T that has been asked for has been made before it is scaled.
+                        const uint32_t last = use - 1;
+                        if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                        tc::tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < S::O_COLS / 16; ++c) {
+                            uint32_t v[16];
+                            tc::tmem_ld_32x16(o_at + 16 * c, v);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) v[n] = __float_as_uint(__uint_as_float(v[n]) * fade_o[(EIGHT ? c / 3 : c) * 16 + n]);
+                            tc::tmem_st_32x16(o_at + 16 * c, v);
+                        }
+                        tc::tmem_wait_st();
+                    }
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s_free[2 * unit + s_buffer]);
+                // ---- weights
+                if (use >= (uint32_t)S::BUFFERS && ok)           // the buffer's weights before have been used
+                    ok = tc::mbar_wait_warp(&o_done[2 * unit + w_buffer], ((use / S::BUFFERS) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                const uint32_t weights = weights_at + w_buffer * S::WEIGHTS;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    uint32_t h[8];
+#pragma unroll
+                    for (int n = 0; n < 16; n += 2) {
+                        const int row = 16 * c + n;
+                        const float e0 = exp2_fast(x[row]), e1 = exp2_fast(x[row + 1]);
+                        sum[row] += e0;
+                        sum[row + 1] += e1;
+                        if constexpr (EIGHT) {
+                            h[n >> 1] = mma_pages::pack_half(exp2_fast(y[row]), exp2_fast(y[row + 1]));
+                        } else {
+                            h[n >> 1] = mma_pages::pack_bf16(e0, e1);
+                            if (stray)
+                                for (int k = 0; k < 2; ++k) {
+                                    if (hidden >> (row + k) & 1u) continue;
+                                    for (int d = 0; d < D; ++d) {
+                                        const unsigned v = *value_in<S::PLANE / 2>(value_row, key, d);
+                                        if ((v & 0x7F80u) == 0x7F80u) atomicAdd(strays + (row + k) * D + d, (k ? e1 : e0) * __uint_as_float(v << 16));
+                                    }
+                                    stray_flag[unit] = 1;
+                                }
+                        }
+                    }
+                    if constexpr (EIGHT) {
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) to_shared4(weights + (((3 * c + k) ^ (key & 7)) << 4), take_codes(h, k < 2));
+                    } else {
+                        to_shared4(weights + (((2 * c) ^ (key & 7)) << 4), make_uint4(h[0], h[1], h[2], h[3]));
+                        to_shared4(weights + (((2 * c + 1) ^ (key & 7)) << 4), make_uint4(h[4], h[5], h[6], h[7]));
+                    }
+                }
+                if constexpr (!EIGHT)
+                    if (a.tree && t0 + KEYS > history) {
+                        // No unit takes such values away before all have read them.
+                        asm volatile("barrier.cta.sync 7, %0;" ::"n"(U * UNIT_WARPS * 32) : "memory");
+                        if (stray)
+                            for (int d = 0; d < D; ++d) {
+                                unsigned short* x = value_in<S::PLANE / 2>(value_row, key, d);
+                                if ((*x & 0x7F80u) == 0x7F80u) *x = 0;
+                            }
+                    }
+                tc::fence_proxy_async();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&w_full[2 * unit + w_buffer]);
+            }
+
+            // ---- the item's sums over this block's keys: a thread has one of the 128 values of every row
+            const uint32_t last = use - 1;
+#pragma unroll
+            for (int n = 0; n < R; ++n) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], o);
+                if (lane == 0) warp_peak[quarter * R + n] = sum[n];
+            }
+            if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+            tc::tc_fence_after();
+            unit_barrier(unit);
+            const bool any_stray = !EIGHT && stray_flag[unit];
+            float* slot = partial + (2 * (size_t)blockIdx.x + !first_segment) * TILE_ROWS * ROWF;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                float o[16];
+                uint32_t v[16];
+                tc::tmem_ld_32x16(o_at + (EIGHT ? 48 : 16) * c, v);
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int n = 0; n < 16; ++n) o[n] = __uint_as_float(v[n]);
+                if constexpr (EIGHT) {
+                    tc::tmem_ld_32x16(o_at + 48 * c + 16, v);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) o[n] = fmaf(__uint_as_float(v[n]), 1.0f / 32.0f, o[n]);
+                    tc::tmem_ld_32x16(o_at + 48 * c + 32, v);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) o[n] = fmaf(__uint_as_float(v[n]), 1.0f / 1024.0f, o[n]);
+                }
+#pragma unroll
+                for (int n = 0; n < 16; ++n) {
+                    const int row = 16 * c + n, pair = first + row;
+                    if (pair >= pairs) continue;
+                    if (any_stray) o[n] += strays[row * D + key];
+                    const float total = (warp_peak[row] + warp_peak[R + row]) + (warp_peak[2 * R + row] + warp_peak[3 * R + row]);
+                    const float peak = -minus_peak[row], top = -minus_top[row];
+                    if (sg.whole) {
+                        const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
+                        out[((size_t)(start + pair / ratio) * heads + sg.kv * ratio + pair % ratio) * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
+                    } else {
+                        float* to = slot + (size_t)(unit * R + row) * ROWF;
+                        to[key] = o[n];
+                        if (key < 3) to[D + key] = key == 0 ? top : key == 1 ? peak : total;
+                    }
+                }
+            }
+            tc::tc_fence_before();
+            unit_barrier(unit);                                  // before the next item's rows take this one's places
+            if (any_stray) {
+                for (int n = thread; n < R * D; n += 128) strays[n] = 0.0f;
+                stray_flag[unit] = 0;
+                unit_barrier(unit);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, S::TMEM);
+    }
+}
+
+}  // namespace tc_pages

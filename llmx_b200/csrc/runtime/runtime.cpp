@@ -45,7 +45,7 @@ typedef cudaStream_t S;
     X(llmx_attention_plain, (const void*, int, const void*, int, void*, const int*, const int*, const int*, int, int,     \
                              int, int, int, int, int, float, S))                                                          \
     X(llmx_attention_pages, (const void*, int, const void*, const void*, int, void*, const int*, const int*, const int*, const int*,  \
-                             int, const void*, int, int, int, int, int, int, int, int, int, int, int, float, void*, long long, S))    \
+                             int, const void*, int, int, int, int, int, int, int, int, int, int, int, float, void*, long long, int*, S)) \
     X(llmx_attention_pages_workspace, (int, int, int, int, int, int, int, int, int, int, long long*))                         \
     X(llmx_expand_requests, (const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, int, int,    \
                              void*, int, int*, int, int*, int*, S))                                                       \
@@ -445,7 +445,7 @@ int pages_attention(Ctx& c, const llmx_pages_call& p) {
         void* at = room ? c.alloc((size_t)room) : nullptr;
         CALL(c, llmx_attention_pages, room ? 2 : 1, p.q, p.q_dtype, p.cache, p.exponents, p.cache_dtype, p.out, p.row_start, p.row_count, p.history,
              p.tables, p.table_stride, p.tree, p.tree_words, p.requests, p.total_rows, max_rows, p.max_context, p.pages, p.heads, p.kv_heads,
-             p.head_dim, p.page_size, p.window, p.scale, at, room, c.stream);
+             p.head_dim, p.page_size, p.window, p.scale, at, room, p.error_word, c.stream);
     };
     // Many rows: their keys and values become bfloat16 once (exact), and the prompt kernel runs over them.  Its tiles of 128 pairs are
     // half empty below FEW_PAIRS.
