@@ -54,7 +54,8 @@ struct Shape {
     static constexpr int S_COLS = EIGHT ? 2 * R : R, O_COLS = EIGHT ? 3 * R : R, U_COLS = 2 * S_COLS + O_COLS;
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
     static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + U * BUFFERS * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
-    // What a unit's threads tell each other, in floats: factors, minus the two maxima, what raising scales the two by, positions [R];
+    // What a unit's threads tell each other, in floats: factors, minus the sum's reference, the weights' beside it, what raising scales
+    // the two by, positions [R];
     // maxima and sums of warps [2][4][R].
     static constexpr int UNIT_FLOATS = 6 * R + 2 * UNIT_WARPS * R;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
@@ -78,10 +79,25 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes),
-                 "r"(tc::smem_u32(bar))
-                 : "memory");
+// An arrival once this thread's asynchronous copies so far have landed (one of those that the barrier counts).
+__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool is_done(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(tc::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ float warp_most(float v) {            // NaN aside
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 // A barrier of a unit's threads; true for all if it is for one.
 __device__ __forceinline__ bool unit_any(int unit, bool mine) {
@@ -164,7 +180,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     const int ratio = heads / kv_heads;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
+        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 17 : 1), tc::mbar_init(&empty[i], 1);     // (copies' bytes; 16 lanes' exponents)
         for (int u = 0; u < U; ++u) {
             tc::mbar_init(&q_full[u], UNIT_WARPS);
             for (int i = 0; i < 2; ++i) {
@@ -252,18 +268,20 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 const unsigned runs = __ballot_sync(0xffffffffu, real) & 0xffu;
                 if (lane == 0) {
                     live[stage] = (int)runs;
-                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * (16 * D * (EIGHT ? 1 : 2) + (EIGHT ? 16 : 0)));
+                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * 16 * D * (EIGHT ? 1 : 2));
                 }
                 __syncwarp();
-                if (real) {
-                    const unsigned row = (((unsigned)page * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
-                    uint8_t* to = smem + stage * S::STAGE + plane * S::PLANE;
-                    if constexpr (EIGHT) {
-                        if (second) copy_bulk(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16, exponents + row, 16, &full[stage]);
-                        else tc::tma_load_2d(to + p * 16 * 128, &map, 0, (int)row, &full[stage]);
-                    } else {
-                        tc::tma_load_2d(to + second * (S::PLANE / 2) + p * 16 * 128, &map, 64 * second, (int)row, &full[stage]);
+                const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+                uint8_t* to = smem + stage * S::STAGE + plane * S::PLANE;
+                if constexpr (EIGHT) {
+                    if (second) {
+                        if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
+                        arrive_after_copies(&full[stage]);
+                    } else if (real) {
+                        tc::tma_load_2d(to + p * 16 * 128, &map, 0, (int)row, &full[stage]);
                     }
+                } else if (real) {
+                    tc::tma_load_2d(to + second * (S::PLANE / 2) + p * 16 * 128, &map, 64 * second, (int)row, &full[stage]);
                 }
             }
         }
@@ -330,11 +348,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem + unit * S::U_COLS + lanes, o_at = s_at + 2 * S::S_COLS;
         float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
-        float *factor = shared, *minus_peak = shared + R, *minus_top = shared + 2 * R, *fade_sum = shared + 3 * R, *fade_o = shared + 4 * R;
+        float *factor = shared, *minus_peak = shared + R, *shift = shared + 2 * R, *fade_sum = shared + 3 * R, *fade_o = shared + 4 * R;
         int* position = reinterpret_cast<int*>(shared + 5 * R);
         float *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
-        const uint32_t rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
+        const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + unit * S::BUFFERS * S::WEIGHTS) + key * 128;
         uint32_t use = 0;
         bool ok = true, first_segment = true;
@@ -392,7 +410,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 }
                 if (part == 0) {
                     factor[row] = f;
-                    minus_peak[row] = minus_top[row] = -NONE;
+                    minus_peak[row] = shift[row] = 0.0f;
                     position[row] = real ? history + token : -1;
                 }
                 tc::fence_proxy_async();
@@ -409,8 +427,21 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             for (int i = 0; i < sg.tiles; ++i, ++use) {
                 const int stage = use % STAGES, s_buffer = use & 1, w_buffer = use % S::BUFFERS;
                 const int t0 = (sg.from + i) * KEYS, t = t0 + key;
-                if (ok) ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                const int runs = live[stage];
+                // The tile's copies, its scores, and that the weights' buffer is free again: asked for together, since an answer takes long.
+                const bool reused = use >= (uint32_t)S::BUFFERS;
+                const uint32_t w_parity = ((use / S::BUFFERS) & 1u) ^ 1u;
+                if (ok) {
+                    const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (use >> 1) & 1u),
+                               a2 = !reused || is_done(&o_done[2 * unit + w_buffer], w_parity);
+                    if (!__all_sync(0xffffffffu, a0 && a1 && a2)) {
+                        ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                        if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (use >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                        if (ok && reused) ok = tc::mbar_wait_warp(&o_done[2 * unit + w_buffer], w_parity, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                    }
+                }
+                tc::tc_fence_after();
+                int runs;
+                asm volatile("ld.shared.s32 %0, [%1];" : "=r"(runs) : "r"(live_at + 4 * stage) : "memory");
                 const bool dead = !(runs >> (key >> 4) & 1);     // a page that is not in the cache: a key of zeros
                 float k_power = 1.0f, v_power = 0.0f;
                 if constexpr (EIGHT) {
@@ -454,11 +485,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         if (!sees) hidden |= 1u << n;
                     }
                 }
-                if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (use >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                tc::tc_fence_after();
-                // ---- the exponents: x of the sum, y of the weights
-                float x[R], y[EIGHT ? R : 1];
-                auto scores = [&](auto&& take) {                 // score by score, without their rows' factors
+                // ---- what the sum's exponentials are of: scores, less the row's reference
+                float x[R];
+                auto scores = [&](bool raw) {
 #pragma unroll
                     for (int c = 0; c < CHUNKS; ++c) {
                         float z[16];
@@ -480,59 +509,63 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                             for (int n = 0; n < 16; ++n) z[n] = hidden >> (16 * c + n) & 1u ? -INFINITY : dead ? 0.0f : z[n];
                         }
 #pragma unroll
-                        for (int n = 0; n < 16; n += 4) take(16 * c + n, z[n], z[n + 1], z[n + 2], z[n + 3]);
+                        for (int n = 0; n < 16; n += 4) {
+                            const float4 f = shared4(rows_at + 4 * (16 * c + n)),
+                                         mp = raw ? make_float4(0.f, 0.f, 0.f, 0.f) : shared4(rows_at + 4 * (R + 16 * c + n));
+                            x[16 * c + n] = fmaf(z[n], f.x, mp.x), x[16 * c + n + 1] = fmaf(z[n + 1], f.y, mp.y);
+                            x[16 * c + n + 2] = fmaf(z[n + 2], f.z, mp.z), x[16 * c + n + 3] = fmaf(z[n + 3], f.w, mp.w);
+                        }
                     }
                 };
-                for (int again = 0; again < 2; ++again) {
+                scores(false);                                   // (a segment's first tile: references of zero)
+                bool raise = i == 0;
+                if (i > 0) {
                     float over = -INFINITY;
-                    scores([&](int n, float z0, float z1, float z2, float z3) {
-                        const float4 f = shared4(rows_at + 4 * n), mp = shared4(rows_at + 4 * (R + n));
-                        x[n] = fmaf(z0, f.x, mp.x), x[n + 1] = fmaf(z1, f.y, mp.y), x[n + 2] = fmaf(z2, f.z, mp.z), x[n + 3] = fmaf(z3, f.w, mp.w);
+#pragma unroll
+                    for (int n = 0; n < R; n += 4) {
                         if constexpr (EIGHT) {
-                            const float4 mt = shared4(rows_at + 4 * (2 * R + n));
-                            y[n] = fmaf(z0, f.x, mt.x + v_power), y[n + 1] = fmaf(z1, f.y, mt.y + v_power);
-                            y[n + 2] = fmaf(z2, f.z, mt.z + v_power), y[n + 3] = fmaf(z3, f.w, mt.w + v_power);
-                            over = max3(max3(over, x[n], y[n]), x[n + 1], y[n + 1]);
-                            over = max3(max3(over, x[n + 2], y[n + 2]), x[n + 3], y[n + 3]);
+                            const float4 s = shared4(rows_at + 4 * (2 * R + n));
+                            over = max3(max3(over, x[n], x[n] + (s.x + v_power)), x[n + 1], x[n + 1] + (s.y + v_power));
+                            over = max3(max3(over, x[n + 2], x[n + 2] + (s.z + v_power)), x[n + 3], x[n + 3] + (s.w + v_power));
                         } else {
                             over = max3(max3(over, x[n], x[n + 1]), x[n + 2], x[n + 3]);
                         }
-                    });
-                    if (!unit_any(unit, again == 0 && over > LIMIT)) break;
+                    }
+                    raise = unit_any(unit, over > LIMIT);
+                    if (raise) scores(true);
+                }
+                if (raise) {
                     // ---- the references rise to this tile's maxima
-                    scores([&](int n, float z0, float z1, float z2, float z3) {
-                        const float z[4] = {z0, z1, z2, z3};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float p = z[k] * factor[n + k], w = p + v_power;
-#pragma unroll
-                            for (int o = 16; o > 0; o >>= 1) {
-                                p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, o));
-                                if (EIGHT) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-                            }
-                            if (lane == 0) warp_peak[quarter * R + n + k] = p, warp_top[quarter * R + n + k] = w;
-                        }
-                    });
+                    for (int n = 0; n < R; ++n) {
+                        const float p = warp_most(x[n]), w = EIGHT ? warp_most(x[n] + v_power) : p;
+                        if (lane == 0) warp_peak[quarter * R + n] = p, warp_top[quarter * R + n] = w;
+                    }
                     unit_barrier(unit);
                     if (thread < R) {
                         const int n = thread;
                         float p = NONE, w = NONE;
 #pragma unroll
                         for (int k = 0; k < UNIT_WARPS; ++k) p = fmaxf(p, warp_peak[k * R + n]), w = fmaxf(w, warp_top[k * R + n]);
-                        const float before = -minus_peak[n], now = fmaxf(before, p == NONE ? NONE : EIGHT ? p + ROOM : p);
-                        const float top_before = -minus_top[n], top_now = EIGHT ? fmaxf(top_before, w == NONE ? NONE : w - RAISED) : now;
+                        const float before = i > 0 ? -minus_peak[n] : NONE, now = fmaxf(before, EIGHT && p > NONE ? p + ROOM : p);
+                        const float top_before = i > 0 ? before - shift[n] : NONE, top_now = EIGHT ? fmaxf(top_before, w > NONE ? w - RAISED : w) : now;
                         fade_sum[n] = exp2_fast(before - now);
                         fade_o[n] = EIGHT ? exp2_fast(top_before - top_now) : fade_sum[n];
-                        minus_peak[n] = -now, minus_top[n] = -top_now;
+                        minus_peak[n] = -now, shift[n] = now - top_now;
                     }
                     unit_barrier(unit);
 #pragma unroll
-                    for (int n = 0; n < R; ++n) sum[n] *= fade_sum[n];
+                    for (int n = 0; n < R; n += 4) {
+                        const float4 mp = shared4(rows_at + 4 * (R + n));
+                        x[n] += mp.x, x[n + 1] += mp.y, x[n + 2] += mp.z, x[n + 3] += mp.w;
+                    }
                     if (i > 0) {
                         // Every O^T that has been asked for has been made before it is scaled.
                         const uint32_t last = use - 1;
                         if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                         tc::tc_fence_after();
+#pragma unroll
+                        for (int n = 0; n < R; ++n) sum[n] *= fade_sum[n];
 #pragma unroll
                         for (int c = 0; c < S::O_COLS / 16; ++c) {
                             uint32_t v[16];
@@ -549,12 +582,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s_free[2 * unit + s_buffer]);
                 // ---- weights
-                if (use >= (uint32_t)S::BUFFERS && ok)           // the buffer's weights before have been used
-                    ok = tc::mbar_wait_warp(&o_done[2 * unit + w_buffer], ((use / S::BUFFERS) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                 const uint32_t weights = weights_at + w_buffer * S::WEIGHTS;
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     uint32_t h[8];
+                    float4 s;
 #pragma unroll
                     for (int n = 0; n < 16; n += 2) {
                         const int row = 16 * c + n;
@@ -562,7 +594,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         sum[row] += e0;
                         sum[row + 1] += e1;
                         if constexpr (EIGHT) {
-                            h[n >> 1] = mma_pages::pack_half(exp2_fast(y[row]), exp2_fast(y[row + 1]));
+                            if (n % 4 == 0) s = shared4(rows_at + 4 * (2 * R + row));
+                            const float s0 = n % 4 == 0 ? s.x : s.z, s1 = n % 4 == 0 ? s.y : s.w;
+                            h[n >> 1] = mma_pages::pack_half(exp2_fast(x[row] + (s0 + v_power)), exp2_fast(x[row + 1] + (s1 + v_power)));
                         } else {
                             h[n >> 1] = mma_pages::pack_bf16(e0, e1);
                             if (stray)
@@ -637,7 +671,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     if (pair >= pairs) continue;
                     if (any_stray) o[n] += strays[row * D + key];
                     const float total = (warp_peak[row] + warp_peak[R + row]) + (warp_peak[2 * R + row] + warp_peak[3 * R + row]);
-                    const float peak = -minus_peak[row], top = -minus_top[row];
+                    const float peak = -minus_peak[row], top = peak - shift[row];
                     if (sg.whole) {
                         const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
                         out[((size_t)(start + pair / ratio) * heads + sg.kv * ratio + pair % ratio) * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
