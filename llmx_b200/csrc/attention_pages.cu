@@ -185,18 +185,18 @@ int pages_map(CUtensorMap* map, const void* cache, bool eight, uint64_t rows) {
                : 10003;
 }
 
-template <bool EIGHT, int U, int R>
+template <bool EIGHT, bool SHARED, int R>
 int tensor_rows(const FewPlan& p, const void* q, const void* cache, const void* exponents, void* out, float* partial, const Rows& a, int requests,
                 int max_rows, int heads, int kv_heads, float scale, int* error_word, cudaStream_t stream) {
     using namespace tc_pages;
     CUtensorMap map;
     if (const int e = pages_map(&map, cache, EIGHT, (uint64_t)a.pages * 2 * kv_heads * a.page_size)) return e;
-    LLMX_ALLOW_SMEM(pages_kernel<EIGHT, U, R>);
-    launch_kernel(pages_kernel<EIGHT, U, R>, dim3((unsigned)p.blocks), dim3(tc_pages::Shape<EIGHT, U, R>::THREADS),
-                  (size_t)tc_pages::Shape<EIGHT, U, R>::BYTES, stream, map, (const __nv_bfloat16*)q, (const uint8_t*)exponents, (__nv_bfloat16*)out, partial, a,
+    LLMX_ALLOW_SMEM(pages_kernel<EIGHT, SHARED, R>);
+    launch_kernel(pages_kernel<EIGHT, SHARED, R>, dim3((unsigned)p.blocks), dim3(tc_pages::Shape<EIGHT, SHARED, R>::THREADS),
+                  (size_t)tc_pages::Shape<EIGHT, SHARED, R>::BYTES, stream, map, (const __nv_bfloat16*)q, (const uint8_t*)exponents, (__nv_bfloat16*)out, partial, a,
                   requests, heads, kv_heads, scale * 1.4426950408889634f, error_word);
     if (const int e = launch_status()) return e;
-    return merge<__nv_bfloat16, EIGHT, 128, U * R, KEYS, 1>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
+    return merge<__nv_bfloat16, EIGHT, 128, SHARED ? R : 2 * R, KEYS, 1>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
 }
 }  // namespace
 
@@ -231,13 +231,13 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
 #define LLMX_FEW_ARGS p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale
         if (p.tensor) {
             if (cache_dtype == LLMX_E4M3) {
-                if (p.rows == 16) return tensor_rows<true, 1, 16>(LLMX_FEW_ARGS, error_word, stream);
-                if (p.rows == 32) return tensor_rows<true, 2, 16>(LLMX_FEW_ARGS, error_word, stream);
-                return tensor_rows<true, 2, 32>(LLMX_FEW_ARGS, error_word, stream);
+                if (p.rows == 16) return tensor_rows<true, true, 16>(LLMX_FEW_ARGS, error_word, stream);
+                if (p.rows == 32) return tensor_rows<true, true, 32>(LLMX_FEW_ARGS, error_word, stream);
+                return tensor_rows<true, false, 32>(LLMX_FEW_ARGS, error_word, stream);
             }
-            if (p.rows == 16) return tensor_rows<false, 1, 16>(LLMX_FEW_ARGS, error_word, stream);
-            if (p.rows == 32) return tensor_rows<false, 2, 16>(LLMX_FEW_ARGS, error_word, stream);
-            return tensor_rows<false, 2, 32>(LLMX_FEW_ARGS, error_word, stream);
+            if (p.rows == 16) return tensor_rows<false, true, 16>(LLMX_FEW_ARGS, error_word, stream);
+            if (p.rows == 32) return tensor_rows<false, true, 32>(LLMX_FEW_ARGS, error_word, stream);
+            return tensor_rows<false, false, 32>(LLMX_FEW_ARGS, error_word, stream);
         }
 #define LLMX_FEW_ROWS(QT, EIGHT, D)                                                         \
     do {                                                                                    \

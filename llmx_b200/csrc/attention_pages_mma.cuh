@@ -238,8 +238,8 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
     constexpr int STAGES = S::STAGES, RUNS = WARPS / RW;         // groups of warps that each walk keys of their own
     constexpr int PARTS = EIGHT && sizeof(QT) == 4 ? 2 : 1;
     constexpr int STEPS = D / 16, TILES = D / 8, TILE_ROWS = 16 * RW, ROWF = D + PART;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();                       // (in this order: the merge reads the requests' counts without waiting)
     extern __shared__ __align__(256) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int run = warp / RW, rw = warp % RW;
@@ -621,13 +621,13 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int RUNS>
 __global__ void __launch_bounds__(128)
 merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, int requests, int heads, int kv_heads, int grid) {
-    pdl_trigger();
-    pdl_wait();
     constexpr int ROWF = D + PART, LANES = D / 4, EACH = 128 / LANES;
     const int r = blockIdx.y, ratio = heads / kv_heads;
+    // The kernel before let this one start when the kernels before it had ended: the requests' counts stand.  Every thread waits before
+    // it returns all the same: who waits for this kernel waits for that one by it.
     const Request rq = request_of<KEYS>(a, r, ratio, TILE_ROWS);
     const long long first_item = (long long)blockIdx.x * EACH;
-    if (first_item >= (long long)rq.count * heads) return;
+    if (first_item >= (long long)rq.count * heads) return pdl_wait();
     int found;
     long long items, unused;
     const long long all = tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
@@ -635,12 +635,13 @@ merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, in
     // The place of this request's tiles: before it lie those of the requests 0 .. r - 1.
     const long long request_at = tiles_before<KEYS>(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
     const long long item = first_item + threadIdx.x / LANES;
-    if (item >= (long long)rq.count * heads) return;
+    if (item >= (long long)rq.count * heads) return pdl_wait();
     const int row = (int)(item / heads), head = (int)(item % heads), kv = head / ratio, pair = row * ratio + head % ratio, d = 4 * (threadIdx.x % LANES);
     const long long x0 = request_at + ((long long)(pair / TILE_ROWS) * kv_heads + kv) * rq.tiles, x1 = x0 + rq.tiles;
     // Block b has the tiles all * b / blocks up to all * (b + 1) / blocks.
     auto block_of = [&](long long x) { return (int)(((x + 1) * blocks - 1) / all); };
     const int b0 = block_of(x0), b1 = block_of(x1 - 1);
+    pdl_wait();
     if (b0 == b1) return;
     // A block's first segment lies in its first slot; the item is that of all blocks but the first, unless that one begins with it.
     const int slot0 = 2 * b0 + (all * b0 / blocks < x0 ? 1 : 0);

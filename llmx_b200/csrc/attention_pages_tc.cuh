@@ -13,8 +13,10 @@
 // own, whose sums are added up in 32 bits.  As in the warp form a value's power of two joins its key's score.
 //
 //   warp 0          page lookups and copies, 16 keys (or their exponents) a lane, STAGES tiles ahead
-//   warp 1          matrix instructions: S^T of the next tile before O^T of this one
-//   warps 2 ..      units of four warps, each with R of the rows: exponentials, weights to shared memory
+//   warp 1          matrix instructions, whichever can be made next: S^T of tiles ahead, O^T
+//   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
+//                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
+//                   tile's rows are R; their states meet at the item's end), or half of the rows each (2 R)
 // The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^4 of them has the unit
 // raise them, and its sums and outputs (in tensor memory) scaled.  Every wait is bounded; the softmax warps go on through their
 // barriers without waiting once one has run out.
@@ -42,8 +44,9 @@ constexpr float RAISED = 4.0f, ROOM = 57.0f, LIMIT = 8.0f;
 constexpr float NONE = -1.0e30f;        // a maximum of no keys
 enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 503 };
 
-template <bool EIGHT, int U, int R>
+template <bool EIGHT, bool SHARED, int R>
 struct Shape {
+    static constexpr int U = 2;
     static constexpr int THREADS = 64 + U * UNIT_WARPS * 32;
     static constexpr int PLANE = KEYS * D * (EIGHT ? 1 : 2);
     static constexpr int STAGE = 2 * PLANE;
@@ -112,6 +115,7 @@ __device__ __forceinline__ bool unit_any(int unit, bool mine) {
         : "memory");
     return r != 0;
 }
+__device__ __forceinline__ void units_barrier() { asm volatile("barrier.cta.sync 7, 256;" ::: "memory"); }      // of both units
 __device__ __forceinline__ void unit_barrier(int unit) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + unit) : "memory"); }
 
 __device__ __forceinline__ float4 shared4(uint32_t at) {
@@ -156,13 +160,13 @@ __device__ __forceinline__ uint4 take_codes(uint32_t (&h)[8], bool more) {
     return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
 }
 
-template <bool EIGHT, int U, int R>
-__global__ void __launch_bounds__(Shape<EIGHT, U, R>::THREADS, 1)
+template <bool EIGHT, bool SHARED, int R>
+__global__ void __launch_bounds__(Shape<EIGHT, SHARED, R>::THREADS, 1)
 pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ exponents,
              __nv_bfloat16* __restrict__ out, float* __restrict__ partial, Rows a, int requests, int heads, int kv_heads, float scale_log2,
              int* error_word) {
-    using S = Shape<EIGHT, U, R>;
-    constexpr int TILE_ROWS = U * R, ROWF = D + PART, STAGES = S::STAGES, CHUNKS = R / 16;
+    using S = Shape<EIGHT, SHARED, R>;
+    constexpr int U = S::U, TILE_ROWS = SHARED ? R : U * R, ROWF = D + PART, STAGES = S::STAGES, CHUNKS = R / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = (uint64_t*)(smem + S::AT_BARRIERS);        // [STAGES]
@@ -209,8 +213,10 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_trigger();                       // (only now: a dependent block must not take the tensor memory that this one waits for)
+    // Dependents may start only now that this block holds its tensor memory (they must not take what it waits for) and the kernels before
+    // have ended (the merge reads the requests' counts without waiting).
     pdl_wait();
+    pdl_trigger();
 
     // ---- the work, which every role walks alike
     int r0;
@@ -287,59 +293,84 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         }
     } else if (warp == 1) {
         if (tc::elect_one()) {
-            uint32_t use = 0, segments = 0;
+            uint32_t use = 0, segments = 0, scored[U] = {0, 0}, weighed[U] = {0, 0};       // tiles so far; units' S^T and O^T so far
             bool ok = true;
-            auto scores = [&](uint32_t n) -> bool {              // S^T of tile use n
-                const int stage = n % STAGES, buffer = n & 1;
-                if (!tc::mbar_wait(&full[stage], (n / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_MMA)) return false;
-                const uint32_t keys = tc::smem_u32(smem + stage * S::STAGE);
-                for (int u = 0; u < U; ++u) {
-                    if (!tc::mbar_wait(&s_free[2 * u + buffer], ((n >> 1) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_MMA)) return false;
-                    tc::tc_fence_after();
-                    const uint32_t queries = tc::smem_u32(smem + S::AT_QUERIES + u * S::QUERIES), d = tmem + u * S::U_COLS + buffer * S::S_COLS;
-                    if constexpr (EIGHT) {
-#pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
-                            mma_e4m3(d, tc::smem_desc_k_sw128(keys + k * 32), tc::smem_desc_k_sw128(queries + k * 32), instruction_e4m3(KEYS, 2 * R), k > 0);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            tc::mma_bf16_ss(d, tc::smem_desc_k_sw128(keys + (k >> 2) * (S::PLANE / 2) + (k & 3) * 32),
-                                            tc::smem_desc_k_sw128(queries + (k >> 2) * (R * 128) + (k & 3) * 32), tc::instr_desc_bf16(KEYS, R), k > 0);
-                    }
-                    tc::mma_commit(&s_full[2 * u + buffer]);
-                }
-                return true;
-            };
             while (ok && next_segment()) {
                 for (int u = 0; u < U && ok; ++u) ok = tc::mbar_wait(&q_full[u], segments & 1u, abort_flag, error_word, ERR_PAGES_MMA);
                 ++segments;
-                tc::tc_fence_after();
-                if (ok) ok = scores(use);
-                for (int i = 0; i < sg.tiles && ok; ++i, ++use) {
-                    if (i + 1 < sg.tiles) ok = scores(use + 1);
-                    const int stage = use % STAGES, buffer = use % S::BUFFERS;
-                    for (int u = 0; u < U && ok; ++u) {
-                        ok = tc::mbar_wait(&w_full[2 * u + buffer], (use / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_MMA);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + S::PLANE), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
-                        const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + (u * S::BUFFERS + buffer) * S::WEIGHTS);
-                        if constexpr (EIGHT) {
+                // S^T of tile `next`, O^T of `tile` (of unit `turn`, where both units have every tile): whichever finds what it needs.
+                int next = 0, tile = 0, turn = 0;
+                unsigned long long since = 0;
+                for (uint32_t idle = 0; tile < sg.tiles && ok;) {
+                    bool made = false;
+                    if (next < sg.tiles) {
+                        const int stage = (use + next) % STAGES, u0 = SHARED ? next & 1 : 0, u1 = SHARED ? u0 : U - 1;
+                        bool ready = is_done(&full[stage], ((use + next) / STAGES) & 1u);
+                        for (int u = u0; u <= u1; ++u) ready = ready && is_done(&s_free[2 * u + (scored[u] & 1)], ((scored[u] >> 1) & 1u) ^ 1u);
+                        if (ready) {
+                            tc::tc_fence_after();
+                            const uint32_t keys = tc::smem_u32(smem + stage * S::STAGE);
+                            for (int u = u0; u <= u1; ++u) {
+                                const int buffer = scored[u]++ & 1;
+                                const uint32_t queries = tc::smem_u32(smem + S::AT_QUERIES + u * S::QUERIES), d = tmem + u * S::U_COLS + buffer * S::S_COLS;
+                                if constexpr (EIGHT) {
 #pragma unroll
-                            for (int k = 0; k < KEYS / 32; ++k)
-                                mma_e4m3(d, desc_mn(values + k * 4096, S::PLANE), desc_mn(weights + k * 4096, S::WEIGHTS),
-                                         instruction_e4m3(D, 3 * R) | TRANSPOSED, i > 0 || k > 0);
-                        } else {
+                                    for (int k = 0; k < D / 32; ++k)
+                                        mma_e4m3(d, tc::smem_desc_k_sw128(keys + k * 32), tc::smem_desc_k_sw128(queries + k * 32), instruction_e4m3(KEYS, 2 * R),
+                                                 k > 0);
+                                } else {
 #pragma unroll
-                            for (int k = 0; k < KEYS / 16; ++k)
-                                tc::mma_bf16_ss(d, desc_mn(values + k * 2048, S::PLANE / 2), desc_mn(weights + k * 2048, S::WEIGHTS),
-                                                tc::instr_desc_bf16(D, R) | TRANSPOSED, i > 0 || k > 0);
+                                    for (int k = 0; k < D / 16; ++k)
+                                        tc::mma_bf16_ss(d, tc::smem_desc_k_sw128(keys + (k >> 2) * (S::PLANE / 2) + (k & 3) * 32),
+                                                        tc::smem_desc_k_sw128(queries + (k >> 2) * (R * 128) + (k & 3) * 32), tc::instr_desc_bf16(KEYS, R), k > 0);
+                                }
+                                tc::mma_commit(&s_full[2 * u + buffer]);
+                            }
+                            ++next;
+                            made = true;
                         }
-                        if (u == U - 1) tc::mma_commit(&empty[stage]);
-                        tc::mma_commit(&o_done[2 * u + buffer]);
+                    }
+                    if (tile < next) {
+                        const int u = SHARED ? tile & 1 : turn, stage = (use + tile) % STAGES, buffer = weighed[u] % S::BUFFERS;
+                        if (is_done(&w_full[2 * u + buffer], (weighed[u] / S::BUFFERS) & 1u)) {
+                            tc::tc_fence_after();
+                            const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + S::PLANE), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
+                            const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + (u * S::BUFFERS + buffer) * S::WEIGHTS);
+                            const bool begun = SHARED ? tile > 1 : tile > 0;
+                            if constexpr (EIGHT) {
+#pragma unroll
+                                for (int k = 0; k < KEYS / 32; ++k)
+                                    mma_e4m3(d, desc_mn(values + k * 4096, S::PLANE), desc_mn(weights + k * 4096, S::WEIGHTS),
+                                             instruction_e4m3(D, 3 * R) | TRANSPOSED, begun || k > 0);
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < KEYS / 16; ++k)
+                                    tc::mma_bf16_ss(d, desc_mn(values + k * 2048, S::PLANE / 2), desc_mn(weights + k * 2048, S::WEIGHTS),
+                                                    tc::instr_desc_bf16(D, R) | TRANSPOSED, begun || k > 0);
+                            }
+                            ++weighed[u];
+                            const bool last = SHARED || turn == U - 1;
+                            if (last) tc::mma_commit(&empty[stage]);
+                            tc::mma_commit(&o_done[2 * u + buffer]);
+                            turn = last ? 0 : turn + 1;
+                            tile += last;
+                            made = true;
+                        }
+                    }
+                    if (made) {
+                        idle = 0;
+                    } else if ((++idle & 255u) == 0) {
+                        const unsigned long long now = tc::global_ns();
+                        if (idle == 256) since = now;
+                        if (*abort_flag) ok = false;
+                        else if (now - since > tc::WAIT_LIMIT_NS) {
+                            *abort_flag = 1;
+                            if (error_word) atomicCAS(error_word, 0, ERR_PAGES_MMA);
+                            ok = false;
+                        }
                     }
                 }
+                use += sg.tiles;
             }
         }
     } else {
@@ -354,10 +385,10 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + unit * S::BUFFERS * S::WEIGHTS) + key * 128;
-        uint32_t use = 0;
+        uint32_t before = 0, mine = 0;                          // tiles of the segments before; this unit's so far
         bool ok = true, first_segment = true;
-        for (; next_segment(); first_segment = false) {
-            const int first = sg.first + unit * R, pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
+        for (; next_segment(); before += sg.tiles, first_segment = false) {
+            const int first = sg.first + (SHARED ? 0 : unit * R), pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
             // ---- the unit's queries: a row by 128 / R threads
             {
                 constexpr int EACH = 128 / R, OWN = D / EACH;
@@ -424,18 +455,20 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             float sum[R];
 #pragma unroll
             for (int n = 0; n < R; ++n) sum[n] = 0.0f;
-            for (int i = 0; i < sg.tiles; ++i, ++use) {
-                const int stage = use % STAGES, s_buffer = use & 1, w_buffer = use % S::BUFFERS;
+            for (int i = SHARED ? unit : 0; i < sg.tiles; i += SHARED ? 2 : 1, ++mine) {
+                const bool opening = i < (SHARED ? 2 : 1);       // the unit's first tile of the item
+                const uint32_t use = before + i;
+                const int stage = use % STAGES, s_buffer = mine & 1, w_buffer = mine % S::BUFFERS;
                 const int t0 = (sg.from + i) * KEYS, t = t0 + key;
                 // The tile's copies, its scores, and that the weights' buffer is free again: asked for together, since an answer takes long.
-                const bool reused = use >= (uint32_t)S::BUFFERS;
-                const uint32_t w_parity = ((use / S::BUFFERS) & 1u) ^ 1u;
+                const bool reused = mine >= (uint32_t)S::BUFFERS;
+                const uint32_t w_parity = ((mine / S::BUFFERS) & 1u) ^ 1u;
                 if (ok) {
-                    const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (use >> 1) & 1u),
+                    const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u),
                                a2 = !reused || is_done(&o_done[2 * unit + w_buffer], w_parity);
                     if (!__all_sync(0xffffffffu, a0 && a1 && a2)) {
                         ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                        if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (use >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                        if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                         if (ok && reused) ok = tc::mbar_wait_warp(&o_done[2 * unit + w_buffer], w_parity, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                     }
                 }
@@ -517,9 +550,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         }
                     }
                 };
-                scores(false);                                   // (a segment's first tile: references of zero)
-                bool raise = i == 0;
-                if (i > 0) {
+                scores(false);                                   // (the first tile: references of zero)
+                bool raise = opening;
+                if (!opening) {
                     float over = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < R; n += 4) {
@@ -547,10 +580,10 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         float p = NONE, w = NONE;
 #pragma unroll
                         for (int k = 0; k < UNIT_WARPS; ++k) p = fmaxf(p, warp_peak[k * R + n]), w = fmaxf(w, warp_top[k * R + n]);
-                        const float before = i > 0 ? -minus_peak[n] : NONE, now = fmaxf(before, EIGHT && p > NONE ? p + ROOM : p);
-                        const float top_before = i > 0 ? before - shift[n] : NONE, top_now = EIGHT ? fmaxf(top_before, w > NONE ? w - RAISED : w) : now;
-                        fade_sum[n] = exp2_fast(before - now);
-                        fade_o[n] = EIGHT ? exp2_fast(top_before - top_now) : fade_sum[n];
+                        const float old = opening ? NONE : -minus_peak[n], now = fmaxf(old, EIGHT && p > NONE ? p + ROOM : p);
+                        const float top_old = opening ? NONE : old - shift[n], top_now = EIGHT ? fmaxf(top_old, w > NONE ? w - RAISED : w) : now;
+                        fade_sum[n] = exp2_fast(old - now);
+                        fade_o[n] = EIGHT ? exp2_fast(top_old - top_now) : fade_sum[n];
                         minus_peak[n] = -now, shift[n] = now - top_now;
                     }
                     unit_barrier(unit);
@@ -559,9 +592,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         const float4 mp = shared4(rows_at + 4 * (R + n));
                         x[n] += mp.x, x[n + 1] += mp.y, x[n + 2] += mp.z, x[n + 3] += mp.w;
                     }
-                    if (i > 0) {
+                    if (!opening) {
                         // Every O^T that has been asked for has been made before it is scaled.
-                        const uint32_t last = use - 1;
+                        const uint32_t last = mine - 1;
                         if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                         tc::tc_fence_after();
 #pragma unroll
@@ -621,7 +654,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 if constexpr (!EIGHT)
                     if (a.tree && t0 + KEYS > history) {
                         // No unit takes such values away before all have read them.
-                        asm volatile("barrier.cta.sync 7, %0;" ::"n"(U * UNIT_WARPS * 32) : "memory");
+                        if (!SHARED) units_barrier();
                         if (stray)
                             for (int d = 0; d < D; ++d) {
                                 unsigned short* x = value_in<S::PLANE / 2>(value_row, key, d);
@@ -635,21 +668,23 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             }
 
             // ---- the item's sums over this block's keys: a thread has one of the 128 values of every row
-            const uint32_t last = use - 1;
+            const bool any_tile = !SHARED || unit < sg.tiles;    // (an item of one tile leaves the second unit none)
+            const uint32_t last = mine - 1;
 #pragma unroll
             for (int n = 0; n < R; ++n) {
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], o);
                 if (lane == 0) warp_peak[quarter * R + n] = sum[n];
             }
-            if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+            if (ok && any_tile) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
             tc::tc_fence_after();
             unit_barrier(unit);
             const bool any_stray = !EIGHT && stray_flag[unit];
             float* slot = partial + (2 * (size_t)blockIdx.x + !first_segment) * TILE_ROWS * ROWF;
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                float o[16];
+            // The second unit's sums go to the first by way of its weights' place.
+            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS + S::BUFFERS * S::WEIGHTS);
+            const bool both = SHARED && sg.tiles > 1;
+            auto outputs = [&](int c, float (&o)[16]) {
                 uint32_t v[16];
                 tc::tmem_ld_32x16(o_at + (EIGHT ? 48 : 16) * c, v);
                 tc::tmem_wait_ld();
@@ -665,25 +700,53 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
 #pragma unroll
                     for (int n = 0; n < 16; ++n) o[n] = fmaf(__uint_as_float(v[n]), 1.0f / 1024.0f, o[n]);
                 }
+                if (any_stray)
 #pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    const int row = 16 * c + n, pair = first + row;
-                    if (pair >= pairs) continue;
-                    if (any_stray) o[n] += strays[row * D + key];
-                    const float total = (warp_peak[row] + warp_peak[R + row]) + (warp_peak[2 * R + row] + warp_peak[3 * R + row]);
-                    const float peak = -minus_peak[row], top = peak - shift[row];
-                    if (sg.whole) {
-                        const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
-                        out[((size_t)(start + pair / ratio) * heads + sg.kv * ratio + pair % ratio) * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
-                    } else {
-                        float* to = slot + (size_t)(unit * R + row) * ROWF;
-                        to[key] = o[n];
-                        if (key < 3) to[D + key] = key == 0 ? top : key == 1 ? peak : total;
+                    for (int n = 0; n < 16; ++n) o[n] += strays[(16 * c + n) * D + key];
+            };
+            auto total_of = [&](const float* sums, int row) { return (sums[row] + sums[R + row]) + (sums[2 * R + row] + sums[3 * R + row]); };
+            if (SHARED && unit == 1) {
+                if (both)
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        float o[16];
+                        outputs(c, o);
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) given[(16 * c + n) * D + key] = o[n];
+                    }
+                units_barrier();
+            } else {
+                if (SHARED) units_barrier();
+                const float *theirs = shared + S::UNIT_FLOATS, *their_sums = theirs + 6 * R;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    float o[16];
+                    outputs(c, o);
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) {
+                        const int row = 16 * c + n, pair = first + row;
+                        if (pair >= pairs) continue;
+                        float total = total_of(warp_peak, row), peak = -minus_peak[row], top = peak - shift[row];
+                        if (both) {
+                            const float peak2 = -theirs[R + row], top2 = peak2 - theirs[2 * R + row], p = fmaxf(peak, peak2), t = fmaxf(top, top2);
+                            total = fmaf(total, exp2_fast(peak - p), total_of(their_sums, row) * exp2_fast(peak2 - p));
+                            o[n] = fmaf(o[n], exp2_fast(top - t), given[row * D + key] * exp2_fast(top2 - t));
+                            peak = p, top = t;
+                        }
+                        if (sg.whole) {
+                            const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
+                            out[((size_t)(start + pair / ratio) * heads + sg.kv * ratio + pair % ratio) * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
+                        } else {
+                            float* to = slot + (size_t)((SHARED ? 0 : unit * R) + row) * ROWF;
+                            to[key] = o[n];
+                            if (key < 3) to[D + key] = key == 0 ? top : key == 1 ? peak : total;
+                        }
                     }
                 }
             }
             tc::tc_fence_before();
-            unit_barrier(unit);                                  // before the next item's rows take this one's places
+            if (SHARED) units_barrier();                         // before the next item's rows take this one's places
+            else unit_barrier(unit);
             if (any_stray) {
                 for (int n = thread; n < R * D; n += 128) strays[n] = 0.0f;
                 stray_flag[unit] = 0;
