@@ -12,7 +12,7 @@
 // to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 16 + w3 / 256 (12 bits, down to 2^-26 of the largest): columns of their
 // own, whose sums are added up in 32 bits.  As in the warp form a value's power of two joins its key's score.
 //
-//   warp 0          page lookups and copies, 16 keys (or their exponents) a lane, STAGES tiles ahead
+//   warps 0, 10     page lookups and copies of keys and of values, 16 rows a copy, STAGES tiles ahead
 //   warp 1          matrix instructions, whichever can be made next: S^T of tiles ahead, O^T
 //   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
@@ -37,7 +37,7 @@ using mma_pages::request_of;
 using mma_pages::Rows;
 
 constexpr int KEYS = 128, D = 128;
-constexpr int UNIT_WARPS = 4;
+constexpr int UNIT_WARPS = 4, LOADER = 10;
 // The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
 // leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
 constexpr float RAISED = 4.0f, ROOM = 57.0f, LIMIT = 8.0f;
@@ -47,7 +47,7 @@ enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 
 template <bool EIGHT, bool SHARED, int R>
 struct Shape {
     static constexpr int U = 2;
-    static constexpr int THREADS = 64 + U * UNIT_WARPS * 32;
+    static constexpr int THREADS = 96 + U * UNIT_WARPS * 32;
     static constexpr int PLANE = KEYS * D * (EIGHT ? 1 : 2);
     static constexpr int STAGE = 2 * PLANE;
     static constexpr int STAGES = EIGHT ? 4 : 2;
@@ -184,7 +184,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     const int ratio = heads / kv_heads;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 17 : 1), tc::mbar_init(&empty[i], 1);     // (copies' bytes; 16 lanes' exponents)
+        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 18 : 2), tc::mbar_init(&empty[i], 1);     // (two loaders' bytes; 16 lanes' exponents)
         for (int u = 0; u < U; ++u) {
             tc::mbar_init(&q_full[u], UNIT_WARPS);
             for (int i = 0; i < 2; ++i) {
@@ -252,42 +252,44 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         return true;
     };
 
-    if (warp == 0) {
-        // Lane: a run of 16 keys, keys or values, and codes or exponents (bfloat16: the row's first or second half).
-        const int p = lane & 7, plane = (lane >> 3) & 1, second = lane >> 4;
+    if (warp == 0 || warp == LOADER) {
+        // Keys (warp 0) or values: a lane finds a run of 16 keys, one issues the copies.
+        const int p = lane & 7, plane = warp == LOADER;
         uint32_t use = 0;
         bool ok = true;
         while (ok && next_segment()) {
             const int* table = a.tables + (size_t)sg.r * a.table_stride;
+            // The pages of four tiles' 32 runs at a time, a lane each, asked for four tiles ahead: a lookup takes as long as a tile.
             auto look_up = [&](int i) {
-                const int n = (sg.from + i) * (KEYS / 16) + p;
-                return i < sg.tiles && n * 16 < sg.rq.end && n * 16 + 16 > sg.rq.low ? table[page_of(n)] : -1;
+                const int n = (sg.from + i) * (KEYS / 16) + lane;
+                return i + lane / 8 < sg.tiles && n * 16 < sg.rq.end && n * 16 + 16 > sg.rq.low ? table[page_of(n)] : -1;
             };
-            int ahead = look_up(0);
+            int four = look_up(0), next_four = look_up(4);
             for (int i = 0; i < sg.tiles; ++i, ++use) {
-                const int stage = use % STAGES, n = (sg.from + i) * (KEYS / 16) + p, page = ahead;
-                ahead = look_up(i + 1);
-                ok = tc::mbar_wait(&empty[stage], ((use / STAGES) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                const int stage = use % STAGES, n = (sg.from + i) * (KEYS / 16) + p, page = __shfl_sync(0xffffffffu, four, (i & 3) * 8 + p);
+                if ((i & 3) == 3) four = next_four, next_four = look_up(i + 5);
                 const bool real = (unsigned)page < (unsigned)a.pages;
                 const unsigned runs = __ballot_sync(0xffffffffu, real) & 0xffu;
+                const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+                ok = tc::mbar_wait_warp(&empty[stage], ((use / STAGES) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
+                if (!ok) break;
                 if (lane == 0) {
-                    live[stage] = (int)runs;
-                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * 16 * D * (EIGHT ? 1 : 2));
+                    if (plane == 0) live[stage] = (int)runs;
+                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 16 * D * (EIGHT ? 1 : 2));
                 }
                 __syncwarp();
-                const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+                if (EIGHT && lane < 8) {
+                    if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
+                    arrive_after_copies(&full[stage]);
+                }
                 uint8_t* to = smem + stage * S::STAGE + plane * S::PLANE;
-                if constexpr (EIGHT) {
-                    if (second) {
-                        if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
-                        arrive_after_copies(&full[stage]);
-                    } else if (real) {
-                        tc::tma_load_2d(to + p * 16 * 128, &map, 0, (int)row, &full[stage]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int y = __shfl_sync(0xffffffffu, (int)row, k);
+                    if (lane == 0 && (runs >> k & 1u)) {
+                        tc::tma_load_2d(to + k * 16 * 128, &map, 0, y, &full[stage]);
+                        if (!EIGHT) tc::tma_load_2d(to + S::PLANE / 2 + k * 16 * 128, &map, 64, y, &full[stage]);
                     }
-                } else if (real) {
-                    tc::tma_load_2d(to + second * (S::PLANE / 2) + p * 16 * 128, &map, 64 * second, (int)row, &full[stage]);
                 }
             }
         }
