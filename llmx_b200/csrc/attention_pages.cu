@@ -172,15 +172,17 @@ int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exp
     return merge<QT, EIGHT, D, 16 * RW, TILE, WARPS / RW>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
 }
 
-// The pages' rows of 128 values, 16 at a time (bfloat16: 64 values of them).
-int pages_map(CUtensorMap* map, const void* cache, bool eight, uint64_t rows) {
-    if (!eight) return llmx_make_map_bf16_2d(map, cache, rows, 128, 16, 64);
+// The pages as (128 bytes of a row) x (eight rows) x (keys, values) x (eights of a plane) x (page): a copy is 16 keys and their values, eight
+// keys, their values, eight keys, ... (bfloat16: of the rows' first or second half).
+int pages_map(CUtensorMap* map, const void* cache, bool eight, int pages, int kv_heads, int page_size) {
     llmx_encode_tiled_fn enc = llmx_encode_tiled();
     if (!enc) return 10003;
-    const cuuint64_t dims[2] = {128, rows}, strides[1] = {128};
-    const cuuint32_t box[2] = {128, 16}, elem[2] = {1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+    const cuuint64_t row = eight ? 128 : 256, plane = row * kv_heads * page_size;
+    const cuuint64_t dims[5] = {128, 8, 2, (cuuint64_t)kv_heads * page_size / 8, (cuuint64_t)pages}, strides[4] = {row, plane, 8 * row, 2 * plane};
+    const cuuint32_t box[5] = {eight ? 128u : 64u, 8, 2, 2, 1}, elem[5] = {1, 1, 1, 1, 1};
+    return enc(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(cache), dims, strides, box, elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? 0
                : 10003;
 }
@@ -190,7 +192,7 @@ int tensor_rows(const FewPlan& p, const void* q, const void* cache, const void* 
                 int max_rows, int heads, int kv_heads, float scale, int* error_word, cudaStream_t stream) {
     using namespace tc_pages;
     CUtensorMap map;
-    if (const int e = pages_map(&map, cache, EIGHT, (uint64_t)a.pages * 2 * kv_heads * a.page_size)) return e;
+    if (const int e = pages_map(&map, cache, EIGHT, a.pages, kv_heads, a.page_size)) return e;
     LLMX_ALLOW_SMEM(pages_kernel<EIGHT, SHARED, R>);
     launch_kernel(pages_kernel<EIGHT, SHARED, R>, dim3((unsigned)p.blocks), dim3(tc_pages::Shape<EIGHT, SHARED, R>::THREADS),
                   (size_t)tc_pages::Shape<EIGHT, SHARED, R>::BYTES, stream, map, (const __nv_bfloat16*)q, (const uint8_t*)exponents, (__nv_bfloat16*)out, partial, a,

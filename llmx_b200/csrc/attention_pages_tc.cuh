@@ -12,7 +12,8 @@
 // to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 16 + w3 / 256 (12 bits, down to 2^-26 of the largest): columns of their
 // own, whose sums are added up in 32 bits.  As in the warp form a value's power of two joins its key's score.
 //
-//   warps 0, 10     page lookups and copies of keys and of values, 16 rows a copy, STAGES tiles ahead
+//   warps 0, 10     page lookups and copies, STAGES tiles ahead, every other tile each: 16 keys and their values a copy (a warp issues
+//                   one in some 100 clocks, which by itself would be less than memory gives)
 //   warp 1          matrix instructions, whichever can be made next: S^T of tiles ahead, O^T
 //   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
@@ -48,8 +49,9 @@ template <bool EIGHT, bool SHARED, int R>
 struct Shape {
     static constexpr int U = 2;
     static constexpr int THREADS = 96 + U * UNIT_WARPS * 32;
-    static constexpr int PLANE = KEYS * D * (EIGHT ? 1 : 2);
-    static constexpr int STAGE = 2 * PLANE;
+    // A stage: eight keys, their values, the next eight keys, ..., rows of 128 bytes; bfloat16: such a half for the rows' first 64 values
+    // and one for the others.
+    static constexpr int HALF = 2 * KEYS * 128, STAGE = EIGHT ? HALF : 2 * HALF;
     static constexpr int STAGES = EIGHT ? 4 : 2;
     static constexpr int WEIGHTS = KEYS * 128;                  // bytes of a unit's weights of a tile: rows of 128 bytes, the first ones used
     static constexpr int BUFFERS = EIGHT ? 2 : 1;               // of weights
@@ -68,10 +70,12 @@ struct Shape {
 };
 
 // MN-major operand of bytes or 16-bit values under the 128-byte swizzle: 128 bytes of the MN dimension in a row, rows of the K dimension 128
-// bytes apart (groups of eight 1024), the MN dimension's next 128 bytes `block` further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t block) {
-    return (uint64_t)((at & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// bytes apart, groups of eight `eight_rows`, the MN dimension's next 128 bytes `block` further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t block, uint32_t eight_rows) {
+    return (uint64_t)((at & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(eight_rows >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+// K-major, rows of 128 bytes, groups of eight 2048 bytes apart (a stage's keys).
+__device__ __forceinline__ uint64_t desc_keys(uint32_t at) { return (uint64_t)((at & 0x3FFFFu) >> 4) | (1ull << 16) | (128ull << 32) | (1ull << 46) | (2ull << 61); }
 constexpr uint32_t TRANSPOSED = (1u << 15) | (1u << 16);
 // kind::f8f6f4, e4m3 on both sides, 32-bit sums.
 __host__ __device__ constexpr uint32_t instruction_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
@@ -184,7 +188,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     const int ratio = heads / kv_heads;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 18 : 2), tc::mbar_init(&empty[i], 1);     // (two loaders' bytes; 16 lanes' exponents)
+        for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 17 : 1), tc::mbar_init(&empty[i], 1);     // (copies' bytes; 16 lanes' exponents)
         for (int u = 0; u < U; ++u) {
             tc::mbar_init(&q_full[u], UNIT_WARPS);
             for (int i = 0; i < 2; ++i) {
@@ -204,8 +208,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         tc::tmem_relinquish();
     }
     // Values that no copy has written yet are zeros, never what the memory held before: a weight of zero meets them.
-    for (int i = threadIdx.x; i < STAGES * S::PLANE / 16; i += S::THREADS)
-        *reinterpret_cast<uint4*>(smem + (i / (S::PLANE / 16)) * S::STAGE + S::PLANE + (i % (S::PLANE / 16)) * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < STAGES * S::STAGE / 16; i += S::THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if constexpr (!EIGHT)
         for (int i = threadIdx.x; i < U * R * D / 4; i += S::THREADS) reinterpret_cast<float4*>(smem + S::AT_STRAY)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     tc::fence_proxy_async();
@@ -253,8 +256,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     };
 
     if (warp == 0 || warp == LOADER) {
-        // Keys (warp 0) or values: a lane finds a run of 16 keys, one issues the copies.
-        const int p = lane & 7, plane = warp == LOADER;
+        const int p = lane & 7, plane = (lane >> 3) & 1;          // a run of 16 keys; for exponents, keys' or values'
         uint32_t use = 0;
         bool ok = true;
         while (ok && next_segment()) {
@@ -268,29 +270,45 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             for (int i = 0; i < sg.tiles; ++i, ++use) {
                 const int stage = use % STAGES, n = (sg.from + i) * (KEYS / 16) + p, page = __shfl_sync(0xffffffffu, four, (i & 3) * 8 + p);
                 if ((i & 3) == 3) four = next_four, next_four = look_up(i + 5);
+                if ((use & 1) != (warp == LOADER)) continue;
                 const bool real = (unsigned)page < (unsigned)a.pages;
                 const unsigned runs = __ballot_sync(0xffffffffu, real) & 0xffu;
-                const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + (n - page_of(n) * runs_a_page) * 16;
+                const int off = (n - page_of(n) * runs_a_page) * 16;
                 ok = tc::mbar_wait_warp(&empty[stage], ((use / STAGES) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
                 if (!ok) break;
                 if (lane == 0) {
-                    if (plane == 0) live[stage] = (int)runs;
-                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 16 * D * (EIGHT ? 1 : 2));
+                    live[stage] = (int)runs;
+                    tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * 16 * D * (EIGHT ? 1 : 2));
                 }
                 __syncwarp();
-                if (EIGHT && lane < 8) {
+                if (EIGHT && lane < 16) {
+                    const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + off;
                     if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
                     arrive_after_copies(&full[stage]);
                 }
-                uint8_t* to = smem + stage * S::STAGE + plane * S::PLANE;
+                // One lane makes all copies, from operands that are there before the first: waits between them would be as long as the copies.
+                uint8_t* to = smem + stage * S::STAGE;
+                const int eights = (sg.kv * a.page_size + off) >> 3;
+                int y[8], at_page[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int y = __shfl_sync(0xffffffffu, (int)row, k);
-                    if (lane == 0 && (runs >> k & 1u)) {
-                        tc::tma_load_2d(to + k * 16 * 128, &map, 0, y, &full[stage]);
-                        if (!EIGHT) tc::tma_load_2d(to + S::PLANE / 2 + k * 16 * 128, &map, 64, y, &full[stage]);
+                for (int k = 0; k < 8; ++k) y[k] = __shfl_sync(0xffffffffu, eights, k), at_page[k] = __shfl_sync(0xffffffffu, page, k);
+                if (lane == 0) {
+                    if (runs == 0xffu) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            tc::tma_load_5d(to + k * 4096, &map, 0, 0, 0, y[k], at_page[k], &full[stage]);
+                            if (!EIGHT) tc::tma_load_5d(to + S::HALF + k * 4096, &map, 64, 0, 0, y[k], at_page[k], &full[stage]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (runs >> k & 1u) {
+                                tc::tma_load_5d(to + k * 4096, &map, 0, 0, 0, y[k], at_page[k], &full[stage]);
+                                if (!EIGHT) tc::tma_load_5d(to + S::HALF + k * 4096, &map, 64, 0, 0, y[k], at_page[k], &full[stage]);
+                            }
                     }
                 }
+                __syncwarp();
             }
         }
     } else if (warp == 1) {
@@ -318,12 +336,12 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                                 if constexpr (EIGHT) {
 #pragma unroll
                                     for (int k = 0; k < D / 32; ++k)
-                                        mma_e4m3(d, tc::smem_desc_k_sw128(keys + k * 32), tc::smem_desc_k_sw128(queries + k * 32), instruction_e4m3(KEYS, 2 * R),
+                                        mma_e4m3(d, desc_keys(keys + k * 32), tc::smem_desc_k_sw128(queries + k * 32), instruction_e4m3(KEYS, 2 * R),
                                                  k > 0);
                                 } else {
 #pragma unroll
                                     for (int k = 0; k < D / 16; ++k)
-                                        tc::mma_bf16_ss(d, tc::smem_desc_k_sw128(keys + (k >> 2) * (S::PLANE / 2) + (k & 3) * 32),
+                                        tc::mma_bf16_ss(d, desc_keys(keys + (k >> 2) * S::HALF + (k & 3) * 32),
                                                         tc::smem_desc_k_sw128(queries + (k >> 2) * (R * 128) + (k & 3) * 32), tc::instr_desc_bf16(KEYS, R), k > 0);
                                 }
                                 tc::mma_commit(&s_full[2 * u + buffer]);
@@ -336,18 +354,18 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         const int u = SHARED ? tile & 1 : turn, stage = (use + tile) % STAGES, buffer = weighed[u] % S::BUFFERS;
                         if (is_done(&w_full[2 * u + buffer], (weighed[u] / S::BUFFERS) & 1u)) {
                             tc::tc_fence_after();
-                            const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + S::PLANE), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
+                            const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + 1024), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
                             const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + (u * S::BUFFERS + buffer) * S::WEIGHTS);
                             const bool begun = SHARED ? tile > 1 : tile > 0;
                             if constexpr (EIGHT) {
 #pragma unroll
                                 for (int k = 0; k < KEYS / 32; ++k)
-                                    mma_e4m3(d, desc_mn(values + k * 4096, S::PLANE), desc_mn(weights + k * 4096, S::WEIGHTS),
+                                    mma_e4m3(d, desc_mn(values + k * 8192, S::HALF, 2048), desc_mn(weights + k * 4096, S::WEIGHTS, 1024),
                                              instruction_e4m3(D, 3 * R) | TRANSPOSED, begun || k > 0);
                             } else {
 #pragma unroll
                                 for (int k = 0; k < KEYS / 16; ++k)
-                                    tc::mma_bf16_ss(d, desc_mn(values + k * 2048, S::PLANE / 2), desc_mn(weights + k * 2048, S::WEIGHTS),
+                                    tc::mma_bf16_ss(d, desc_mn(values + k * 4096, S::HALF, 2048), desc_mn(weights + k * 2048, S::WEIGHTS, 1024),
                                                     tc::instr_desc_bf16(D, R) | TRANSPOSED, begun || k > 0);
                             }
                             ++weighed[u];
@@ -488,7 +506,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 }
                 const bool whole = t0 >= all_from && t0 + KEYS <= all_to && runs == 0xff;
                 const bool in_reach = t >= sg.rq.low && t < sg.rq.end;
-                uint8_t* value_row = smem + stage * S::STAGE + S::PLANE + key * 128;
+                uint8_t* value_row = smem + stage * S::STAGE + (key >> 3) * 2048 + 1024 + (key & 7) * 128;
                 bool stray = false;
                 unsigned hidden = 0;                             // rows that do not see this key
                 if (!whole) {
@@ -496,13 +514,13 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         // Values that nobody sees must be numbers, those of a page that is not there zeros.
 #pragma unroll
                         for (int n = 0; n < (EIGHT ? 8 : 16); ++n)
-                            *reinterpret_cast<uint4*>(value_row + (n >> 3) * (S::PLANE / 2) + (n & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(value_row + (n >> 3) * S::HALF + (n & 7) * 16) = make_uint4(0, 0, 0, 0);
                     } else if (!EIGHT && a.tree && t >= history) {
                         // Values that are no numbers, of a key that not every row sees: their products are added up beside the others, for
                         // the rows that do, and zeros take their place (a weight of zero times an infinity is no zero).
 #pragma unroll
                         for (int n = 0; n < 16; ++n) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(value_row + (n >> 3) * (S::PLANE / 2) + (n & 7) * 16);
+                            const uint4 v = *reinterpret_cast<const uint4*>(value_row + (n >> 3) * S::HALF + (n & 7) * 16);
                             const unsigned x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) stray |= (x[k] & 0x7F80u) == 0x7F80u || (x[k] & 0x7F800000u) == 0x7F800000u;
@@ -638,7 +656,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                                 for (int k = 0; k < 2; ++k) {
                                     if (hidden >> (row + k) & 1u) continue;
                                     for (int d = 0; d < D; ++d) {
-                                        const unsigned v = *value_in<S::PLANE / 2>(value_row, key, d);
+                                        const unsigned v = *value_in<S::HALF>(value_row, key, d);
                                         if ((v & 0x7F80u) == 0x7F80u) atomicAdd(strays + (row + k) * D + d, (k ? e1 : e0) * __uint_as_float(v << 16));
                                     }
                                     stray_flag[unit] = 1;
@@ -659,7 +677,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         if (!SHARED) units_barrier();
                         if (stray)
                             for (int d = 0; d < D; ++d) {
-                                unsigned short* x = value_in<S::PLANE / 2>(value_row, key, d);
+                                unsigned short* x = value_in<S::HALF>(value_row, key, d);
                                 if ((*x & 0x7F80u) == 0x7F80u) *x = 0;
                             }
                     }
