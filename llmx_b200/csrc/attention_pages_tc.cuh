@@ -52,13 +52,16 @@ struct Shape {
     // A stage: eight keys, their values, the next eight keys, ..., rows of 128 bytes; bfloat16: such a half for the rows' first 64 values
     // and one for the others.
     static constexpr int HALF = 2 * KEYS * 128, STAGE = EIGHT ? HALF : 2 * HALF;
-    static constexpr int STAGES = EIGHT ? 4 : 2;
-    static constexpr int WEIGHTS = KEYS * 128;                  // bytes of a unit's weights of a tile: rows of 128 bytes, the first ones used
-    static constexpr int BUFFERS = EIGHT ? 2 : 1;               // of weights
+    // As many stages as there is room for: a stage is taken for some 5,000 clocks, a third of them until its copies have come, and
+    // memory gives one in 1,000.
+    static constexpr int STAGES = !EIGHT ? 2 : R == 16 ? 6 : 5;
+    // A tile's weights: rows of 128 bytes a key, of which a unit has one half, or all.
+    static constexpr int WEIGHTS = KEYS * 128;
+    static constexpr bool HALVES = !EIGHT || R == 16;
     static constexpr int QUERIES = (EIGHT ? 2 * R * D : R * D * 2);
     static constexpr int S_COLS = EIGHT ? 2 * R : R, O_COLS = EIGHT ? 3 * R : R, U_COLS = 2 * S_COLS + O_COLS;
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
-    static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + U * BUFFERS * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
+    static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
     // What a unit's threads tell each other, in floats: factors, minus the sum's reference, the weights' beside it, what raising scales
     // the two by, positions [R];
     // maxima and sums of warps [2][4][R].
@@ -178,9 +181,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     uint64_t* q_full = empty + STAGES;                          // [U]
     uint64_t* s_full = q_full + U;                              // [U][2]
     uint64_t* s_free = s_full + 2 * U;                          // [U][2]
-    uint64_t* w_full = s_free + 2 * U;                          // [U][BUFFERS]
-    uint64_t* o_done = w_full + 2 * U;                          // [U][BUFFERS]: O^T with that buffer's weights
-    uint32_t* tmem_slot = (uint32_t*)(o_done + 2 * U);
+    uint64_t* w_full = s_free + 2 * U;                          // [U]
+    uint64_t* o_done = w_full + U;                              // [U]: O^T with these weights
+    uint32_t* tmem_slot = (uint32_t*)(o_done + U);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* live = abort_flag + 1;                        // [STAGES]: which of the stage's runs of 16 keys are in the cache
     volatile int* stray_flag = live + STAGES;                   // [U]
@@ -194,9 +197,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             for (int i = 0; i < 2; ++i) {
                 tc::mbar_init(&s_full[2 * u + i], 1);
                 tc::mbar_init(&s_free[2 * u + i], UNIT_WARPS);
-                tc::mbar_init(&w_full[2 * u + i], UNIT_WARPS);
-                tc::mbar_init(&o_done[2 * u + i], 1);
             }
+            tc::mbar_init(&w_full[u], UNIT_WARPS);
+            tc::mbar_init(&o_done[u], 1);
             stray_flag[u] = 0;
         }
         *abort_flag = 0;
@@ -281,11 +284,6 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     tc::mbar_expect_tx(&full[stage], (uint32_t)__popc(runs) * 2 * 16 * D * (EIGHT ? 1 : 2));
                 }
                 __syncwarp();
-                if (EIGHT && lane < 16) {
-                    const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + off;
-                    if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
-                    arrive_after_copies(&full[stage]);
-                }
                 // One lane makes all copies, from operands that are there before the first: waits between them would be as long as the copies.
                 uint8_t* to = smem + stage * S::STAGE;
                 const int eights = (sg.kv * a.page_size + off) >> 3;
@@ -309,6 +307,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     }
                 }
                 __syncwarp();
+                if (EIGHT && lane < 16) {
+                    const unsigned row = (((unsigned)(real ? page : 0) * 2 + plane) * kv_heads + sg.kv) * a.page_size + off;
+                    if (real) copy16(tc::smem_u32(smem + S::AT_EXPONENTS + stage * 256 + plane * KEYS + p * 16), exponents + row);
+                    arrive_after_copies(&full[stage]);
+                }
             }
         }
     } else if (warp == 1) {
@@ -351,11 +354,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         }
                     }
                     if (tile < next) {
-                        const int u = SHARED ? tile & 1 : turn, stage = (use + tile) % STAGES, buffer = weighed[u] % S::BUFFERS;
-                        if (is_done(&w_full[2 * u + buffer], (weighed[u] / S::BUFFERS) & 1u)) {
+                        const int u = SHARED ? tile & 1 : turn, stage = (use + tile) % STAGES;
+                        if (is_done(&w_full[u], weighed[u] & 1u)) {
                             tc::tc_fence_after();
                             const uint32_t values = tc::smem_u32(smem + stage * S::STAGE + 1024), d = tmem + u * S::U_COLS + 2 * S::S_COLS;
-                            const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + (u * S::BUFFERS + buffer) * S::WEIGHTS);
+                            const uint32_t weights = tc::smem_u32(smem + S::AT_WEIGHTS + u * (S::HALVES ? 64 : S::WEIGHTS));
                             const bool begun = SHARED ? tile > 1 : tile > 0;
                             if constexpr (EIGHT) {
 #pragma unroll
@@ -371,7 +374,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                             ++weighed[u];
                             const bool last = SHARED || turn == U - 1;
                             if (last) tc::mma_commit(&empty[stage]);
-                            tc::mma_commit(&o_done[2 * u + buffer]);
+                            tc::mma_commit(&o_done[u]);
                             turn = last ? 0 : turn + 1;
                             tile += last;
                             made = true;
@@ -404,7 +407,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         float *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
-        const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + unit * S::BUFFERS * S::WEIGHTS) + key * 128;
+        const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + (S::HALVES ? 0 : unit * S::WEIGHTS)) + key * 128;
         uint32_t before = 0, mine = 0;                          // tiles of the segments before; this unit's so far
         bool ok = true, first_segment = true;
         for (; next_segment(); before += sg.tiles, first_segment = false) {
@@ -478,18 +481,18 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             for (int i = SHARED ? unit : 0; i < sg.tiles; i += SHARED ? 2 : 1, ++mine) {
                 const bool opening = i < (SHARED ? 2 : 1);       // the unit's first tile of the item
                 const uint32_t use = before + i;
-                const int stage = use % STAGES, s_buffer = mine & 1, w_buffer = mine % S::BUFFERS;
+                const int stage = use % STAGES, s_buffer = mine & 1;
                 const int t0 = (sg.from + i) * KEYS, t = t0 + key;
                 // The tile's copies, its scores, and that the weights' buffer is free again: asked for together, since an answer takes long.
-                const bool reused = mine >= (uint32_t)S::BUFFERS;
-                const uint32_t w_parity = ((mine / S::BUFFERS) & 1u) ^ 1u;
+                const bool reused = mine > 0;
+                const uint32_t w_parity = (mine & 1u) ^ 1u;
                 if (ok) {
                     const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u),
-                               a2 = !reused || is_done(&o_done[2 * unit + w_buffer], w_parity);
+                               a2 = !reused || is_done(&o_done[unit], w_parity);
                     if (!__all_sync(0xffffffffu, a0 && a1 && a2)) {
                         ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                         if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                        if (ok && reused) ok = tc::mbar_wait_warp(&o_done[2 * unit + w_buffer], w_parity, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                        if (ok && reused) ok = tc::mbar_wait_warp(&o_done[unit], w_parity, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                     }
                 }
                 tc::tc_fence_after();
@@ -613,10 +616,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         x[n] += mp.x, x[n + 1] += mp.y, x[n + 2] += mp.z, x[n + 3] += mp.w;
                     }
                     if (!opening) {
-                        // Every O^T that has been asked for has been made before it is scaled.
-                        const uint32_t last = mine - 1;
-                        if (ok) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                        tc::tc_fence_after();
+                        // (Every O^T that has been asked for has been made: the weights' buffer is free.)
 #pragma unroll
                         for (int n = 0; n < R; ++n) sum[n] *= fade_sum[n];
 #pragma unroll
@@ -635,7 +635,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s_free[2 * unit + s_buffer]);
                 // ---- weights
-                const uint32_t weights = weights_at + w_buffer * S::WEIGHTS;
+                constexpr int SKIP = S::HALVES ? 4 : 0;             // pieces of 16 bytes to the second unit's half
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     uint32_t h[8];
@@ -665,10 +665,10 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     }
                     if constexpr (EIGHT) {
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) to_shared4(weights + (((3 * c + k) ^ (key & 7)) << 4), take_codes(h, k < 2));
+                        for (int k = 0; k < 3; ++k) to_shared4(weights_at + (((SKIP * unit + 3 * c + k) ^ (key & 7)) << 4), take_codes(h, k < 2));
                     } else {
-                        to_shared4(weights + (((2 * c) ^ (key & 7)) << 4), make_uint4(h[0], h[1], h[2], h[3]));
-                        to_shared4(weights + (((2 * c + 1) ^ (key & 7)) << 4), make_uint4(h[4], h[5], h[6], h[7]));
+                        to_shared4(weights_at + (((SKIP * unit + 2 * c) ^ (key & 7)) << 4), make_uint4(h[0], h[1], h[2], h[3]));
+                        to_shared4(weights_at + (((SKIP * unit + 2 * c + 1) ^ (key & 7)) << 4), make_uint4(h[4], h[5], h[6], h[7]));
                     }
                 }
                 if constexpr (!EIGHT)
@@ -684,7 +684,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 tc::fence_proxy_async();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&w_full[2 * unit + w_buffer]);
+                if (lane == 0) tc::mbar_arrive(&w_full[unit]);
             }
 
             // ---- the item's sums over this block's keys: a thread has one of the 128 values of every row
@@ -696,13 +696,14 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 for (int o = 16; o > 0; o >>= 1) sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], o);
                 if (lane == 0) warp_peak[quarter * R + n] = sum[n];
             }
-            if (ok && any_tile) ok = tc::mbar_wait_warp(&o_done[2 * unit + last % S::BUFFERS], (last / S::BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+            if (ok && any_tile) ok = tc::mbar_wait_warp(&o_done[unit], last & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
             tc::tc_fence_after();
             unit_barrier(unit);
             const bool any_stray = !EIGHT && stray_flag[unit];
             float* slot = partial + (2 * (size_t)blockIdx.x + !first_segment) * TILE_ROWS * ROWF;
-            // The second unit's sums go to the first by way of its weights' place.
-            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS + S::BUFFERS * S::WEIGHTS);
+            // The second unit's sums go to the first by way of the weights' place, once both have no use for that.
+            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS);
+            if (SHARED) units_barrier();
             const bool both = SHARED && sg.tiles > 1;
             auto outputs = [&](int c, float (&o)[16]) {
                 uint32_t v[16];
