@@ -131,7 +131,7 @@ int multiprocessors() {
 // How a call is cut up; `rows` 0: only the general form takes these sizes.
 struct FewPlan {
     bool tensor = false;                  // tcgen05, else the warps' instruction
-    int rows = 0, blocks = 0;             // (row, head) pairs of a tile
+    int rows = 0, blocks = 0, max_tiles = 0;      // (row, head) pairs of a tile; tiles of keys of a request at most
     long long bytes(int head_dim) const { return 2ll * blocks * rows * (head_dim + mma_pages::PART) * 4; }      // two states a block
 };
 
@@ -146,15 +146,17 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
     // As many blocks as find an SM at one time.  The kernel leaves some of them without work where there is too little.
     const long long items = (pairs + p.rows - 1) / p.rows * kv_heads * requests;
     const long long keys = window > 0 ? min((long long)max_context, (long long)window + max_rows) : max_context;
+    p.max_tiles = max_context / (p.tensor ? tc_pages::KEYS : mma_pages::TILE) + 2;
     const long long tiles = items * (keys / (p.tensor ? tc_pages::KEYS : mma_pages::TILE) + 2);
+    if (items * (p.max_tiles + mma_pages::OPEN) >= (1ll << 31)) p.rows = 0;      // (places are counted in 32 bits)
     p.blocks = (int)min((p.tensor ? 1ll : 2ll) * multiprocessors(), max(items, tiles / 2));
     return p;
 }
 
-template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int RUNS>
+template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int OPEN, int RUNS>
 int merge(const FewPlan& p, void* out, const float* partial, const Rows& a, int requests, int max_rows, int heads, int kv_heads, cudaStream_t stream) {
     const long long rows = (long long)max_rows * heads, blocks = (rows * (D / 4) + 127) / 128;
-    launch_kernel(mma_pages::merge_kernel<QT, EIGHT, D, TILE_ROWS, KEYS, RUNS>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, partial,
+    launch_kernel(mma_pages::merge_kernel<QT, EIGHT, D, TILE_ROWS, KEYS, OPEN, RUNS>, dim3((unsigned)blocks, (unsigned)requests), dim3(128), 0, stream, partial,
                   (QT*)out, a, requests, heads, kv_heads, p.blocks);
     return launch_status();
 }
@@ -169,7 +171,7 @@ int few_rows(const FewPlan& p, const void* q, const void* cache, const void* exp
                   (const QT*)q, (const uint8_t*)cache, (const uint8_t*)exponents, (QT*)out, partial, a, requests, heads, kv_heads,
                   scale * 1.4426950408889634f);
     if (const int e = launch_status()) return e;
-    return merge<QT, EIGHT, D, 16 * RW, TILE, WARPS / RW>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
+    return merge<QT, EIGHT, D, 16 * RW, TILE, OPEN, WARPS / RW>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
 }
 
 // The pages as (128 bytes of a row) x (eight rows) x (keys, values) x (eights of a plane) x (page): a copy is 16 keys and their values, eight
@@ -198,7 +200,7 @@ int tensor_rows(const FewPlan& p, const void* q, const void* cache, const void* 
                   (size_t)tc_pages::Shape<EIGHT, SHARED, R>::BYTES, stream, map, (const __nv_bfloat16*)q, (const uint8_t*)exponents, (__nv_bfloat16*)out, partial, a,
                   requests, heads, kv_heads, scale * 1.4426950408889634f, error_word);
     if (const int e = launch_status()) return e;
-    return merge<__nv_bfloat16, EIGHT, 128, SHARED ? R : 2 * R, KEYS, 1>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
+    return merge<__nv_bfloat16, EIGHT, 128, SHARED ? R : 2 * R, KEYS, OPEN, 1>(p, out, partial, a, requests, max_rows, heads, kv_heads, stream);
 }
 }  // namespace
 
@@ -223,11 +225,12 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
         return LLMX_ERR_UNSUPPORTED;
-    const Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words,
-                    ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), max_rows};
+    Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words,
+                    ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), 0, max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
-    if (p.rows && pages > 0 && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
+    a.max_tiles = p.max_tiles;
+    if (p.rows && pages > 0 && (long long)total_rows * heads < (1ll << 31) && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
         (long long)pages * 2 * kv_heads * page_size < (1ll << 31)) {
         if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes(head_dim)) return LLMX_ERR_BAD_ARGUMENT;
 #define LLMX_FEW_ARGS p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale

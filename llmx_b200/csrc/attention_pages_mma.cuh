@@ -7,7 +7,7 @@
 // more rows than a tile holds, RW warps work on the same keys, each on 16 rows of its own, and share the ring.
 //
 // The work is cut evenly: the tiles of 32 keys of all (request, tile of rows, key/value head) items in a row, every block of the grid
-// an equal share of them, however unlike the requests' lengths.  An item that lies within a block is written at once; one that is
+// an equal share of them (Walk), however unlike the requests' lengths.  An item that lies within a block is written at once; one that is
 // cut leaves a state in each block's slots, and a second kernel adds those up.
 //
 // Codes become halves in registers (exact) and meet queries as halves, which carry a power of two a row so that every one of them
@@ -31,6 +31,7 @@ namespace mma_pages {
 
 constexpr int TILE = 32;             // keys of a stage
 constexpr int WARPS = 4;
+constexpr int OPEN = 8;              // tiles that an item's beginning and end take as long as
 constexpr int MOST_KEYS = 1 << 30;   // of a request: places are counted in 32 bits
 // Weights are 2^10 times themselves over codes, so that small ones lie above a half's steps; the maxima that the exponentials use are
 // raised only when a row's true one has grown by more than 2^5 (2^15 is a half, and most tiles then leave the sums alone).
@@ -45,6 +46,7 @@ struct Rows {                        // whose rows these are and where their key
     const unsigned* tree;            // [rows, tree_words] or null
     int tree_words;
     unsigned run_pages;              // 2^31 / (page_size / 16), rounded up: t / page_size = (t / 16) * run_pages >> 31 for t < 2^30
+    int max_tiles;                   // the most tiles of keys of a request
     int max_rows;                    // the most rows of a request of this call; one with more is another's
 };
 
@@ -173,7 +175,12 @@ __device__ __forceinline__ void add_no_numbers(float (&o)[4], uint32_t (&v)[4], 
     }
 }
 
-// A request's part of the work: tiles of KEYS keys (at least one, so that rows that see nothing are written too) and tiles of rows.
+// ---- the work, cut evenly ----
+// An item (a tile of a request's rows and a key/value head) has a request's tiles of KEYS keys, and takes OPEN tiles' time more to begin
+// and to end.  So items lie in a row with OPEN + tiles places each, and block b of `blocks` has the places all * b / blocks up to
+// all * (b + 1) / blocks.  What a block has of an item whose places it shares with others goes to its first slot where the item began
+// before the block's places, else to its second.  Places are counted in 32 bits: a request's tiles are cut off at `max_tiles`, by
+// which the host knows that they suffice.
 struct Request {
     int count, history, start, pairs, low, end, tile0, tiles, row_tiles;
 };
@@ -188,31 +195,31 @@ __device__ __forceinline__ Request request_of(const Rows& a, int r, int ratio, i
     q.end = min(reach, q.history + (a.tree ? min(q.count, 32 * a.tree_words) : q.count));
     q.low = a.window > 0 ? max(0, q.history - a.window + 1) : 0;
     q.tile0 = q.low / KEYS;
-    q.tiles = ours ? max((q.end + KEYS - 1) / KEYS - q.tile0, 1) : 0;
+    // (At least one tile, so that rows that see nothing are written too.)
+    q.tiles = ours ? min(max((q.end + KEYS - 1) / KEYS - q.tile0, 1), a.max_tiles) : 0;
     q.row_tiles = (q.pairs + tile_rows - 1) / tile_rows;
     return q;
 }
-// Requests' tiles in a row, by whole warps: those of all, or those before the request that place `x` falls in (which `found` names).
-template <int KEYS>
-__device__ __forceinline__ long long tiles_before(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, long long x, int& found,
-                                                  long long& items) {
+// The places of all requests, and how many items they are; where `x` is at least 0, the places before the request that it falls in,
+// which `found` names.  By whole warps.
+template <int KEYS, int OPEN>
+__device__ __forceinline__ int places_before(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, int x, int& found, int& items) {
     const int lane = threadIdx.x & 31;
-    long long before = 0;
+    int before = 0;
     items = 0;
     found = requests;
     for (int r0 = 0; r0 < requests; r0 += 32) {
-        long long n = 0, of = 0;
+        int n = 0, of = 0;
         if (r0 + lane < requests) {
             const Request q = request_of<KEYS>(a, r0 + lane, ratio, tile_rows);
-            of = (long long)q.row_tiles * kv_heads;
-            n = of * q.tiles;
+            of = q.row_tiles * kv_heads;
+            n = of * (q.tiles + OPEN);
         }
-        long long upto = n;
+        int upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o), w = __shfl_xor_sync(0xffffffffu, of, o);
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
-            of += w;
         }
         const unsigned here = __ballot_sync(0xffffffffu, x >= 0 && x < before + upto);
         if (here) {
@@ -221,14 +228,53 @@ __device__ __forceinline__ long long tiles_before(const Rows& a, int requests, i
             return before + __shfl_sync(0xffffffffu, upto - n, at);
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
-        items += of;
+        items += (int)__reduce_add_sync(0xffffffffu, (unsigned)of);
     }
     return before;
 }
 // The blocks that share the work: all of the grid, as far as each gets two tiles a group of warps or an item of its own.
-__device__ __forceinline__ int working_blocks(long long tiles, long long items, int blocks, int runs) {
-    return (int)min((long long)blocks, max(items, tiles / (2 * runs)));
-}
+template <int OPEN>
+__device__ __forceinline__ int working_blocks(int all, int items, int blocks, int runs) { return min(blocks, max(items, (all - items * OPEN) / (2 * runs))); }
+__device__ __forceinline__ int share_begins(int all, int blocks, int b) { return (int)((unsigned long long)all * b / blocks); }
+
+// A block's items one after another.
+template <int KEYS, int OPEN>
+struct Walk {
+    Request rq;
+    int r, kv, first, from, tiles, slot;     // request, head, first pair; the tiles of the item that are the block's (none: go on); slot for its state
+    bool whole;                              // all of the item's
+    int at, until, request_at, tile_rows, kv_heads, ratio;
+    __device__ __forceinline__ Walk(const Rows& a, int requests, int ratio_, int tile_rows_, int kv_heads_, int grid, int runs)
+        : tile_rows(tile_rows_), kv_heads(kv_heads_), ratio(ratio_) {
+        int items, unused;
+        const int all = places_before<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, -1, r, items), blocks = working_blocks<OPEN>(all, items, grid, runs);
+        const bool works = (int)blockIdx.x < blocks;
+        at = works ? share_begins(all, blocks, blockIdx.x) : 0;
+        until = works ? share_begins(all, blocks, blockIdx.x + 1) : 0;
+        request_at = places_before<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, at, r, unused);
+        if (at < until) rq = request_of<KEYS>(a, r, ratio, tile_rows);
+    }
+    __device__ __forceinline__ bool next(const Rows& a) {
+        do {
+            if (at >= until) return false;
+            int places = rq.row_tiles * kv_heads * (rq.tiles + OPEN);
+            while (at >= request_at + places) {
+                request_at += places;
+                rq = request_of<KEYS>(a, ++r, ratio, tile_rows);
+                places = rq.row_tiles * kv_heads * (rq.tiles + OPEN);
+            }
+            const int each = rq.tiles + OPEN, item = (at - request_at) / each, item_at = request_at + item * each, upto = min(until, item_at + each);
+            kv = item % kv_heads, first = item / kv_heads * tile_rows;
+            const int skipped = max(at - item_at - OPEN, 0);
+            tiles = max(upto - item_at - OPEN, 0) - skipped;
+            from = rq.tile0 + skipped;
+            whole = tiles == rq.tiles;
+            slot = at > item_at ? 0 : 1;
+            at = upto;
+        } while (tiles == 0);
+        return true;
+    }
+};
 
 template <typename QT, bool EIGHT, int D, int RW>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -245,16 +291,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
     const int run = warp / RW, rw = warp % RW;
     const int ratio = heads / kv_heads;
 
-    int r;
-    long long items;
-    const long long all = tiles_before<TILE>(a, requests, ratio, TILE_ROWS, kv_heads, -1, r, items);
-    const int blocks = working_blocks(all, items, gridDim.x, RUNS);
-    if ((int)blockIdx.x >= blocks) return;
-    long long at = all * blockIdx.x / blocks;
-    const long long until = all * (blockIdx.x + 1) / blocks;
-    if (at >= until) return;
-    long long unused;
-    long long request_at = tiles_before<TILE>(a, requests, ratio, TILE_ROWS, kv_heads, at, r, unused);
+    Walk<TILE, OPEN> walk(a, requests, ratio, TILE_ROWS, kv_heads, gridDim.x, RUNS);
 
     // Where this lane's pieces lie: what it copies, keys (by the two, or four, quarters of a row's bytes), values.
     const uint32_t ring_at = shared_address(smem) + run * (STAGES * S::STAGE);
@@ -266,22 +303,10 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
     const unsigned plane = (unsigned)kv_heads * a.page_size;     // rows of a plane of a page
     auto page_of = [&](int sixteenth) { return (int)(((uint64_t)(unsigned)sixteenth * a.run_pages) >> 31); };
 
-    for (bool first_segment = true;; first_segment = false) {
-        // The item at `at`, and the part of its tiles that is this block's.
-        Request rq = request_of<TILE>(a, r, ratio, TILE_ROWS);
-        while (at >= request_at + (long long)rq.row_tiles * kv_heads * rq.tiles) {
-            request_at += (long long)rq.row_tiles * kv_heads * rq.tiles;
-            rq = request_of<TILE>(a, ++r, ratio, TILE_ROWS);
-        }
-        const long long item = (at - request_at) / rq.tiles;
-        const int kv = (int)(item % kv_heads), first = (int)(item / kv_heads) * TILE_ROWS;
-        const long long item_at = request_at + item * rq.tiles;
-        const int skipped = (int)(at - item_at), taken = (int)(min(until, item_at + rq.tiles) - at);
-        const bool whole_item = skipped == 0 && taken == rq.tiles;
-        at += taken;
-        const int history = rq.history, start = rq.start, pairs = rq.pairs, end = rq.end, low = rq.low;
-        const int from = rq.tile0 + skipped;
-        const int mine = max(0, (taken - run + RUNS - 1) / RUNS);             // tiles of this group: from + run, + RUNS, ...
+    while (walk.next(a)) {
+        const int history = walk.rq.history, start = walk.rq.start, pairs = walk.rq.pairs, end = walk.rq.end, low = walk.rq.low;
+        const int from = walk.from, first = walk.first, kv = walk.kv, r = walk.r;
+        const int mine = max(0, (walk.tiles - run + RUNS - 1) / RUNS);             // tiles of this group: from + run, + RUNS, ...
 
         const int* table = a.tables + (size_t)r * a.table_stride;
         // A tile's keys lie in two runs of 16, each within a page.  Lookups are made one tile ahead of the copies.
@@ -583,7 +608,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
             }
         }
         __syncthreads();
-        float* slot = partial + (2 * (size_t)blockIdx.x + !first_segment) * TILE_ROWS * ROWF;
+        float* slot = partial + (2 * (size_t)blockIdx.x + walk.slot) * TILE_ROWS * ROWF;
         for (int x = threadIdx.x; x < TILE_ROWS * (D / 4); x += WARPS * 32) {
             const int local = x / (D / 4), d = 4 * (x % (D / 4)), pair = first + local;
             if (pair >= pairs) continue;
@@ -604,21 +629,20 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
                 acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
                 l = fmaf(row[D + 2], share(row[D + 1], most), l);
             }
-            if (whole_item) {
+            if (walk.whole) {
                 write4(out + ((size_t)(start + pair / ratio) * heads + kv * ratio + pair % ratio) * D + d, finished<EIGHT>(acc, t, most, l));
             } else {
                 *reinterpret_cast<float4*>(slot + (size_t)local * ROWF + d) = acc;
                 if (d == 0) *reinterpret_cast<float4*>(slot + (size_t)local * ROWF + D) = make_float4(t, most, l, 0.0f);
             }
         }
-        if (at >= until) return;
         __syncthreads();
     }
 }
 
 // Adds up the items that blocks share, one warp for 128 of a (row, head)'s values (two rows of 64).  Which blocks those are follows
 // from the same counts as in the kernel before.
-template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int RUNS>
+template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int OPEN, int RUNS>
 __global__ void __launch_bounds__(128)
 merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, int requests, int heads, int kv_heads, int grid) {
     constexpr int ROWF = D + PART, LANES = D / 4, EACH = 128 / LANES;
@@ -628,45 +652,42 @@ merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, in
     const Request rq = request_of<KEYS>(a, r, ratio, TILE_ROWS);
     const long long first_item = (long long)blockIdx.x * EACH;
     if (first_item >= (long long)rq.count * heads) return pdl_wait();
-    int found;
-    long long items, unused;
-    const long long all = tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
-    const int blocks = working_blocks(all, items, grid, RUNS);
-    // The place of this request's tiles: before it lie those of the requests 0 .. r - 1.
-    const long long request_at = tiles_before<KEYS>(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
+    int found, items, unused;
+    const int all = places_before<KEYS, OPEN>(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
+    const int blocks = working_blocks<OPEN>(all, items, grid, RUNS);
+    // The place of this request's items: before it lie those of the requests 0 .. r - 1.
+    const int request_at = places_before<KEYS, OPEN>(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
     const long long item = first_item + threadIdx.x / LANES;
     if (item >= (long long)rq.count * heads) return pdl_wait();
-    const int row = (int)(item / heads), head = (int)(item % heads), kv = head / ratio, pair = row * ratio + head % ratio, d = 4 * (threadIdx.x % LANES);
-    const long long x0 = request_at + ((long long)(pair / TILE_ROWS) * kv_heads + kv) * rq.tiles, x1 = x0 + rq.tiles;
-    // Block b has the tiles all * b / blocks up to all * (b + 1) / blocks.
-    auto block_of = [&](long long x) { return (int)(((x + 1) * blocks - 1) / all); };
-    const int b0 = block_of(x0), b1 = block_of(x1 - 1);
+    const int row = (int)item / heads, head = (int)item % heads, kv = head / ratio, pair = row * ratio + head % ratio, d = 4 * (threadIdx.x % LANES);
+    const int x0 = request_at + (pair / TILE_ROWS * kv_heads + kv) * (rq.tiles + OPEN), x1 = x0 + rq.tiles + OPEN;
+    auto block_of = [&](int x) { return (int)(((unsigned long long)(x + 1) * blocks - 1) / all); };
+    const int b0 = block_of(x0 + OPEN), b1 = block_of(x1 - 1);       // of the first tile and the last
     pdl_wait();
     if (b0 == b1) return;
-    // A block's first segment lies in its first slot; the item is that of all blocks but the first, unless that one begins with it.
-    const int slot0 = 2 * b0 + (all * b0 / blocks < x0 ? 1 : 0);
+    const int slot0 = 2 * b0 + (share_begins(all, blocks, b0) > x0 ? 0 : 1);
     const float* base = partial + (size_t)(pair % TILE_ROWS) * ROWF;
     auto state = [&](int b) { return base + (size_t)(b == b0 ? slot0 : 2 * b) * TILE_ROWS * ROWF; };
     float t = -INFINITY, most = -INFINITY;
-    for (int b = b0; b <= b1; b += 4) {
-        float4 m[4];
+    for (int b = b0; b <= b1; b += 8) {
+        float4 m[8];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) m[n] = *reinterpret_cast<const float4*>(state(min(b + n, b1)) + D);
+        for (int n = 0; n < 8; ++n) m[n] = *reinterpret_cast<const float4*>(state(min(b + n, b1)) + D);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) t = fmaxf(t, m[n].x), most = fmaxf(most, m[n].y);
+        for (int n = 0; n < 8; ++n) t = fmaxf(t, m[n].x), most = fmaxf(most, m[n].y);
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f;
-    for (int b = b0; b <= b1; b += 4) {
-        float4 v[4], m[4];
+    for (int b = b0; b <= b1; b += 8) {
+        float4 v[8], m[8];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 8; ++n) {
             const float* s = state(min(b + n, b1));
             v[n] = *reinterpret_cast<const float4*>(s + d);
             m[n] = *reinterpret_cast<const float4*>(s + D);
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 8; ++n)
             if (b + n <= b1) {
                 const float f = share(m[n].x, t);
                 acc.x = fmaf(v[n].x, f, acc.x); acc.y = fmaf(v[n].y, f, acc.y); acc.z = fmaf(v[n].z, f, acc.z); acc.w = fmaf(v[n].w, f, acc.w);

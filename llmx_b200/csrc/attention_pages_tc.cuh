@@ -33,11 +33,10 @@ using mma_pages::copy16;
 using mma_pages::exp2_fast;
 using mma_pages::max3;
 using mma_pages::PART;
-using mma_pages::Request;
-using mma_pages::request_of;
 using mma_pages::Rows;
 
 constexpr int KEYS = 128, D = 128;
+constexpr int OPEN = 3;                 // tiles that an item's beginning and end take as long as
 constexpr int UNIT_WARPS = 4, LOADER = 10;
 // The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
 // leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
@@ -63,9 +62,9 @@ struct Shape {
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
     static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
     // What a unit's threads tell each other, in floats: factors, minus the sum's reference, the weights' beside it, what raising scales
-    // the two by, positions [R];
+    // the two by, positions, rows of the output [R];
     // maxima and sums of warps [2][4][R].
-    static constexpr int UNIT_FLOATS = 6 * R + 2 * UNIT_WARPS * R;
+    static constexpr int UNIT_FLOATS = 8 * R + 2 * UNIT_WARPS * R;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
     static constexpr int AT_STRAY = AT_FLOATS + U * UNIT_FLOATS * 4;                    // [rows][D] products with values that are no numbers
     static constexpr int AT_BARRIERS = AT_STRAY + (EIGHT ? 0 : U * R * D * 4);
@@ -225,44 +224,15 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     pdl_trigger();
 
     // ---- the work, which every role walks alike
-    int r0;
-    long long items;
-    const long long all = mma_pages::tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, -1, r0, items);
-    const int blocks = mma_pages::working_blocks(all, items, gridDim.x, 1);
-    long long at = (int)blockIdx.x < blocks ? all * blockIdx.x / blocks : 0;
-    const long long until = (int)blockIdx.x < blocks ? all * (blockIdx.x + 1) / blocks : 0;
-    long long unused;
-    long long request_at = mma_pages::tiles_before<KEYS>(a, requests, ratio, TILE_ROWS, kv_heads, at, r0, unused);
+    mma_pages::Walk<KEYS, OPEN> sg(a, requests, ratio, TILE_ROWS, kv_heads, gridDim.x, 1);
     const int runs_a_page = a.page_size >> 4;
     auto page_of = [&](int sixteenth) { return (int)(((uint64_t)(unsigned)sixteenth * a.run_pages) >> 31); };
-    struct Segment {
-        Request rq;
-        int r, kv, first, from, tiles;
-        bool whole;
-    } sg;
-    sg.r = r0;
-    auto next_segment = [&]() -> bool {
-        if (at >= until) return false;
-        sg.rq = request_of<KEYS>(a, sg.r, ratio, TILE_ROWS);
-        while (at >= request_at + (long long)sg.rq.row_tiles * kv_heads * sg.rq.tiles) {
-            request_at += (long long)sg.rq.row_tiles * kv_heads * sg.rq.tiles;
-            sg.rq = request_of<KEYS>(a, ++sg.r, ratio, TILE_ROWS);
-        }
-        const long long item = (at - request_at) / sg.rq.tiles, item_at = request_at + item * sg.rq.tiles;
-        sg.kv = (int)(item % kv_heads), sg.first = (int)(item / kv_heads) * TILE_ROWS;
-        const int skipped = (int)(at - item_at);
-        sg.tiles = (int)(min(until, item_at + sg.rq.tiles) - at);
-        sg.whole = skipped == 0 && sg.tiles == sg.rq.tiles;
-        sg.from = sg.rq.tile0 + skipped;
-        at += sg.tiles;
-        return true;
-    };
 
     if (warp == 0 || warp == LOADER) {
         const int p = lane & 7, plane = (lane >> 3) & 1;          // a run of 16 keys; for exponents, keys' or values'
         uint32_t use = 0;
         bool ok = true;
-        while (ok && next_segment()) {
+        while (ok && sg.next(a)) {
             const int* table = a.tables + (size_t)sg.r * a.table_stride;
             // The pages of four tiles' 32 runs at a time, a lane each, asked for four tiles ahead: a lookup takes as long as a tile.
             auto look_up = [&](int i) {
@@ -318,7 +288,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         if (tc::elect_one()) {
             uint32_t use = 0, segments = 0, scored[U] = {0, 0}, weighed[U] = {0, 0};       // tiles so far; units' S^T and O^T so far
             bool ok = true;
-            while (ok && next_segment()) {
+            while (ok && sg.next(a)) {
                 for (int u = 0; u < U && ok; ++u) ok = tc::mbar_wait(&q_full[u], segments & 1u, abort_flag, error_word, ERR_PAGES_MMA);
                 ++segments;
                 // S^T of tile `next`, O^T of `tile` (of unit `turn`, where both units have every tile): whichever finds what it needs.
@@ -404,13 +374,14 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
         float *factor = shared, *minus_peak = shared + R, *shift = shared + 2 * R, *fade_sum = shared + 3 * R, *fade_o = shared + 4 * R;
         int* position = reinterpret_cast<int*>(shared + 5 * R);
-        float *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
+        int* out_row = position + R;                            // (head's row of the output, -1: none)
+        float *warp_peak = shared + 8 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + (S::HALVES ? 0 : unit * S::WEIGHTS)) + key * 128;
         uint32_t before = 0, mine = 0;                          // tiles of the segments before; this unit's so far
-        bool ok = true, first_segment = true;
-        for (; next_segment(); before += sg.tiles, first_segment = false) {
+        bool ok = true;
+        for (; sg.next(a); before += sg.tiles) {
             const int first = sg.first + (SHARED ? 0 : unit * R), pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
             // ---- the unit's queries: a row by 128 / R threads
             {
@@ -466,6 +437,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     factor[row] = f;
                     minus_peak[row] = shift[row] = 0.0f;
                     position[row] = real ? history + token : -1;
+                    out_row[row] = real ? (start + token) * heads + sg.kv * ratio + pair % ratio : -1;
                 }
                 tc::fence_proxy_async();
                 unit_barrier(unit);
@@ -700,7 +672,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             tc::tc_fence_after();
             unit_barrier(unit);
             const bool any_stray = !EIGHT && stray_flag[unit];
-            float* slot = partial + (2 * (size_t)blockIdx.x + !first_segment) * TILE_ROWS * ROWF;
+            float* slot = partial + (2 * (size_t)blockIdx.x + sg.slot) * TILE_ROWS * ROWF;
             // The second unit's sums go to the first by way of the weights' place, once both have no use for that.
             float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS);
             if (SHARED) units_barrier();
@@ -738,15 +710,15 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 units_barrier();
             } else {
                 if (SHARED) units_barrier();
-                const float *theirs = shared + S::UNIT_FLOATS, *their_sums = theirs + 6 * R;
+                const float *theirs = shared + S::UNIT_FLOATS, *their_sums = theirs + 8 * R;
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     float o[16];
                     outputs(c, o);
 #pragma unroll
                     for (int n = 0; n < 16; ++n) {
-                        const int row = 16 * c + n, pair = first + row;
-                        if (pair >= pairs) continue;
+                        const int row = 16 * c + n, to_row = out_row[row];
+                        if (to_row < 0) continue;
                         float total = total_of(warp_peak, row), peak = -minus_peak[row], top = peak - shift[row];
                         if (both) {
                             const float peak2 = -theirs[R + row], top2 = peak2 - theirs[2 * R + row], p = fmaxf(peak, peak2), t = fmaxf(top, top2);
@@ -756,7 +728,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         }
                         if (sg.whole) {
                             const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
-                            out[((size_t)(start + pair / ratio) * heads + sg.kv * ratio + pair % ratio) * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
+                            out[(size_t)to_row * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
                         } else {
                             float* to = slot + (size_t)((SHARED ? 0 : unit * R) + row) * ROWF;
                             to[key] = o[n];
