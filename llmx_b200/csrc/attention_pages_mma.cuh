@@ -200,42 +200,58 @@ __device__ __forceinline__ Request request_of(const Rows& a, int r, int ratio, i
     q.row_tiles = (q.pairs + tile_rows - 1) / tile_rows;
     return q;
 }
-// The places of all requests, and how many items they are; where `x` is at least 0, the places before the request that it falls in,
-// which `found` names.  By whole warps.
+// A request's items and places.
 template <int KEYS, int OPEN>
-__device__ __forceinline__ int places_before(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, int x, int& found, int& items) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;
+__device__ __forceinline__ int places_of(const Rows& a, int r, int requests, int ratio, int tile_rows, int kv_heads, int& items) {
     items = 0;
-    found = requests;
-    for (int r0 = 0; r0 < requests; r0 += 32) {
-        int n = 0, of = 0;
-        if (r0 + lane < requests) {
-            const Request q = request_of<KEYS>(a, r0 + lane, ratio, tile_rows);
-            of = q.row_tiles * kv_heads;
-            n = of * (q.tiles + OPEN);
-        }
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned here = __ballot_sync(0xffffffffu, x >= 0 && x < before + upto);
-        if (here) {
-            const int at = __ffs(here) - 1;
-            found = r0 + at;
-            return before + __shfl_sync(0xffffffffu, upto - n, at);
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-        items += (int)__reduce_add_sync(0xffffffffu, (unsigned)of);
+    if (r >= requests) return 0;
+    const Request q = request_of<KEYS>(a, r, ratio, tile_rows);
+    items = q.row_tiles * kv_heads;
+    return items * (q.tiles + OPEN);
+}
+// The places and items of all requests, and the places of the first `stop`.  By whole warps.
+template <int KEYS, int OPEN>
+__device__ __forceinline__ int all_places(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, int& items, int stop, int& before) {
+    const int lane = threadIdx.x & 31;
+    unsigned all = 0, of = 0, first = 0;
+    for (int r = lane; r - lane < requests; r += 32) {
+        int n;
+        const unsigned places = places_of<KEYS, OPEN>(a, r, requests, ratio, tile_rows, kv_heads, n);
+        all += places, of += n;
+        if (r < stop) first += places;
     }
-    return before;
+    items = (int)__reduce_add_sync(0xffffffffu, of);
+    before = (int)__reduce_add_sync(0xffffffffu, first);
+    return (int)__reduce_add_sync(0xffffffffu, all);
+}
+// The request that place `x` falls in, and the places before it.  By whole warps.
+template <int KEYS, int OPEN>
+__device__ __forceinline__ int request_at_place(const Rows& a, int requests, int ratio, int tile_rows, int kv_heads, int x, int& before) {
+    const int lane = threadIdx.x & 31;
+    before = 0;
+    for (int r0 = 0; r0 < requests; r0 += 32) {
+        int items, upto = places_of<KEYS, OPEN>(a, r0 + lane, requests, ratio, tile_rows, kv_heads, items);
+        const int n = upto, sum = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+        if (x < before + sum) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int in = __ffs(__ballot_sync(0xffffffffu, x < before + upto)) - 1;
+            before += __shfl_sync(0xffffffffu, upto - n, in);
+            return r0 + in;
+        }
+        before += sum;
+    }
+    return requests;
 }
 // The blocks that share the work: all of the grid, as far as each gets two tiles a group of warps or an item of its own.
 template <int OPEN>
 __device__ __forceinline__ int working_blocks(int all, int items, int blocks, int runs) { return min(blocks, max(items, (all - items * OPEN) / (2 * runs))); }
-__device__ __forceinline__ int share_begins(int all, int blocks, int b) { return (int)((unsigned long long)all * b / blocks); }
+__device__ __forceinline__ int share_begins(int all, int blocks, int b) {
+    return all < 1 << 20 ? (int)((unsigned)all * b / blocks) : (int)((unsigned long long)all * b / blocks);      // (blocks are a few hundred)
+}
 
 // A block's items one after another.
 template <int KEYS, int OPEN>
@@ -247,11 +263,11 @@ struct Walk {
     __device__ __forceinline__ Walk(const Rows& a, int requests, int ratio_, int tile_rows_, int kv_heads_, int grid, int runs)
         : tile_rows(tile_rows_), kv_heads(kv_heads_), ratio(ratio_) {
         int items, unused;
-        const int all = places_before<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, -1, r, items), blocks = working_blocks<OPEN>(all, items, grid, runs);
+        const int all = all_places<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, items, 0, unused), blocks = working_blocks<OPEN>(all, items, grid, runs);
         const bool works = (int)blockIdx.x < blocks;
         at = works ? share_begins(all, blocks, blockIdx.x) : 0;
         until = works ? share_begins(all, blocks, blockIdx.x + 1) : 0;
-        request_at = places_before<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, at, r, unused);
+        r = request_at_place<KEYS, OPEN>(a, requests, ratio, tile_rows, kv_heads, at, request_at);
         if (at < until) rq = request_of<KEYS>(a, r, ratio, tile_rows);
     }
     __device__ __forceinline__ bool next(const Rows& a) {
@@ -652,11 +668,9 @@ merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, in
     const Request rq = request_of<KEYS>(a, r, ratio, TILE_ROWS);
     const long long first_item = (long long)blockIdx.x * EACH;
     if (first_item >= (long long)rq.count * heads) return pdl_wait();
-    int found, items, unused;
-    const int all = places_before<KEYS, OPEN>(a, requests, ratio, TILE_ROWS, kv_heads, -1, found, items);
-    const int blocks = working_blocks<OPEN>(all, items, grid, RUNS);
-    // The place of this request's items: before it lie those of the requests 0 .. r - 1.
-    const int request_at = places_before<KEYS, OPEN>(a, r, ratio, TILE_ROWS, kv_heads, -1, found, unused);
+    // (The place of this request's items: before it lie those of the requests 0 .. r - 1.)
+    int items, request_at;
+    const int all = all_places<KEYS, OPEN>(a, requests, ratio, TILE_ROWS, kv_heads, items, r, request_at), blocks = working_blocks<OPEN>(all, items, grid, RUNS);
     const long long item = first_item + threadIdx.x / LANES;
     if (item >= (long long)rq.count * heads) return pdl_wait();
     const int row = (int)item / heads, head = (int)item % heads, kv = head / ratio, pair = row * ratio + head % ratio, d = 4 * (threadIdx.x % LANES);

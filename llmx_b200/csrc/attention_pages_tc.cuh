@@ -15,6 +15,7 @@
 //   warps 0, 10     page lookups and copies, STAGES tiles ahead, every other tile each: 16 keys and their values a copy (a warp issues
 //                   one in some 100 clocks, which by itself would be less than memory gives)
 //   warp 1          matrix instructions, whichever can be made next: S^T of tiles ahead, O^T
+//   warp 11         an item's queries, while the item before is worked on
 //   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
 //                   tile's rows are R; their states meet at the item's end), or half of the rows each (2 R)
@@ -37,7 +38,7 @@ using mma_pages::Rows;
 
 constexpr int KEYS = 128, D = 128;
 constexpr int OPEN = 3;                 // tiles that an item's beginning and end take as long as
-constexpr int UNIT_WARPS = 4, LOADER = 10;
+constexpr int UNIT_WARPS = 4, LOADER = 10, QUERIES = 11;
 // The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
 // leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
 constexpr float RAISED = 4.0f, ROOM = 57.0f, LIMIT = 8.0f;
@@ -47,7 +48,7 @@ enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 
 template <bool EIGHT, bool SHARED, int R>
 struct Shape {
     static constexpr int U = 2;
-    static constexpr int THREADS = 96 + U * UNIT_WARPS * 32;
+    static constexpr int THREADS = 128 + U * UNIT_WARPS * 32;
     // A stage: eight keys, their values, the next eight keys, ..., rows of 128 bytes; bfloat16: such a half for the rows' first 64 values
     // and one for the others.
     static constexpr int HALF = 2 * KEYS * 128, STAGE = EIGHT ? HALF : 2 * HALF;
@@ -57,16 +58,19 @@ struct Shape {
     // A tile's weights: rows of 128 bytes a key, of which a unit has one half, or all.
     static constexpr int WEIGHTS = KEYS * 128;
     static constexpr bool HALVES = !EIGHT || R == 16;
-    static constexpr int QUERIES = (EIGHT ? 2 * R * D : R * D * 2);
+    static constexpr int ROWS = SHARED ? R : U * R;             // of an item
+    static constexpr int Q_BYTES = 2 * R * D;                   // R rows' queries: two codes each, or bfloat16
+    static constexpr int Q_BUFFERS = SHARED ? 2 : 1;            // (two would not fit)
     static constexpr int S_COLS = EIGHT ? 2 * R : R, O_COLS = EIGHT ? 3 * R : R, U_COLS = 2 * S_COLS + O_COLS;
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
-    static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + U * QUERIES;
-    // What a unit's threads tell each other, in floats: factors, minus the sum's reference, the weights' beside it, what raising scales
-    // the two by, positions, rows of the output [R];
-    // maxima and sums of warps [2][4][R].
-    static constexpr int UNIT_FLOATS = 8 * R + 2 * UNIT_WARPS * R;
+    static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + Q_BUFFERS * (ROWS / R) * Q_BYTES;
+    // What a unit's threads tell each other, in floats: minus the sum's reference, the weights' beside it, what raising scales the two by,
+    // what the item's end scales its outputs and the other unit's by [R]; maxima and sums of warps [2][4][R].
+    static constexpr int UNIT_FLOATS = 6 * R + 2 * UNIT_WARPS * R;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
-    static constexpr int AT_STRAY = AT_FLOATS + U * UNIT_FLOATS * 4;                    // [rows][D] products with values that are no numbers
+    // What the queries' warp tells, of an item's rows: factors, positions, rows of the output (-1: none).
+    static constexpr int AT_ROWS = AT_FLOATS + U * UNIT_FLOATS * 4;
+    static constexpr int AT_STRAY = AT_ROWS + Q_BUFFERS * 3 * ROWS * 4;                 // [rows][D] products with values that are no numbers
     static constexpr int AT_BARRIERS = AT_STRAY + (EIGHT ? 0 : U * R * D * 4);
     static constexpr int BYTES = AT_BARRIERS + 512 + 1024;                              // and to the next 1024
 };
@@ -177,8 +181,9 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = (uint64_t*)(smem + S::AT_BARRIERS);        // [STAGES]
     uint64_t* empty = full + STAGES;                            // [STAGES]
-    uint64_t* q_full = empty + STAGES;                          // [U]
-    uint64_t* s_full = q_full + U;                              // [U][2]
+    uint64_t* q_full = empty + STAGES;                          // [Q_BUFFERS]
+    uint64_t* q_free = q_full + 2;                              // [Q_BUFFERS]
+    uint64_t* s_full = q_free + 2;                              // [U][2]
     uint64_t* s_free = s_full + 2 * U;                          // [U][2]
     uint64_t* w_full = s_free + 2 * U;                          // [U]
     uint64_t* o_done = w_full + U;                              // [U]: O^T with these weights
@@ -192,7 +197,8 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], EIGHT ? 17 : 1), tc::mbar_init(&empty[i], 1);     // (copies' bytes; 16 lanes' exponents)
         for (int u = 0; u < U; ++u) {
-            tc::mbar_init(&q_full[u], UNIT_WARPS);
+            tc::mbar_init(&q_full[u], 1);
+            tc::mbar_init(&q_free[u], 1 + U * UNIT_WARPS);
             for (int i = 0; i < 2; ++i) {
                 tc::mbar_init(&s_full[2 * u + i], 1);
                 tc::mbar_init(&s_free[2 * u + i], UNIT_WARPS);
@@ -209,8 +215,6 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         tc::tmem_alloc(tmem_slot, S::TMEM);
         tc::tmem_relinquish();
     }
-    // Values that no copy has written yet are zeros, never what the memory held before: a weight of zero meets them.
-    for (int i = threadIdx.x; i < STAGES * S::STAGE / 16; i += S::THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if constexpr (!EIGHT)
         for (int i = threadIdx.x; i < U * R * D / 4; i += S::THREADS) reinterpret_cast<float4*>(smem + S::AT_STRAY)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     tc::fence_proxy_async();
@@ -284,13 +288,80 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 }
             }
         }
+    } else if (warp == QUERIES) {
+        // An item's queries while the one before it is worked on: two lanes a row.
+        uint32_t segment = 0;
+        bool ok = true;
+        for (; sg.next(a); ++segment) {
+            const int buffer = segment % S::Q_BUFFERS;
+            ok = tc::mbar_wait_warp(&q_free[buffer], ((segment / S::Q_BUFFERS) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
+            if (!ok) break;
+            float* info = reinterpret_cast<float*>(smem + S::AT_ROWS) + buffer * 3 * S::ROWS;
+            const int part = lane & 1;
+            for (int row0 = 0; row0 < S::ROWS; row0 += 16) {
+                const int item_row = row0 + (lane >> 1), row = item_row % R, pair = sg.first + item_row;
+                const bool real = pair < sg.rq.pairs;
+                const int token = real ? pair / ratio : 0, to_row = (sg.rq.start + token) * heads + sg.kv * ratio + (real ? pair - token * ratio : 0);
+                const __nv_bfloat16* src = q + (size_t)to_row * D + part * 64;
+                uint8_t* queries = smem + S::AT_QUERIES + (buffer * (S::ROWS / R) + item_row / R) * S::Q_BYTES;
+                uint4 x[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) x[n] = real ? reinterpret_cast<const uint4*>(src)[n] : make_uint4(0, 0, 0, 0);
+                float f = scale_log2;
+                if constexpr (EIGHT) {
+                    unsigned most = 0;                           // magnitudes of bfloat16 compare as their bits do
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const unsigned v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) most = max(most, max(v[k] & 0x7FFFu, v[k] >> 16 & 0x7FFFu));
+                    }
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    const int e = min(max((int)(most >> 7) - 127, -100), 127);     // the row's largest lies in 2^e .. 2^(e + 1): to 2^7 .. 2^8
+                    const float up = __int_as_float((127 + 7 - e) << 23);
+                    f = fmaxf(__int_as_float((127 - 7 + e) << 23) * scale_log2, 1.0e-44f);     // (not zero: a masked score stays -inf)
+                    const bool bad = most >= 0x7F80u;            // a row with an infinity or a NaN: codes that are NaN
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        uint32_t one[4], two[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4& from = x[2 * n + (k >> 1)];
+                            const unsigned w0 = k & 1 ? from.z : from.x, w1 = k & 1 ? from.w : from.y;
+                            const float v[4] = {__uint_as_float(w0 << 16) * up, __uint_as_float(w0 & 0xffff0000u) * up, __uint_as_float(w1 << 16) * up,
+                                                __uint_as_float(w1 & 0xffff0000u) * up};
+                            const unsigned c0 = e4m3::pack2(v[0], v[1]), c1 = e4m3::pack2(v[2], v[3]);
+                            const float2 b0 = mma_pages::from_halves(e4m3::halves((unsigned short)c0)), b1 = mma_pages::from_halves(e4m3::halves((unsigned short)c1));
+                            one[k] = bad ? 0x7F7F7F7Fu : c0 | c1 << 16;
+                            two[k] = e4m3::pack2((v[0] - b0.x) * 32.0f, (v[1] - b0.y) * 32.0f) | e4m3::pack2((v[2] - b1.x) * 32.0f, (v[3] - b1.y) * 32.0f) << 16;
+                        }
+                        const int piece = part * 4 + n, r1 = (row >> 4) * 32 + (row & 15), r2 = r1 + 16;
+                        *reinterpret_cast<uint4*>(queries + r1 * 128 + ((piece ^ (r1 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
+                        *reinterpret_cast<uint4*>(queries + r2 * 128 + ((piece ^ (r2 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) *reinterpret_cast<uint4*>(queries + part * (R * 128) + row * 128 + ((n ^ (row & 7)) << 4)) = x[n];
+                }
+                if (part == 0) {
+                    info[item_row] = f;
+                    reinterpret_cast<int*>(info)[S::ROWS + item_row] = real ? sg.rq.history + token : -1;
+                    reinterpret_cast<int*>(info)[2 * S::ROWS + item_row] = real ? to_row : -1;
+                }
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&q_full[buffer]);
+        }
     } else if (warp == 1) {
         if (tc::elect_one()) {
             uint32_t use = 0, segments = 0, scored[U] = {0, 0}, weighed[U] = {0, 0};       // tiles so far; units' S^T and O^T so far
             bool ok = true;
             while (ok && sg.next(a)) {
-                for (int u = 0; u < U && ok; ++u) ok = tc::mbar_wait(&q_full[u], segments & 1u, abort_flag, error_word, ERR_PAGES_MMA);
+                const int q_buffer = segments % S::Q_BUFFERS;
+                ok = tc::mbar_wait(&q_full[q_buffer], (segments / S::Q_BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_MMA);
                 ++segments;
+                tc::tc_fence_after();
                 // S^T of tile `next`, O^T of `tile` (of unit `turn`, where both units have every tile): whichever finds what it needs.
                 int next = 0, tile = 0, turn = 0;
                 unsigned long long since = 0;
@@ -305,7 +376,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                             const uint32_t keys = tc::smem_u32(smem + stage * S::STAGE);
                             for (int u = u0; u <= u1; ++u) {
                                 const int buffer = scored[u]++ & 1;
-                                const uint32_t queries = tc::smem_u32(smem + S::AT_QUERIES + u * S::QUERIES), d = tmem + u * S::U_COLS + buffer * S::S_COLS;
+                                const uint32_t queries = tc::smem_u32(smem + S::AT_QUERIES + (q_buffer * (S::ROWS / R) + (SHARED ? 0 : u)) * S::Q_BYTES), d = tmem + u * S::U_COLS + buffer * S::S_COLS;
                                 if constexpr (EIGHT) {
 #pragma unroll
                                     for (int k = 0; k < D / 32; ++k)
@@ -319,7 +390,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                                 }
                                 tc::mma_commit(&s_full[2 * u + buffer]);
                             }
-                            ++next;
+                            if (++next == sg.tiles) tc::mma_commit(&q_free[q_buffer]);
                             made = true;
                         }
                     }
@@ -372,77 +443,21 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem + unit * S::U_COLS + lanes, o_at = s_at + 2 * S::S_COLS;
         float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
-        float *factor = shared, *minus_peak = shared + R, *shift = shared + 2 * R, *fade_sum = shared + 3 * R, *fade_o = shared + 4 * R;
-        int* position = reinterpret_cast<int*>(shared + 5 * R);
-        int* out_row = position + R;                            // (head's row of the output, -1: none)
-        float *warp_peak = shared + 8 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
+        float *minus_peak = shared, *shift = shared + R, *fade_sum = shared + 2 * R, *fade_o = shared + 3 * R, *own_scale = shared + 4 * R,
+              *given_scale = shared + 5 * R, *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + (S::HALVES ? 0 : unit * S::WEIGHTS)) + key * 128;
-        uint32_t before = 0, mine = 0;                          // tiles of the segments before; this unit's so far
+        const float* rows_info = reinterpret_cast<const float*>(smem + S::AT_ROWS) + (SHARED ? 0 : unit * R);
+        uint32_t before = 0, mine = 0, segment = 0;             // tiles of the items before; this unit's so far; items
         bool ok = true;
-        for (; sg.next(a); before += sg.tiles) {
+        for (; sg.next(a); before += sg.tiles, ++segment) {
             const int first = sg.first + (SHARED ? 0 : unit * R), pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
-            // ---- the unit's queries: a row by 128 / R threads
-            {
-                constexpr int EACH = 128 / R, OWN = D / EACH;
-                const int row = thread / EACH, part = thread % EACH, pair = first + row;
-                const bool real = pair < pairs;
-                const int token = real ? pair / ratio : 0;
-                const __nv_bfloat16* src = q + ((size_t)(start + token) * heads + sg.kv * ratio + (real ? pair % ratio : 0)) * D + part * OWN;
-                uint4 x[OWN / 8];
-#pragma unroll
-                for (int n = 0; n < OWN / 8; ++n) x[n] = real ? reinterpret_cast<const uint4*>(src)[n] : make_uint4(0, 0, 0, 0);
-                uint8_t* queries = smem + S::AT_QUERIES + unit * S::QUERIES;
-                float f = scale_log2;
-                if constexpr (EIGHT) {
-                    unsigned most = 0;                           // magnitudes of bfloat16 compare as their bits do
-#pragma unroll
-                    for (int n = 0; n < OWN / 8; ++n) {
-                        const unsigned v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) most = max(most, max(v[k] & 0x7FFFu, v[k] >> 16 & 0x7FFFu));
-                    }
-#pragma unroll
-                    for (int o = 1; o < EACH; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    const int e = min(max((int)(most >> 7) - 127, -100), 127);     // the row's largest lies in 2^e .. 2^(e + 1): to 2^7 .. 2^8
-                    const float up = __int_as_float((127 + 7 - e) << 23);
-                    f = fmaxf(__int_as_float((127 - 7 + e) << 23) * scale_log2, 1.0e-44f);     // (not zero: a masked score stays -inf)
-                    const bool bad = most >= 0x7F80u;            // a row with an infinity or a NaN: codes that are NaN
-#pragma unroll
-                    for (int n = 0; n < OWN / 16; ++n) {
-                        uint32_t one[4], two[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const unsigned w0 = (&x[2 * n + (k >> 1)].x)[2 * (k & 1)], w1 = (&x[2 * n + (k >> 1)].x)[2 * (k & 1) + 1];
-                            const float v[4] = {__uint_as_float(w0 << 16) * up, __uint_as_float(w0 & 0xffff0000u) * up, __uint_as_float(w1 << 16) * up,
-                                                __uint_as_float(w1 & 0xffff0000u) * up};
-                            const unsigned c0 = e4m3::pack2(v[0], v[1]), c1 = e4m3::pack2(v[2], v[3]);
-                            const float2 b0 = mma_pages::from_halves(e4m3::halves((unsigned short)c0)), b1 = mma_pages::from_halves(e4m3::halves((unsigned short)c1));
-                            one[k] = bad ? 0x7F7F7F7Fu : c0 | c1 << 16;
-                            two[k] = e4m3::pack2((v[0] - b0.x) * 32.0f, (v[1] - b0.y) * 32.0f) | e4m3::pack2((v[2] - b1.x) * 32.0f, (v[3] - b1.y) * 32.0f) << 16;
-                        }
-                        const int piece = part * (OWN / 16) + n, r1 = (row >> 4) * 32 + (row & 15), r2 = r1 + 16;
-                        *reinterpret_cast<uint4*>(queries + r1 * 128 + ((piece ^ (r1 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
-                        *reinterpret_cast<uint4*>(queries + r2 * 128 + ((piece ^ (r2 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < OWN / 8; ++n) {
-                        const int piece = part * (OWN / 8) + n;
-                        *reinterpret_cast<uint4*>(queries + (piece >> 3) * (R * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = x[n];
-                    }
-                }
-                if (part == 0) {
-                    factor[row] = f;
-                    minus_peak[row] = shift[row] = 0.0f;
-                    position[row] = real ? history + token : -1;
-                    out_row[row] = real ? (start + token) * heads + sg.kv * ratio + pair % ratio : -1;
-                }
-                tc::fence_proxy_async();
-                unit_barrier(unit);
-                if (lane == 0) tc::mbar_arrive(&q_full[unit]);
-            }
+            const int q_buffer = segment % S::Q_BUFFERS;
+            if (ok) ok = tc::mbar_wait_warp(&q_full[q_buffer], (segment / S::Q_BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+            const float* factor = rows_info + q_buffer * 3 * S::ROWS;
+            const int *position = reinterpret_cast<const int*>(factor) + S::ROWS, *out_row = position + S::ROWS;
+            const uint32_t factors_at = tc::smem_u32(factor);
             const int row0 = first / ratio, row1 = max(row0, (min(first + R, pairs) - 1) / ratio);
             const int all_to = a.tree ? min(history, sg.rq.end) : min(history + row0 + 1, sg.rq.end);
             const int all_from = a.window > 0 ? max(history + row1 - a.window + 1, 0) : 0;
@@ -538,21 +553,21 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         }
 #pragma unroll
                         for (int n = 0; n < 16; n += 4) {
-                            const float4 f = shared4(rows_at + 4 * (16 * c + n)),
-                                         mp = raw ? make_float4(0.f, 0.f, 0.f, 0.f) : shared4(rows_at + 4 * (R + 16 * c + n));
+                            const float4 f = shared4(factors_at + 4 * (16 * c + n)),
+                                         mp = raw ? make_float4(0.f, 0.f, 0.f, 0.f) : shared4(rows_at + 4 * (16 * c + n));
                             x[16 * c + n] = fmaf(z[n], f.x, mp.x), x[16 * c + n + 1] = fmaf(z[n + 1], f.y, mp.y);
                             x[16 * c + n + 2] = fmaf(z[n + 2], f.z, mp.z), x[16 * c + n + 3] = fmaf(z[n + 3], f.w, mp.w);
                         }
                     }
                 };
-                scores(false);                                   // (the first tile: references of zero)
+                scores(opening);                                 // (the first tile has no references yet)
                 bool raise = opening;
                 if (!opening) {
                     float over = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < R; n += 4) {
                         if constexpr (EIGHT) {
-                            const float4 s = shared4(rows_at + 4 * (2 * R + n));
+                            const float4 s = shared4(rows_at + 4 * (R + n));
                             over = max3(max3(over, x[n], x[n] + (s.x + v_power)), x[n + 1], x[n + 1] + (s.y + v_power));
                             over = max3(max3(over, x[n + 2], x[n + 2] + (s.z + v_power)), x[n + 3], x[n + 3] + (s.w + v_power));
                         } else {
@@ -584,7 +599,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     unit_barrier(unit);
 #pragma unroll
                     for (int n = 0; n < R; n += 4) {
-                        const float4 mp = shared4(rows_at + 4 * (R + n));
+                        const float4 mp = shared4(rows_at + 4 * n);
                         x[n] += mp.x, x[n + 1] += mp.y, x[n + 2] += mp.z, x[n + 3] += mp.w;
                     }
                     if (!opening) {
@@ -619,7 +634,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         sum[row] += e0;
                         sum[row + 1] += e1;
                         if constexpr (EIGHT) {
-                            if (n % 4 == 0) s = shared4(rows_at + 4 * (2 * R + row));
+                            if (n % 4 == 0) s = shared4(rows_at + 4 * (R + row));
                             const float s0 = n % 4 == 0 ? s.x : s.z, s1 = n % 4 == 0 ? s.y : s.w;
                             h[n >> 1] = mma_pages::pack_half(exp2_fast(x[row] + (s0 + v_power)), exp2_fast(x[row + 1] + (s1 + v_power)));
                         } else {
@@ -670,13 +685,12 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             }
             if (ok && any_tile) ok = tc::mbar_wait_warp(&o_done[unit], last & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
             tc::tc_fence_after();
-            unit_barrier(unit);
-            const bool any_stray = !EIGHT && stray_flag[unit];
-            float* slot = partial + (2 * (size_t)blockIdx.x + sg.slot) * TILE_ROWS * ROWF;
-            // The second unit's sums go to the first by way of the weights' place, once both have no use for that.
-            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS);
             if (SHARED) units_barrier();
-            const bool both = SHARED && sg.tiles > 1;
+            else unit_barrier(unit);
+            const bool any_stray = !EIGHT && stray_flag[unit], both = SHARED && sg.tiles > 1;
+            // The second unit's sums go to the first by way of the weights' place, for which both have no more use.
+            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS);
+            float* slot = partial + ((2 * (size_t)blockIdx.x + sg.slot) * TILE_ROWS + (SHARED ? 0 : unit * R)) * ROWF;
             auto outputs = [&](int c, float (&o)[16]) {
                 uint32_t v[16];
                 tc::tmem_ld_32x16(o_at + (EIGHT ? 48 : 16) * c, v);
@@ -697,7 +711,6 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
 #pragma unroll
                     for (int n = 0; n < 16; ++n) o[n] += strays[(16 * c + n) * D + key];
             };
-            auto total_of = [&](const float* sums, int row) { return (sums[row] + sums[R + row]) + (sums[2 * R + row] + sums[3 * R + row]); };
             if (SHARED && unit == 1) {
                 if (both)
 #pragma unroll
@@ -707,32 +720,46 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
 #pragma unroll
                         for (int n = 0; n < 16; ++n) given[(16 * c + n) * D + key] = o[n];
                     }
-                units_barrier();
-            } else {
-                if (SHARED) units_barrier();
-                const float *theirs = shared + S::UNIT_FLOATS, *their_sums = theirs + 8 * R;
+            } else if (thread < R) {
+                // A row's sum, and what its outputs are to be multiplied by.
+                const int row = thread;
+                auto total_of = [&](const float* sums) { return (sums[row] + sums[R + row]) + (sums[2 * R + row] + sums[3 * R + row]); };
+                float total = total_of(warp_peak), peak = -minus_peak[row], top = peak - shift[row], f = 1.0f, g = 0.0f;
+                if (both) {
+                    const float* theirs = shared + S::UNIT_FLOATS;
+                    const float peak2 = -theirs[row], top2 = peak2 - theirs[R + row], p = fmaxf(peak, peak2), t = fmaxf(top, top2);
+                    total = fmaf(total, exp2_fast(peak - p), total_of(theirs + 6 * R) * exp2_fast(peak2 - p));
+                    f = exp2_fast(top - t), g = exp2_fast(top2 - t);
+                    peak = p, top = t;
+                }
+                if (sg.whole) {
+                    const float s = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
+                    f *= s, g *= s;
+                } else if (out_row[row] >= 0) {
+                    float* to = slot + (size_t)row * ROWF + D;
+                    to[0] = top, to[1] = peak, to[2] = total;
+                }
+                own_scale[row] = f, given_scale[row] = g;
+            }
+            if (SHARED) units_barrier();
+            else unit_barrier(unit);
+            if (!SHARED || unit == 0) {
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     float o[16];
                     outputs(c, o);
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) {
-                        const int row = 16 * c + n, to_row = out_row[row];
-                        if (to_row < 0) continue;
-                        float total = total_of(warp_peak, row), peak = -minus_peak[row], top = peak - shift[row];
-                        if (both) {
-                            const float peak2 = -theirs[R + row], top2 = peak2 - theirs[2 * R + row], p = fmaxf(peak, peak2), t = fmaxf(top, top2);
-                            total = fmaf(total, exp2_fast(peak - p), total_of(their_sums, row) * exp2_fast(peak2 - p));
-                            o[n] = fmaf(o[n], exp2_fast(top - t), given[row * D + key] * exp2_fast(top2 - t));
-                            peak = p, top = t;
-                        }
-                        if (sg.whole) {
-                            const float f = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
-                            out[(size_t)to_row * D + key] = __float2bfloat16_rn(total == 0.0f ? 0.0f : o[n] * f);
-                        } else {
-                            float* to = slot + (size_t)((SHARED ? 0 : unit * R) + row) * ROWF;
-                            to[key] = o[n];
-                            if (key < 3) to[D + key] = key == 0 ? top : key == 1 ? peak : total;
+                    for (int n = 0; n < 16; n += 4) {
+                        const int row = 16 * c + n;
+                        const float4 f = shared4(tc::smem_u32(own_scale + row)), g = shared4(tc::smem_u32(given_scale + row));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            o[n + k] *= at4(f, k);
+                            if (both) o[n + k] = fmaf(given[(row + k) * D + key], at4(g, k), o[n + k]);
+                            const int to_row = out_row[row + k];
+                            if (to_row < 0) continue;
+                            if (sg.whole) out[(size_t)to_row * D + key] = __float2bfloat16_rn(o[n + k]);
+                            else slot[(size_t)(row + k) * ROWF + key] = o[n + k];
                         }
                     }
                 }
@@ -740,6 +767,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             tc::tc_fence_before();
             if (SHARED) units_barrier();                         // before the next item's rows take this one's places
             else unit_barrier(unit);
+            if (lane == 0) tc::mbar_arrive(&q_free[q_buffer]);
             if (any_stray) {
                 for (int n = thread; n < R * D; n += 128) strays[n] = 0.0f;
                 stray_flag[unit] = 0;
