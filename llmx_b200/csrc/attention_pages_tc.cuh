@@ -37,7 +37,7 @@ using mma_pages::PART;
 using mma_pages::Rows;
 
 constexpr int KEYS = 128, D = 128;
-constexpr int OPEN = 3;                 // tiles that an item's beginning and end take as long as
+constexpr int OPEN = 5;                 // tiles that an item's beginning and end take as long as
 constexpr int UNIT_WARPS = 4, LOADER = 10, QUERIES = 11;
 // The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
 // leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
@@ -133,6 +133,12 @@ __device__ __forceinline__ float4 shared4(uint32_t at) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ float shared1(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void to_shared1(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 __device__ __forceinline__ void to_shared4(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -689,7 +695,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
             else unit_barrier(unit);
             const bool any_stray = !EIGHT && stray_flag[unit], both = SHARED && sg.tiles > 1;
             // The second unit's sums go to the first by way of the weights' place, for which both have no more use.
-            float* given = reinterpret_cast<float*>(smem + S::AT_WEIGHTS);
+            const uint32_t given_at = tc::smem_u32(smem + S::AT_WEIGHTS);
             float* slot = partial + ((2 * (size_t)blockIdx.x + sg.slot) * TILE_ROWS + (SHARED ? 0 : unit * R)) * ROWF;
             auto outputs = [&](int c, float (&o)[16]) {
                 uint32_t v[16];
@@ -718,22 +724,24 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         float o[16];
                         outputs(c, o);
 #pragma unroll
-                        for (int n = 0; n < 16; ++n) given[(16 * c + n) * D + key] = o[n];
+                        for (int n = 0; n < 16; ++n) to_shared1(given_at + ((16 * c + n) * D + key) * 4, o[n]);
                     }
             } else if (thread < R) {
                 // A row's sum, and what its outputs are to be multiplied by.
                 const int row = thread;
-                auto total_of = [&](const float* sums) { return (sums[row] + sums[R + row]) + (sums[2 * R + row] + sums[3 * R + row]); };
-                float total = total_of(warp_peak), peak = -minus_peak[row], top = peak - shift[row], f = 1.0f, g = 0.0f;
+                auto total_of = [&](uint32_t sums) {
+                    return (shared1(sums + 4 * row) + shared1(sums + 4 * (R + row))) + (shared1(sums + 4 * (2 * R + row)) + shared1(sums + 4 * (3 * R + row)));
+                };
+                float total = total_of(rows_at + 24 * R), peak = -shared1(rows_at + 4 * row), top = peak - shared1(rows_at + 4 * (R + row)), f = 1.0f, g = 0.0f;
                 if (both) {
-                    const float* theirs = shared + S::UNIT_FLOATS;
-                    const float peak2 = -theirs[row], top2 = peak2 - theirs[R + row], p = fmaxf(peak, peak2), t = fmaxf(top, top2);
-                    total = fmaf(total, exp2_fast(peak - p), total_of(theirs + 6 * R) * exp2_fast(peak2 - p));
+                    const uint32_t theirs = rows_at + S::UNIT_FLOATS * 4;
+                    const float peak2 = -shared1(theirs + 4 * row), top2 = peak2 - shared1(theirs + 4 * (R + row)), p = fmaxf(peak, peak2), t = fmaxf(top, top2);
+                    total = fmaf(total, exp2_fast(peak - p), total_of(theirs + 24 * R) * exp2_fast(peak2 - p));
                     f = exp2_fast(top - t), g = exp2_fast(top2 - t);
                     peak = p, top = t;
                 }
                 if (sg.whole) {
-                    const float s = total == 0.0f ? 0.0f : (EIGHT ? exp2f(top - peak) : 1.0f) / total;
+                    const float s = total == 0.0f ? 0.0f : __fdividef(EIGHT ? exp2_fast(top - peak) : 1.0f, total);
                     f *= s, g *= s;
                 } else if (out_row[row] >= 0) {
                     float* to = slot + (size_t)row * ROWF + D;
@@ -751,12 +759,12 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
 #pragma unroll
                     for (int n = 0; n < 16; n += 4) {
                         const int row = 16 * c + n;
-                        const float4 f = shared4(tc::smem_u32(own_scale + row)), g = shared4(tc::smem_u32(given_scale + row));
+                        const float4 f = shared4(rows_at + 4 * (4 * R + row)), g = shared4(rows_at + 4 * (5 * R + row)), to = shared4(factors_at + 4 * (2 * S::ROWS + row));
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             o[n + k] *= at4(f, k);
-                            if (both) o[n + k] = fmaf(given[(row + k) * D + key], at4(g, k), o[n + k]);
-                            const int to_row = out_row[row + k];
+                            if (both) o[n + k] = fmaf(shared1(given_at + ((row + k) * D + key) * 4), at4(g, k), o[n + k]);
+                            const int to_row = __float_as_int(at4(to, k));
                             if (to_row < 0) continue;
                             if (sg.whole) out[(size_t)to_row * D + key] = __float2bfloat16_rn(o[n + k]);
                             else slot[(size_t)(row + k) * ROWF + key] = o[n + k];
