@@ -9,17 +9,17 @@
 // nothing.  A softmax thread has one key and all rows, so that a key's power of two is its thread's own.
 //
 // Eight bits on both sides: a query is two codes that add up to it, q = (q1 + q2 / 32) 2^e (bfloat16 has 8 bits, a code 4: exact down
-// to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 16 + w3 / 256 (12 bits, down to 2^-26 of the largest): columns of their
-// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two joins its key's score.
+// to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 32 + w3 / 1024 (12 bits, down to 2^-20 of the largest): columns of their
+// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two belongs to its key's weight.
 //
 //   warps 0, 10     page lookups and copies, STAGES tiles ahead, every other tile each: 16 keys and their values a copy (a warp issues
 //                   one in some 100 clocks, which by itself would be less than memory gives)
 //   warp 1          matrix instructions, whichever can be made next: S^T of tiles ahead, O^T
-//   warp 11         an item's queries, while the item before is worked on
+//   warp 11         an item's queries, while the item before is worked on (the first item's are the softmax warps' work)
 //   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
 //                   tile's rows are R; their states meet at the item's end), or half of the rows each (2 R)
-// The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^4 of them has the unit
+// The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^8 of them has the unit
 // raise them, and its sums and outputs (in tensor memory) scaled.  Every wait is bounded; the softmax warps go on through their
 // barriers without waiting once one has run out.
 //
@@ -39,9 +39,10 @@ using mma_pages::Rows;
 constexpr int KEYS = 128, D = 128;
 constexpr int OPEN = 5;                 // tiles that an item's beginning and end take as long as
 constexpr int UNIT_WARPS = 4, LOADER = 10, QUERIES = 11;
-// The exponentials' references: weights are 2^4 times themselves at the maximum, and up to 2^8 before it is raised (parts of a code then
-// leave 8 at most, of which 32 is a code again); the sum's lie 2^57 lower, so that one limit holds for both exponents.
-constexpr float RAISED = 4.0f, ROOM = 57.0f, LIMIT = 8.0f;
+// The exponentials' references.  A weight is 1 at the maximum, and up to 2^8 before that is raised (what a code leaves of it is then 8 at
+// most, of which 32 is a code again); over bfloat16, which has the exponents, up to 2^60.  The sum's exponentials are 2^24 at the
+// maximum: a weight is made from one by its value's power and its row's, which may be 2^120 apart, and must not be lost before.
+constexpr float ROOM = 24.0f;
 constexpr float NONE = -1.0e30f;        // a maximum of no keys
 enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 503 };
 
@@ -65,8 +66,9 @@ struct Shape {
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
     static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + Q_BUFFERS * (ROWS / R) * Q_BYTES;
     // What a unit's threads tell each other, in floats: minus the sum's reference, the weights' beside it, what raising scales the two by,
-    // what the item's end scales its outputs and the other unit's by [R]; maxima and sums of warps [2][4][R].
-    static constexpr int UNIT_FLOATS = 6 * R + 2 * UNIT_WARPS * R;
+    // what the item's end scales its outputs and the other unit's by, 2^(the second) [R]; maxima and sums of warps [2][4][R].
+    static constexpr int UNIT_FLOATS = 7 * R + 2 * UNIT_WARPS * R;
+    static constexpr float LIMIT = EIGHT ? 256.0f : 0x1p60f;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
     // What the queries' warp tells, of an item's rows: factors, positions, rows of the output (-1: none).
     static constexpr int AT_ROWS = AT_FLOATS + U * UNIT_FLOATS * 4;
@@ -238,6 +240,61 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
     const int runs_a_page = a.page_size >> 4;
     auto page_of = [&](int sixteenth) { return (int)(((uint64_t)(unsigned)sixteenth * a.run_pages) >> 31); };
 
+    // 16 of an item's rows' queries, two lanes a row, and what is to be known of the rows.
+    auto lay_out = [&](int buffer, int row0) {
+        float* info = reinterpret_cast<float*>(smem + S::AT_ROWS) + buffer * 3 * S::ROWS;
+        const int part = lane & 1;
+        const int item_row = row0 + (lane >> 1), row = item_row % R, pair = sg.first + item_row;
+        const bool real = pair < sg.rq.pairs;
+        const int token = real ? pair / ratio : 0, to_row = (sg.rq.start + token) * heads + sg.kv * ratio + (real ? pair - token * ratio : 0);
+        const __nv_bfloat16* src = q + (size_t)to_row * D + part * 64;
+        uint8_t* queries = smem + S::AT_QUERIES + (buffer * (S::ROWS / R) + item_row / R) * S::Q_BYTES;
+        uint4 x[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[n] = real ? reinterpret_cast<const uint4*>(src)[n] : make_uint4(0, 0, 0, 0);
+        float f = scale_log2;
+        if constexpr (EIGHT) {
+            unsigned most = 0;                           // magnitudes of bfloat16 compare as their bits do
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const unsigned v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = max(most, max(v[k] & 0x7FFFu, v[k] >> 16 & 0x7FFFu));
+            }
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            const int e = min(max((int)(most >> 7) - 127, -100), 127);     // the row's largest lies in 2^e .. 2^(e + 1): to 2^7 .. 2^8
+            const float up = __int_as_float((127 + 7 - e) << 23);
+            f = fmaxf(__int_as_float((127 - 7 + e) << 23) * scale_log2, 1.0e-44f);     // (not zero: a masked score stays -inf)
+            const bool bad = most >= 0x7F80u;            // a row with an infinity or a NaN: codes that are NaN
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                uint32_t one[4], two[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint4& from = x[2 * n + (k >> 1)];
+                    const unsigned w0 = k & 1 ? from.z : from.x, w1 = k & 1 ? from.w : from.y;
+                    const float v[4] = {__uint_as_float(w0 << 16) * up, __uint_as_float(w0 & 0xffff0000u) * up, __uint_as_float(w1 << 16) * up,
+                                        __uint_as_float(w1 & 0xffff0000u) * up};
+                    const unsigned c0 = e4m3::pack2(v[0], v[1]), c1 = e4m3::pack2(v[2], v[3]);
+                    const float2 b0 = mma_pages::from_halves(e4m3::halves((unsigned short)c0)), b1 = mma_pages::from_halves(e4m3::halves((unsigned short)c1));
+                    one[k] = bad ? 0x7F7F7F7Fu : c0 | c1 << 16;
+                    two[k] = e4m3::pack2((v[0] - b0.x) * 32.0f, (v[1] - b0.y) * 32.0f) | e4m3::pack2((v[2] - b1.x) * 32.0f, (v[3] - b1.y) * 32.0f) << 16;
+                }
+                const int piece = part * 4 + n, r1 = (row >> 4) * 32 + (row & 15), r2 = r1 + 16;
+                *reinterpret_cast<uint4*>(queries + r1 * 128 + ((piece ^ (r1 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
+                *reinterpret_cast<uint4*>(queries + r2 * 128 + ((piece ^ (r2 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) *reinterpret_cast<uint4*>(queries + part * (R * 128) + row * 128 + ((n ^ (row & 7)) << 4)) = x[n];
+        }
+        if (part == 0) {
+            info[item_row] = f;
+            reinterpret_cast<int*>(info)[S::ROWS + item_row] = real ? sg.rq.history + token : -1;
+            reinterpret_cast<int*>(info)[2 * S::ROWS + item_row] = real ? to_row : -1;
+        }
+    };
+
     if (warp == 0 || warp == LOADER) {
         const int p = lane & 7, plane = (lane >> 3) & 1;          // a run of 16 keys; for exponents, keys' or values'
         uint32_t use = 0;
@@ -299,62 +356,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         uint32_t segment = 0;
         bool ok = true;
         for (; sg.next(a); ++segment) {
+            if (segment == 0) continue;                          // (the softmax warps lay out the first)
             const int buffer = segment % S::Q_BUFFERS;
             ok = tc::mbar_wait_warp(&q_free[buffer], ((segment / S::Q_BUFFERS) & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_PRODUCER);
             if (!ok) break;
-            float* info = reinterpret_cast<float*>(smem + S::AT_ROWS) + buffer * 3 * S::ROWS;
-            const int part = lane & 1;
-            for (int row0 = 0; row0 < S::ROWS; row0 += 16) {
-                const int item_row = row0 + (lane >> 1), row = item_row % R, pair = sg.first + item_row;
-                const bool real = pair < sg.rq.pairs;
-                const int token = real ? pair / ratio : 0, to_row = (sg.rq.start + token) * heads + sg.kv * ratio + (real ? pair - token * ratio : 0);
-                const __nv_bfloat16* src = q + (size_t)to_row * D + part * 64;
-                uint8_t* queries = smem + S::AT_QUERIES + (buffer * (S::ROWS / R) + item_row / R) * S::Q_BYTES;
-                uint4 x[8];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) x[n] = real ? reinterpret_cast<const uint4*>(src)[n] : make_uint4(0, 0, 0, 0);
-                float f = scale_log2;
-                if constexpr (EIGHT) {
-                    unsigned most = 0;                           // magnitudes of bfloat16 compare as their bits do
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const unsigned v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) most = max(most, max(v[k] & 0x7FFFu, v[k] >> 16 & 0x7FFFu));
-                    }
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    const int e = min(max((int)(most >> 7) - 127, -100), 127);     // the row's largest lies in 2^e .. 2^(e + 1): to 2^7 .. 2^8
-                    const float up = __int_as_float((127 + 7 - e) << 23);
-                    f = fmaxf(__int_as_float((127 - 7 + e) << 23) * scale_log2, 1.0e-44f);     // (not zero: a masked score stays -inf)
-                    const bool bad = most >= 0x7F80u;            // a row with an infinity or a NaN: codes that are NaN
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        uint32_t one[4], two[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint4& from = x[2 * n + (k >> 1)];
-                            const unsigned w0 = k & 1 ? from.z : from.x, w1 = k & 1 ? from.w : from.y;
-                            const float v[4] = {__uint_as_float(w0 << 16) * up, __uint_as_float(w0 & 0xffff0000u) * up, __uint_as_float(w1 << 16) * up,
-                                                __uint_as_float(w1 & 0xffff0000u) * up};
-                            const unsigned c0 = e4m3::pack2(v[0], v[1]), c1 = e4m3::pack2(v[2], v[3]);
-                            const float2 b0 = mma_pages::from_halves(e4m3::halves((unsigned short)c0)), b1 = mma_pages::from_halves(e4m3::halves((unsigned short)c1));
-                            one[k] = bad ? 0x7F7F7F7Fu : c0 | c1 << 16;
-                            two[k] = e4m3::pack2((v[0] - b0.x) * 32.0f, (v[1] - b0.y) * 32.0f) | e4m3::pack2((v[2] - b1.x) * 32.0f, (v[3] - b1.y) * 32.0f) << 16;
-                        }
-                        const int piece = part * 4 + n, r1 = (row >> 4) * 32 + (row & 15), r2 = r1 + 16;
-                        *reinterpret_cast<uint4*>(queries + r1 * 128 + ((piece ^ (r1 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
-                        *reinterpret_cast<uint4*>(queries + r2 * 128 + ((piece ^ (r2 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) *reinterpret_cast<uint4*>(queries + part * (R * 128) + row * 128 + ((n ^ (row & 7)) << 4)) = x[n];
-                }
-                if (part == 0) {
-                    info[item_row] = f;
-                    reinterpret_cast<int*>(info)[S::ROWS + item_row] = real ? sg.rq.history + token : -1;
-                    reinterpret_cast<int*>(info)[2 * S::ROWS + item_row] = real ? to_row : -1;
-                }
-            }
+            for (int row0 = 0; row0 < S::ROWS; row0 += 16) lay_out(buffer, row0);
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&q_full[buffer]);
@@ -450,7 +456,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         const uint32_t s_at = tmem + unit * S::U_COLS + lanes, o_at = s_at + 2 * S::S_COLS;
         float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
         float *minus_peak = shared, *shift = shared + R, *fade_sum = shared + 2 * R, *fade_o = shared + 3 * R, *own_scale = shared + 4 * R,
-              *given_scale = shared + 5 * R, *warp_peak = shared + 6 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
+              *given_scale = shared + 5 * R, *power = shared + 6 * R, *warp_peak = shared + 7 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + (S::HALVES ? 0 : unit * S::WEIGHTS)) + key * 128;
@@ -460,6 +466,12 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         for (; sg.next(a); before += sg.tiles, ++segment) {
             const int first = sg.first + (SHARED ? 0 : unit * R), pairs = sg.rq.pairs, history = sg.rq.history, start = sg.rq.start;
             const int q_buffer = segment % S::Q_BUFFERS;
+            if (segment == 0) {
+                if (warp - 2 < S::ROWS / 16) lay_out(0, 16 * (warp - 2));
+                tc::fence_proxy_async();
+                units_barrier();
+                if (warp == 2 && lane == 0) tc::mbar_arrive(&q_full[0]);
+            }
             if (ok) ok = tc::mbar_wait_warp(&q_full[q_buffer], (segment / S::Q_BUFFERS) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
             const float* factor = rows_info + q_buffer * 3 * S::ROWS;
             const int *position = reinterpret_cast<const int*>(factor) + S::ROWS, *out_row = position + S::ROWS;
@@ -492,13 +504,14 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 int runs;
                 asm volatile("ld.shared.s32 %0, [%1];" : "=r"(runs) : "r"(live_at + 4 * stage) : "memory");
                 const bool dead = !(runs >> (key >> 4) & 1);     // a page that is not in the cache: a key of zeros
-                float k_power = 1.0f, v_power = 0.0f;
+                float k_power = 1.0f, v_power = 1.0f, v_exponent = 0.0f;
                 if constexpr (EIGHT) {
                     const uint32_t b = exponents_at + stage * 256 + key;
                     const unsigned kb = shared_byte(b), vb = shared_byte(b + KEYS);
                     // A value that is no number makes its key none: NaN for the rows that see it.
                     k_power = dead ? 0.0f : vb == e4m3::NOT_NUMBERS ? NAN : e4m3::up(kb);
-                    v_power = dead || vb == e4m3::NOT_NUMBERS ? 0.0f : (float)((int)vb - 127);
+                    v_power = dead || vb == e4m3::NOT_NUMBERS ? 1.0f : e4m3::up(vb);
+                    v_exponent = dead || vb == e4m3::NOT_NUMBERS ? 0.0f : (float)((int)vb - 127);
                 }
                 const bool whole = t0 >= all_from && t0 + KEYS <= all_to && runs == 0xff;
                 const bool in_reach = t >= sg.rq.low && t < sg.rq.end;
@@ -567,27 +580,35 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     }
                 };
                 scores(opening);                                 // (the first tile has no references yet)
-                bool raise = opening;
-                if (!opening) {
-                    float over = -INFINITY;
+                // ---- exponentials (in place of what they are of) and weights, two halves (bfloat16 values) to a register
+                uint32_t h[R / 2];
+                auto weights = [&]() -> float {                  // the largest weight
+                    float most = 0.0f;
 #pragma unroll
                     for (int n = 0; n < R; n += 4) {
-                        if constexpr (EIGHT) {
-                            const float4 s = shared4(rows_at + 4 * (R + n));
-                            over = max3(max3(over, x[n], x[n] + (s.x + v_power)), x[n + 1], x[n + 1] + (s.y + v_power));
-                            over = max3(max3(over, x[n + 2], x[n + 2] + (s.z + v_power)), x[n + 3], x[n + 3] + (s.w + v_power));
-                        } else {
-                            over = max3(max3(over, x[n], x[n + 1]), x[n + 2], x[n + 3]);
+                        float w[4];
+                        const float4 s = EIGHT ? shared4(rows_at + 4 * (6 * R + n)) : make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            x[n + k] = exp2_fast(x[n + k]);
+                            w[k] = EIGHT ? x[n + k] * (at4(s, k) * v_power) : x[n + k];
                         }
+                        most = max3(max3(most, w[0], w[1]), w[2], w[3]);
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) h[(n + k) / 2] = EIGHT ? mma_pages::pack_half(w[k], w[k + 1]) : mma_pages::pack_bf16(w[k], w[k + 1]);
                     }
-                    raise = unit_any(unit, over > LIMIT);
+                    return most;
+                };
+                bool raise = opening;
+                if (!opening) {
+                    raise = unit_any(unit, weights() > S::LIMIT);
                     if (raise) scores(true);
                 }
                 if (raise) {
                     // ---- the references rise to this tile's maxima
 #pragma unroll
                     for (int n = 0; n < R; ++n) {
-                        const float p = warp_most(x[n]), w = EIGHT ? warp_most(x[n] + v_power) : p;
+                        const float p = warp_most(x[n]), w = EIGHT ? warp_most(x[n] + v_exponent) : p;
                         if (lane == 0) warp_peak[quarter * R + n] = p, warp_top[quarter * R + n] = w;
                     }
                     unit_barrier(unit);
@@ -596,11 +617,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         float p = NONE, w = NONE;
 #pragma unroll
                         for (int k = 0; k < UNIT_WARPS; ++k) p = fmaxf(p, warp_peak[k * R + n]), w = fmaxf(w, warp_top[k * R + n]);
-                        const float old = opening ? NONE : -minus_peak[n], now = fmaxf(old, EIGHT && p > NONE ? p + ROOM : p);
-                        const float top_old = opening ? NONE : old - shift[n], top_now = EIGHT ? fmaxf(top_old, w > NONE ? w - RAISED : w) : now;
+                        const float old = opening ? NONE : -minus_peak[n], now = fmaxf(old, EIGHT && p > NONE ? p - ROOM : p);
+                        const float top_old = opening ? NONE : old - shift[n], top_now = EIGHT ? fmaxf(top_old, w) : now;
                         fade_sum[n] = exp2_fast(old - now);
                         fade_o[n] = EIGHT ? exp2_fast(top_old - top_now) : fade_sum[n];
-                        minus_peak[n] = -now, shift[n] = now - top_now;
+                        minus_peak[n] = -now, shift[n] = now - top_now, power[n] = exp2_fast(now - top_now);
                     }
                     unit_barrier(unit);
 #pragma unroll
@@ -608,6 +629,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         const float4 mp = shared4(rows_at + 4 * n);
                         x[n] += mp.x, x[n + 1] += mp.y, x[n + 2] += mp.z, x[n + 3] += mp.w;
                     }
+                    weights();
                     if (!opening) {
                         // (Every O^T that has been asked for has been made: the weights' buffer is free.)
 #pragma unroll
@@ -627,41 +649,35 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s_free[2 * unit + s_buffer]);
-                // ---- weights
-                constexpr int SKIP = S::HALVES ? 4 : 0;             // pieces of 16 bytes to the second unit's half
+                // ---- the weights to shared memory
+                constexpr int SKIP = S::HALVES ? 4 : 0;          // pieces of 16 bytes to the second unit's half
+#pragma unroll
+                for (int n = 0; n < R; ++n) sum[n] += x[n];
+                if constexpr (!EIGHT)
+                    if (stray) {
+#pragma unroll
+                        for (int row = 0; row < R; ++row) {
+                            if (hidden >> row & 1u) continue;
+                            for (int d = 0; d < D; ++d) {
+                                const unsigned v = *value_in<S::HALF>(value_row, key, d);
+                                if ((v & 0x7F80u) == 0x7F80u) atomicAdd(strays + row * D + d, x[row] * __uint_as_float(v << 16));
+                            }
+                        }
+                        stray_flag[unit] = 1;
+                    }
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
-                    uint32_t h[8];
-                    float4 s;
-#pragma unroll
-                    for (int n = 0; n < 16; n += 2) {
-                        const int row = 16 * c + n;
-                        const float e0 = exp2_fast(x[row]), e1 = exp2_fast(x[row + 1]);
-                        sum[row] += e0;
-                        sum[row + 1] += e1;
-                        if constexpr (EIGHT) {
-                            if (n % 4 == 0) s = shared4(rows_at + 4 * (R + row));
-                            const float s0 = n % 4 == 0 ? s.x : s.z, s1 = n % 4 == 0 ? s.y : s.w;
-                            h[n >> 1] = mma_pages::pack_half(exp2_fast(x[row] + (s0 + v_power)), exp2_fast(x[row + 1] + (s1 + v_power)));
-                        } else {
-                            h[n >> 1] = mma_pages::pack_bf16(e0, e1);
-                            if (stray)
-                                for (int k = 0; k < 2; ++k) {
-                                    if (hidden >> (row + k) & 1u) continue;
-                                    for (int d = 0; d < D; ++d) {
-                                        const unsigned v = *value_in<S::HALF>(value_row, key, d);
-                                        if ((v & 0x7F80u) == 0x7F80u) atomicAdd(strays + (row + k) * D + d, (k ? e1 : e0) * __uint_as_float(v << 16));
-                                    }
-                                    stray_flag[unit] = 1;
-                                }
-                        }
-                    }
                     if constexpr (EIGHT) {
+                        uint32_t left[8];
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) to_shared4(weights_at + (((SKIP * unit + 3 * c + k) ^ (key & 7)) << 4), take_codes(h, k < 2));
+                        for (int n = 0; n < 8; ++n) left[n] = h[8 * c + n];
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) to_shared4(weights_at + (((SKIP * unit + 3 * c + k) ^ (key & 7)) << 4), take_codes(left, k < 2));
                     } else {
-                        to_shared4(weights_at + (((SKIP * unit + 2 * c) ^ (key & 7)) << 4), make_uint4(h[0], h[1], h[2], h[3]));
-                        to_shared4(weights_at + (((SKIP * unit + 2 * c + 1) ^ (key & 7)) << 4), make_uint4(h[4], h[5], h[6], h[7]));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            to_shared4(weights_at + (((SKIP * unit + 2 * c + k) ^ (key & 7)) << 4),
+                                       make_uint4(h[8 * c + 4 * k], h[8 * c + 4 * k + 1], h[8 * c + 4 * k + 2], h[8 * c + 4 * k + 3]));
                     }
                 }
                 if constexpr (!EIGHT)
@@ -732,11 +748,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 auto total_of = [&](uint32_t sums) {
                     return (shared1(sums + 4 * row) + shared1(sums + 4 * (R + row))) + (shared1(sums + 4 * (2 * R + row)) + shared1(sums + 4 * (3 * R + row)));
                 };
-                float total = total_of(rows_at + 24 * R), peak = -shared1(rows_at + 4 * row), top = peak - shared1(rows_at + 4 * (R + row)), f = 1.0f, g = 0.0f;
+                float total = total_of(rows_at + 28 * R), peak = -shared1(rows_at + 4 * row), top = peak - shared1(rows_at + 4 * (R + row)), f = 1.0f, g = 0.0f;
                 if (both) {
                     const uint32_t theirs = rows_at + S::UNIT_FLOATS * 4;
                     const float peak2 = -shared1(theirs + 4 * row), top2 = peak2 - shared1(theirs + 4 * (R + row)), p = fmaxf(peak, peak2), t = fmaxf(top, top2);
-                    total = fmaf(total, exp2_fast(peak - p), total_of(theirs + 24 * R) * exp2_fast(peak2 - p));
+                    total = fmaf(total, exp2_fast(peak - p), total_of(theirs + 28 * R) * exp2_fast(peak2 - p));
                     f = exp2_fast(top - t), g = exp2_fast(top2 - t);
                     peak = p, top = t;
                 }

@@ -7,8 +7,9 @@ output o = sum w v is off by
     bits, (D + 8) 2^-24 of scale * sum |q k|,
     a weight's rounding to half precision, 2^-11 of it, where queries are bfloat16, 2^-21 (two halves) where they are float32; to
     bfloat16, whose eight bits leave half a step of 2^-8, over a bfloat16 cache and where a request's many rows run the prompt
-    kernel; and, of a weight that is small beside the row's largest, half of 2^-24 of the
-    largest, for each key,
+    kernel; and, of a weight that is small beside the row's largest, half of 2^-24 of the largest, for each key (heads of 128 with
+    bfloat16 queries over eight bits: weights are three codes that add up, the third in steps of 2^-9 / 1024, half of which is
+    2^-20 of the largest),
     the sums over the keys in 32 bits, (keys + 16) 2^-23."""
 import math
 
@@ -225,8 +226,9 @@ class Case:
                 o = w @ v
                 score_error = (self.dim + 8) * 2.0 ** -24 * self.scale * torch.where(ok, x.abs() @ k.abs().T, 0.0).amax(-1, keepdim=True)
                 size = w @ v.abs()
-                # The weights that multiply the values carry the values' powers of two: half of 2^-24 of the largest product, a key.
-                least = 2.0 ** -25 * weight_step / 2.0 ** -11 * (w[:, :, None] * v.abs().amax(-1)[None, :, None]).amax(1) * 2 * ok.sum(-1, keepdim=True)
+                # The weights that multiply the values carry the values' powers of two: it is the largest product that counts.
+                codes = self.store == "e4m3" and self.dim == 128 and self.dtype is BF16 and not prompt
+                least = (2.0 ** -20 if codes else 2.0 ** -24 * min(1.0, weight_step / 2.0 ** -11)) * (w[:, :, None] * v.abs().amax(-1)[None, :, None]).amax(1) * ok.sum(-1, keepdim=True)
                 limit = half_step * o.abs() + size * (2 * score_error + weight_step + (n + h + 16) * 2.0 ** -23) + least + 1e-30
                 mine = got[self.starts[r]:self.starts[r] + n, head * self.dim:(head + 1) * self.dim]
                 bad = ~((mine - o).abs() <= limit)
