@@ -10,10 +10,70 @@ namespace {
 constexpr int WARPS = 4;
 constexpr int MAX_WIDTH = 256;      // values of a row: a lane holds an eighth of 64 of them at most
 
-__device__ __forceinline__ float read1(const float* p) { return *p; }
-__device__ __forceinline__ float read1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+// ---- writing: bound by the bytes of the rows (a code for two or four of them is little) ----
+// 16 bytes of a row a lane: LANES of them are a row, and a warp has EACH * 32 / LANES rows, whose loads are all asked for before the
+// first is used.  Items are (row, plane, head), heads of a row next to one another.
+__device__ __forceinline__ void read16(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+__device__ __forceinline__ void read16(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
 
-// One warp a (row, plane, head).  The row stays in registers between its maximum and its codes.
+template <typename T, int LANES, int EACH>
+__global__ void __launch_bounds__(WARPS * 32)
+quantize_wide_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict__ v, long long v_stride, const int* __restrict__ slots,
+                     uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, int items, int kv_heads, int page_size, long long total_slots) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int VALUES = 16 / sizeof(T), D = LANES * VALUES, ROWS = 32 / LANES;
+    const int lane = threadIdx.x & 31, part = lane % LANES;
+    const int first = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * (ROWS * EACH) + lane / LANES;
+    float x[EACH][VALUES];
+    int slot[EACH], head[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int item = first + e * ROWS, row = item / (2 * kv_heads), rest = item - row * 2 * kv_heads, plane = rest >= kv_heads, g = rest - plane * kv_heads;
+        head[e] = rest;
+        slot[e] = -1;
+        if (item < items) {
+            slot[e] = slots[row];
+            read16((plane ? v + row * v_stride : k + row * k_stride) + g * D + part * VALUES, x[e]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) x[e][i] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        unsigned peak = 0;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) peak = max(peak, __float_as_uint(x[e][i]) & 0x7FFFFFFFu);
+        if constexpr (LANES == 32) peak = __reduce_max_sync(0xffffffffu, peak);
+        else
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+        const unsigned byte = e4m3::exponent_byte(peak);
+        const float f = byte == e4m3::NOT_NUMBERS ? 0.0f : e4m3::down(byte);
+        unsigned w[VALUES / 4];
+#pragma unroll
+        for (int i = 0; i < VALUES / 4; ++i)
+            w[i] = byte == e4m3::NOT_NUMBERS ? 0u : e4m3::pack2(x[e][4 * i] * f, x[e][4 * i + 1] * f) | e4m3::pack2(x[e][4 * i + 2] * f, x[e][4 * i + 3] * f) << 16;
+        if (slot[e] < 0 || slot[e] >= total_slots) continue;
+        const int page = slot[e] / page_size;
+        const size_t at = ((size_t)page * 2 * kv_heads + head[e]) * page_size + (slot[e] - page * page_size);
+        if (part == 0) exponents[at] = (uint8_t)byte;
+        if constexpr (VALUES == 4) *reinterpret_cast<unsigned*>(codes + at * D + 4 * part) = w[0];
+        else *reinterpret_cast<uint2*>(codes + at * D + 8 * part) = make_uint2(w[0], w[1]);
+    }
+}
+
+// Any width, rows that start anywhere: one warp an item, 32 values at a time.  The row stays in registers between its maximum and its
+// codes.
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32)
 quantize_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict__ v, long long v_stride, const int* __restrict__ slots,
@@ -33,7 +93,7 @@ quantize_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict
 #pragma unroll
     for (int i = 0; i < MAX_WIDTH / 32; ++i) {
         const int d = lane + 32 * i;
-        x[i] = d < head_dim ? read1(src + d) : 0.0f;
+        x[i] = d < head_dim ? to_float(src[d]) : 0.0f;
         peak = max(peak, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     }
     const unsigned byte = e4m3::exponent_byte(__reduce_max_sync(0xffffffffu, peak));
@@ -47,7 +107,63 @@ quantize_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict
     }
 }
 
-// One warp a row of a page.
+// ---- reading back: bound by the bytes written ----
+// 16 bytes of the output a thread (8 codes, or 4), four of them 256 pieces apart, whose loads are all asked for before the first is used; a
+// block has up to 1024 pieces of a page.
+__device__ __forceinline__ float code_value(unsigned halves, bool upper) {
+    return __half2float(__ushort_as_half((unsigned short)(upper ? halves >> 16 : halves & 0xffffu)));
+}
+__device__ __forceinline__ uint4 values16(uint2 w, float f, __nv_bfloat16) {
+    unsigned r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned h = e4m3::halves((unsigned short)((i < 2 ? w.x : w.y) >> (16 * (i & 1))));
+        const __nv_bfloat162 b = __floats2bfloat162_rn(code_value(h, false) * f, code_value(h, true) * f);
+        r[i] = *reinterpret_cast<const unsigned*>(&b);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ uint4 values16(uint2 w, float f, float) {
+    const unsigned a = e4m3::halves((unsigned short)w.x), b = e4m3::halves((unsigned short)(w.x >> 16));
+    return make_uint4(__float_as_uint(code_value(a, false) * f), __float_as_uint(code_value(a, true) * f), __float_as_uint(code_value(b, false) * f),
+                      __float_as_uint(code_value(b, true) * f));
+}
+
+constexpr int READERS = 256, PIECES = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(READERS)
+dequantize_wide_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ pages,
+                       const int* __restrict__ used, T* __restrict__ out, int blocks_a_page, int pieces_a_page, int pieces_a_row, int page_size,
+                       int total_pages) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int CODES = 16 / sizeof(T);
+    const int i = blockIdx.x / blocks_a_page, first = (blockIdx.x % blocks_a_page) * (READERS * PIECES) + threadIdx.x;
+    const int page = pages[i], live = page < 0 || page >= total_pages ? 0 : used ? used[i] : page_size;
+    const size_t rows_a_page = pieces_a_page / pieces_a_row;
+    uint2 w[PIECES];
+    float f[PIECES];
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+        const int piece = first + n * READERS, row = piece / pieces_a_row;
+        w[n] = make_uint2(0, 0);
+        f[n] = 0.0f;
+        if (piece < pieces_a_page && row % page_size < live) {
+            const uint8_t* src = codes + ((size_t)page * pieces_a_page + piece) * CODES;
+            if constexpr (CODES == 8) w[n] = *reinterpret_cast<const uint2*>(src);
+            else w[n].x = *reinterpret_cast<const unsigned*>(src);
+            f[n] = e4m3::up(exponents[page * rows_a_page + row]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+        const int piece = first + n * READERS;
+        if (piece < pieces_a_page) reinterpret_cast<uint4*>(out)[(size_t)i * pieces_a_page + piece] = values16(w[n], f[n], T());
+    }
+}
+
+// Any width: one warp a row of a page.
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ pages,
@@ -63,23 +179,21 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     const bool live = page >= 0 && page < total_pages && (!used || place < used[i]);
     const size_t at = ((size_t)max(page, 0) * 2 * kv_heads + head % (2 * kv_heads)) * page_size + place;
     const float f = live ? e4m3::up(exponents[at]) : 0.0f;
-    for (int d = lane; d < head_dim; d += 32) {
-        const unsigned h = live ? e4m3::halves(codes[at * head_dim + d]) : 0u;
-        out[item * head_dim + d] = from_float<T>(__half2float(__ushort_as_half((unsigned short)(h & 0xffffu))) * f);
-    }
+    for (int d = lane; d < head_dim; d += 32)
+        out[item * head_dim + d] = from_float<T>(live ? code_value(e4m3::halves(codes[at * head_dim + d]), false) * f : 0.0f);
 }
 
-constexpr int EXPANDED = 16;         // slots of an expanded page
+constexpr int EXPANDED = 16, ROW_PIECES = 16;         // slots of an expanded page; pieces of eight of a head's 128 values
 
 // Requests' keys and values as bfloat16 pages of 16 slots, for a kernel that reads those: the requests of more than `rows_over` rows, one
 // after another without gaps, a block a page.  `out_table` names a request's pages, `out_count` has its rows (none for the requests
 // that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value.
 // A value row that is no numbers comes as zeros with its key as NaN: the attention's mask then keeps it from the rows that do
 // not see it (a weight of zero would not), and makes NaN of those that do, as it has to.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(READERS)
 expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ row_count,
               const int* __restrict__ history, const int* __restrict__ tables, int table_stride, int requests, int rows_over, int window, int pages,
-              int kv_heads, int head_dim, int page_size, __nv_bfloat16* __restrict__ out, int* __restrict__ out_table, int out_stride,
+              int kv_heads, int page_size, __nv_bfloat16* __restrict__ out, int* __restrict__ out_table, int out_stride,
               int* __restrict__ out_count, int* __restrict__ out_list) {
     pdl_trigger();
     pdl_wait();
@@ -118,40 +232,43 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
     if (r < 0) return;
     if (threadIdx.x == 0) out_table[(size_t)r * out_stride + j] = blockIdx.x;
     const int keys = min(history[r] + row_count[r], table_stride * page_size);
-    const int pieces = head_dim / 16;
+    const int total = 2 * kv_heads * EXPANDED * ROW_PIECES, low = window > 0 ? max(0, history[r] - window + 1) : 0;
     const int* table = tables + (size_t)r * table_stride;
     const size_t plane = (size_t)kv_heads * page_size;
-    for (int x = threadIdx.x; x < 2 * kv_heads * EXPANDED * pieces; x += blockDim.x) {
-        const int piece = x % pieces, slot = x / pieces % EXPANDED, head = x / (pieces * EXPANDED);      // head: plane * kv_heads + g
-        const int t = j * EXPANDED + slot;
-        const int page = t < keys ? table[t / page_size] : -1;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (page >= 0 && page < pages) {
-            const size_t at = ((size_t)page * 2 * kv_heads + head) * page_size + t % page_size;
-            const unsigned byte = exponents[at];
-            const bool key = head < kv_heads;
-            const bool bad = byte == e4m3::NOT_NUMBERS || (key && exponents[at + plane] == e4m3::NOT_NUMBERS);
-            if (bad) {
-                if (key) lo = hi = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u);
-            } else {
-                const uint4 w = *reinterpret_cast<const uint4*>(codes + at * head_dim + piece * 16);
-                const float f = e4m3::up(byte);
-                auto four = [&](unsigned c, unsigned& a, unsigned& b) {
-                    const unsigned h0 = e4m3::halves((unsigned short)(c & 0xffffu)), h1 = e4m3::halves((unsigned short)(c >> 16));
-                    const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                    const __nv_bfloat162 y0 = __floats2bfloat162_rn(x0.x * f, x0.y * f), y1 = __floats2bfloat162_rn(x1.x * f, x1.y * f);
-                    a = *reinterpret_cast<const unsigned*>(&y0);
-                    b = *reinterpret_cast<const unsigned*>(&y1);
-                };
-                four(w.x, lo.x, lo.y);
-                four(w.y, lo.z, lo.w);
-                four(w.z, hi.x, hi.y);
-                four(w.w, hi.z, hi.w);
+    uint4* to = reinterpret_cast<uint4*>(out) + (size_t)blockIdx.x * total;
+    // The run's 16 slots lie in one page where pages are whole 16s.
+    const bool together = page_size % EXPANDED == 0;
+    const int t0 = j * EXPANDED, run_page = together && t0 < keys ? table[t0 / page_size] : -1, run_off = t0 % page_size;
+    // Eight codes a piece; four pieces' loads are asked for before the first is used.
+    for (int x0 = threadIdx.x; x0 < total; x0 += PIECES * READERS) {
+        uint2 w[PIECES];
+        unsigned byte[PIECES], other[PIECES];
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int x = x0 + n * READERS, piece = x % ROW_PIECES, slot = x / ROW_PIECES % EXPANDED, head = x / (ROW_PIECES * EXPANDED);   // plane * kv_heads + g
+            const int t = t0 + slot;
+            const bool wanted = x < total && t >= low && t < keys;
+            const int page = together ? run_page : wanted ? table[t / page_size] : -1, off = together ? run_off + slot : t % page_size;
+            w[n] = make_uint2(0, 0);
+            byte[n] = other[n] = 0;
+            if (wanted && page >= 0 && page < pages) {
+                const size_t at = ((size_t)page * 2 * kv_heads + head) * page_size + off;
+                w[n] = *reinterpret_cast<const uint2*>(codes + at * (8 * ROW_PIECES) + piece * 8);
+                byte[n] = exponents[at];
+                if (head < kv_heads) other[n] = exponents[at + plane];
             }
         }
-        uint4* to = reinterpret_cast<uint4*>(out + (((size_t)blockIdx.x * 2 * kv_heads + head) * EXPANDED + slot) * head_dim + piece * 16);
-        to[0] = lo;
-        to[1] = hi;
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int x = x0 + n * READERS;
+            if (x >= total) continue;
+            uint4 v = values16(w[n], e4m3::up(byte[n]), __nv_bfloat16());
+            if (byte[n] == e4m3::NOT_NUMBERS || other[n] == e4m3::NOT_NUMBERS) {
+                const unsigned nan = x < total / 2 ? 0x7FC07FC0u : 0u;
+                v = make_uint4(nan, nan, nan, nan);
+            }
+            to[x] = v;
+        }
     }
 }
 
@@ -162,9 +279,40 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
 LLMX_EXPORT int llmx_quantize_kv(const void* k, long long k_stride, const void* v, long long v_stride, int dtype, const int* slots, void* codes,
                                  void* exponents, int rows, int kv_heads, int head_dim, int page_size, int pages, cudaStream_t stream) {
     if (rows <= 0) return 0;
+    if (dtype != LLMX_F32 && dtype != LLMX_BF16) return LLMX_ERR_BAD_ARGUMENT;
     if (kv_heads <= 0 || head_dim <= 0 || head_dim > MAX_WIDTH || page_size <= 0 || pages < 0) return LLMX_ERR_UNSUPPORTED;
     const long long items = (long long)rows * 2 * kv_heads, blocks = (items + WARPS - 1) / WARPS;
     if (blocks >= (1ll << 31)) return LLMX_ERR_UNSUPPORTED;
+    // Rows in 16-byte pieces where they lie so and a warp's lanes are whole rows.  Few items: one at a time a warp, so that they find more
+    // of the device's warps (8 rows of 16 heads of 128 float32: 1.7 us either way); many: four, for their loads' latency.
+    const int size = dtype == LLMX_F32 ? 4 : 2, lanes = head_dim * size / 16;
+    const bool wide = head_dim * size % 16 == 0 && (lanes == 8 || lanes == 16 || lanes == 32) && !((k_stride | v_stride) * size % 16) &&
+                      !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)codes) & 15) && items < (1ll << 30);
+    if (wide) {
+        const int each = items * lanes >= 148ll * 32 * 64 ? 4 : 1;
+        const long long per = (long long)WARPS * (32 / lanes) * each;
+#define LLMX_QUANTIZE(T, LANES, EACH)                                                                                                  \
+    launch_kernel(quantize_wide_kernel<T, LANES, EACH>, dim3((unsigned)((items + per - 1) / per)), dim3(WARPS * 32), 0, stream, (const T*)k,  \
+                  k_stride, (const T*)v, v_stride, slots, (uint8_t*)codes, (uint8_t*)exponents, (int)items, kv_heads, page_size,              \
+                  (long long)pages * page_size)
+#define LLMX_QUANTIZE_EACH(T, LANES)                   \
+    do {                                               \
+        if (each == 4) LLMX_QUANTIZE(T, LANES, 4);     \
+        else LLMX_QUANTIZE(T, LANES, 1);               \
+    } while (0)
+        if (dtype == LLMX_F32) {
+            if (lanes == 32) LLMX_QUANTIZE_EACH(float, 32);
+            else if (lanes == 16) LLMX_QUANTIZE_EACH(float, 16);
+            else LLMX_QUANTIZE_EACH(float, 8);
+        } else {
+            if (lanes == 32) LLMX_QUANTIZE_EACH(__nv_bfloat16, 32);
+            else if (lanes == 16) LLMX_QUANTIZE_EACH(__nv_bfloat16, 16);
+            else LLMX_QUANTIZE_EACH(__nv_bfloat16, 8);
+        }
+#undef LLMX_QUANTIZE_EACH
+#undef LLMX_QUANTIZE
+        return launch_status();
+    }
 #define LLMX_QUANTIZE(T)                                                                                                            \
     launch_kernel(quantize_kernel<T>, dim3((unsigned)blocks), dim3(WARPS * 32), 0, stream, (const T*)k, k_stride, (const T*)v, v_stride, slots, \
                   (uint8_t*)codes, (uint8_t*)exponents, rows, kv_heads, head_dim, page_size, (long long)pages * page_size)
@@ -183,6 +331,18 @@ LLMX_EXPORT int llmx_dequantize_pages(const void* codes, const void* exponents, 
     if (kv_heads <= 0 || head_dim <= 0 || page_size <= 0) return LLMX_ERR_UNSUPPORTED;
     const long long rows = (long long)n * 2 * kv_heads * page_size, blocks = (rows + WARPS - 1) / WARPS;
     if (blocks >= (1ll << 31)) return LLMX_ERR_UNSUPPORTED;
+    if (dtype != LLMX_F32 && dtype != LLMX_BF16) return LLMX_ERR_BAD_ARGUMENT;
+    const int per = dtype == LLMX_F32 ? 4 : 8;          // codes for 16 bytes
+    const long long pieces = (long long)2 * kv_heads * page_size * (head_dim / per), blocks_a_page = (pieces + READERS * PIECES - 1) / (READERS * PIECES);
+    if (head_dim % per == 0 && !(((uintptr_t)codes | (uintptr_t)out) & 15) && pieces < (1ll << 30) && n * blocks_a_page < (1ll << 31)) {
+#define LLMX_DEQUANTIZE(T)                                                                                                            \
+    launch_kernel(dequantize_wide_kernel<T>, dim3((unsigned)(n * blocks_a_page)), dim3(READERS), 0, stream, (const uint8_t*)codes,            \
+                  (const uint8_t*)exponents, pages, used, (T*)out, (int)blocks_a_page, (int)pieces, head_dim / per, page_size, total_pages)
+        if (dtype == LLMX_BF16) LLMX_DEQUANTIZE(__nv_bfloat16);
+        else LLMX_DEQUANTIZE(float);
+#undef LLMX_DEQUANTIZE
+        return launch_status();
+    }
 #define LLMX_DEQUANTIZE(T)                                                                                                            \
     launch_kernel(dequantize_kernel<T>, dim3((unsigned)blocks), dim3(WARPS * 32), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, \
                   pages, used, (T*)out, rows, kv_heads, head_dim, page_size, total_pages)
@@ -193,15 +353,15 @@ LLMX_EXPORT int llmx_dequantize_pages(const void* codes, const void* exponents, 
     return launch_status();
 }
 
-// Requests of more than `rows_over` rows, their keys and values as bfloat16 pages out[0 .. capacity) of [2, kv_heads, 16, head_dim]: all of
+// Requests of more than `rows_over` rows, their keys and values as bfloat16 pages out[0 .. capacity) of [2, kv_heads, 16, 128]: all of
 // them, or under a window those from the stage of 128 that the first row's window starts in.  `capacity` pages must hold them.
 LLMX_EXPORT int llmx_expand_requests(const void* codes, const void* exponents, const int* row_count, const int* history, const int* tables,
                                      int table_stride, int requests, int rows_over, int window, int pages, int kv_heads, int head_dim, int page_size,
                                      void* out, int capacity, int* out_table, int out_stride, int* out_count, int* out_list, cudaStream_t stream) {
     if (requests <= 0 || capacity <= 0) return 0;
-    if (kv_heads <= 0 || head_dim <= 0 || head_dim % 16 || page_size <= 0 || (((uintptr_t)codes | (uintptr_t)out) & 15)) return LLMX_ERR_UNSUPPORTED;
-    launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(256), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_count, history,
-                  tables, table_stride, requests, rows_over, window, pages, kv_heads, head_dim, page_size, (__nv_bfloat16*)out, out_table, out_stride,
+    if (kv_heads <= 0 || head_dim != 8 * ROW_PIECES || page_size <= 0 || (((uintptr_t)codes | (uintptr_t)out) & 15)) return LLMX_ERR_UNSUPPORTED;
+    launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(READERS), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_count, history,
+                  tables, table_stride, requests, rows_over, window, pages, kv_heads, page_size, (__nv_bfloat16*)out, out_table, out_stride,
                   out_count, out_list);
     return launch_status();
 }
