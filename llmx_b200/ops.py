@@ -12,6 +12,7 @@ these functions raise.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -1302,11 +1303,13 @@ class QuantizedPages:
     __slots__ = ("codes", "exponents", "pages", "kv_heads", "page_size", "head_dim")
 
     def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
-        _need(codes.dtype is torch.float8_e4m3fn and exponents.dtype is torch.uint8 and codes.dim() == 5 and codes.shape[1] == 2
-              and codes.shape[:4] == exponents.shape and codes.is_contiguous() and exponents.is_contiguous() and codes.device == exponents.device,
-              "quantized pages: codes float8_e4m3fn [pages, 2, kv_heads, page size, head width] and exponents uint8 without the last axis, contiguous")
+        shape = codes.shape
+        if not (codes.dtype is torch.float8_e4m3fn and exponents.dtype is torch.uint8 and len(shape) == 5 and shape[1] == 2
+                and shape[:4] == exponents.shape and codes.is_contiguous() and exponents.is_contiguous() and codes.device == exponents.device):
+            raise KernelError("quantized pages: codes float8_e4m3fn [pages, 2, kv_heads, page size, head width] and exponents uint8 without the "
+                              "last axis, contiguous")
         self.codes, self.exponents = codes, exponents
-        self.pages, _, self.kv_heads, self.page_size, self.head_dim = codes.shape
+        self.pages, _, self.kv_heads, self.page_size, self.head_dim = shape
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device) -> "QuantizedPages":
@@ -1315,50 +1318,64 @@ class QuantizedPages:
                    torch.full((pages, 2, kv_heads, page_size), 127, dtype=torch.uint8, device=device))
 
 
-def _launched(device: torch.device, call):
-    """`call(stream)` with `device` the current one, on its current stream."""
-    _need(device.type == "cuda", "kernel arguments must be CUDA tensors (there is no CPU path)")
-    if device.index == torch.cuda.current_device():
-        return call(_stream())
-    with torch.cuda.device(device):
-        return call(_stream())
+class _on:
+    """The device of a call's tensors as the current one (where it is not), and its current stream."""
+    __slots__ = ("index", "back")
 
+    def __init__(self, what: str, device: torch.device, *tensors: Optional[torch.Tensor]):
+        if device.type != "cuda":
+            raise KernelError("kernel arguments must be CUDA tensors (there is no CPU path)")
+        for t in tensors:
+            if t is not None and t.device != device:
+                raise KernelError(f"{what}: tensors on different devices")
+        self.index, self.back = device.index, -1
 
-def _same_device(what: str, device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    for t in tensors:
-        _need(t is None or t.device == device, f"{what}: tensors on different devices")
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.index:
+            self.back = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+        return runtime.current_stream()
+
+    def __exit__(self, *exc) -> None:
+        if self.back >= 0:
+            torch.cuda.set_device(self.back)
 
 
 def quantize_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: QuantizedPages) -> None:
     """Row r of keys and values goes to slot slots[r] (page * page size + place) of a cache in eight bits; k, v float32 or bfloat16
     [rows, kv_heads, head_dim], each row contiguous and rows at any distance (columns of a product's output); slots int32
     [rows], each named once, negative ones (and ones beyond the cache) not kept."""
-    _need(k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype and tuple(k.shape[1:]) == (cache.kv_heads, cache.head_dim),
-          "quantize_kv: keys and values [rows, kv_heads, head_dim] of one type and of the cache's heads")
-    rows, heads, dim = k.shape
-    for t in (k, v):
-        _need(rows == 0 or ((dim == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == dim)), "quantize_kv: a row's heads must lie one after another")
-    _need(slots.dtype is torch.int32 and slots.numel() == rows and slots.is_contiguous(), "quantize_kv: an int32 slot per row")
+    shape = k.shape
+    if not (len(shape) == 3 and v.shape == shape and v.dtype is k.dtype and shape[1] == cache.kv_heads and shape[2] == cache.head_dim):
+        raise KernelError("quantize_kv: keys and values [rows, kv_heads, head_dim] of one type and of the cache's heads")
+    rows, heads, dim = shape
+    ks, vs = k.stride(), v.stride()
+    if rows and (dim > 1 and (ks[2] != 1 or vs[2] != 1) or heads > 1 and (ks[1] != dim or vs[1] != dim)):
+        raise KernelError("quantize_kv: a row's heads must lie one after another")
+    if slots.dtype is not torch.int32 or slots.numel() != rows or not slots.is_contiguous():
+        raise KernelError("quantize_kv: an int32 slot per row")
     _need(dim <= 256, "quantize_kv: heads of 256 values at most")
-    code = _code(k)
-    _same_device("quantize_kv", k.device, v, slots, cache.codes)
-    _check(_launched(k.device, lambda stream: _fn("cache_e4m3", "llmx_quantize_kv")(
-        _ptr(k), k.stride(0), _ptr(v), v.stride(0), code, _ptr(slots), _ptr(cache.codes), _ptr(cache.exponents), rows, heads, dim, cache.page_size,
-        cache.pages, stream)), "quantize_kv")
+    code, codes = _code(k), cache.codes
+    with _on("quantize_kv", k.device, v, slots, codes) as stream:
+        _check(_fn("cache_e4m3", "llmx_quantize_kv")(
+            k.data_ptr(), ks[0], v.data_ptr(), vs[0], code, slots.data_ptr(), codes.data_ptr(), cache.exponents.data_ptr(), rows, heads, dim,
+            cache.page_size, cache.pages, stream), "quantize_kv")
 
 
 def dequantize_pages(cache: QuantizedPages, pages: torch.Tensor, out: torch.Tensor, used: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[i] = page pages[i] of a cache in eight bits; out float32 or bfloat16 [n, 2, kv_heads, page_size, head_dim], pages int32 [n].
     `used` int32 [n]: how many of each page's slots hold tokens; the others (and pages outside of the cache) come as zeros."""
-    n = pages.numel()
-    _need(pages.dtype is torch.int32 and pages.is_contiguous() and tuple(out.shape) == (n, *cache.codes.shape[1:]) and out.is_contiguous(),
-          "dequantize_pages: int32 page ids and an output [ids, 2, kv_heads, page size, head width], contiguous")
-    _need(used is None or (used.dtype is torch.int32 and used.numel() == n and used.is_contiguous()), "dequantize_pages: an int32 count per page id")
+    n, codes = pages.numel(), cache.codes
+    if not (pages.dtype is torch.int32 and pages.is_contiguous() and out.dim() == 5 and out.shape[0] == n and out.shape[1:] == codes.shape[1:]
+            and out.is_contiguous()):
+        raise KernelError("dequantize_pages: int32 page ids and an output [ids, 2, kv_heads, page size, head width], contiguous")
+    if used is not None and not (used.dtype is torch.int32 and used.numel() == n and used.is_contiguous()):
+        raise KernelError("dequantize_pages: an int32 count per page id")
     code = _code(out)
-    _same_device("dequantize_pages", out.device, pages, used, cache.codes)
-    _check(_launched(out.device, lambda stream: _fn("cache_e4m3", "llmx_dequantize_pages")(
-        _ptr(cache.codes), _ptr(cache.exponents), _ptr(pages), _ptr(used), _ptr(out), code, n, cache.kv_heads, cache.head_dim, cache.page_size, cache.pages,
-        stream)), "dequantize_pages")
+    with _on("dequantize_pages", out.device, pages, used, codes) as stream:
+        _check(_fn("cache_e4m3", "llmx_dequantize_pages")(
+            codes.data_ptr(), cache.exponents.data_ptr(), pages.data_ptr(), None if used is None else used.data_ptr(), out.data_ptr(), code, n,
+            cache.kv_heads, cache.head_dim, cache.page_size, cache.pages, stream), "dequantize_pages")
     return out
 
 
@@ -1379,43 +1396,55 @@ def tree_bits(parents: Sequence[Sequence[int]]) -> np.ndarray:
     return bits.view(np.int32)
 
 
+_CALL = struct.Struct("@9P8iq6if1PN2P")       # llmx_pages_call (csrc/runtime/llmx_runtime.h)
+_pages_rooms = {}                             # what the sizes of calls ask for as a workspace
+
+
 def _attention_pages(what: str, q, cache, out, row_start, row_count, history, block_tables, tree, heads, kv_heads, head_dim, window, scale, max_rows,
                      max_context):
-    eight = isinstance(cache, QuantizedPages)
+    eight = type(cache) is QuantizedPages
     stored = cache.codes if eight else cache
-    rows, requests = q.shape[0], row_start.numel()
-    _need(q.dim() == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and q.shape[1] == heads * head_dim and out.shape == q.shape
-          and out.dtype == q.dtype and q.is_contiguous() and out.is_contiguous(), f"{what}: q and out [rows, heads * head_dim] of one type, contiguous")
-    _need(stored.dim() == 5 and stored.shape[1] == 2 and stored.shape[2] == kv_heads and stored.shape[4] == head_dim and stored.is_contiguous(),
-          f"{what}: a cache [pages, 2, kv_heads, page size, head_dim]")
-    _need(head_dim <= 256, f"{what}: heads of 256 values at most")
+    shape, at = q.shape, stored.shape
+    rows, requests, dtype = shape[0], row_start.numel(), q.dtype
+    if not (len(shape) == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and shape[1] == heads * head_dim and out.shape == shape
+            and out.dtype is dtype and q.is_contiguous() and out.is_contiguous()):
+        raise KernelError(f"{what}: q and out [rows, heads * head_dim] of one type, contiguous")
+    if not (len(at) == 5 and at[1] == 2 and at[2] == kv_heads and at[4] == head_dim and (eight or stored.is_contiguous())):
+        raise KernelError(f"{what}: a cache [pages, 2, kv_heads, page size, head_dim]")
+    _need(head_dim <= 256, "attention over pages: heads of 256 values at most")
     for t in (row_start, row_count, history):
-        _need(t.dtype is torch.int32 and t.numel() == requests and t.is_contiguous(), f"{what}: int32 first rows, row counts and histories, one per request")
-    _need(block_tables.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests and block_tables.is_contiguous(),
-          f"{what}: int32 block tables [requests, pages]")
-    _need(tree is None or (tree.dtype is torch.int32 and tree.dim() == 2 and tree.shape[0] == rows and tree.is_contiguous()),
-          f"{what}: int32 words of bits, [rows, words]")
-    _need(max_rows >= 0 and max_context >= 0 and (window is None or window > 0) and scale > 0,
-          f"{what}: bounds of at least 0, a window of at least 1, a scale above 0")
-    q_code, code = _code(q), E4M3 if eight else _code(stored)
-    _same_device(what, q.device, out, stored, row_start, row_count, history, block_tables, tree)
-    call = runtime.PagesCall(q.data_ptr(), out.data_ptr(), stored.data_ptr(), cache.exponents.data_ptr() if eight else None, row_start.data_ptr(),
-                             row_count.data_ptr(), history.data_ptr(), block_tables.data_ptr(), None if tree is None else tree.data_ptr(), q_code, code,
-                             block_tables.shape[1], 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), int(max_context), 0,
-                             stored.shape[0], heads, kv_heads, head_dim, stored.shape[3], int(window or 0), float(scale))
-    _launched(q.device, lambda stream: _pages_attention(what, call, q.device, stream))
+        if t.dtype is not torch.int32 or t.numel() != requests or not t.is_contiguous():
+            raise KernelError(f"{what}: int32 first rows, row counts and histories, one per request")
+    if not (block_tables.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests and block_tables.is_contiguous()):
+        raise KernelError(f"{what}: int32 block tables [requests, pages]")
+    if tree is not None and not (tree.dtype is torch.int32 and tree.dim() == 2 and tree.shape[0] == rows and tree.is_contiguous()):
+        raise KernelError(f"{what}: int32 words of bits, [rows, words]")
+    if not (0 <= max_rows < 2 ** 31 and 0 <= max_context < 2 ** 31 and (window is None or 0 < window < 2 ** 31) and scale > 0):
+        raise KernelError(f"{what}: bounds of at least 0, a window of at least 1, a scale above 0")
+    q_code, code, device = _code(q), E4M3 if eight else _code(stored), q.device
+    sizes = (q_code, code, block_tables.shape[1], 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), int(max_context), 0, at[0], heads,
+             kv_heads, head_dim, at[3], int(window or 0))
+    with _on(what, device, out, stored, row_start, row_count, history, block_tables, tree) as stream:
+        error_word = runtime.error_word(device).data_ptr()
+        pointers = (q.data_ptr(), out.data_ptr(), stored.data_ptr(), cache.exponents.data_ptr() if eight else 0, row_start.data_ptr(),
+                    row_count.data_ptr(), history.data_ptr(), block_tables.data_ptr(), 0 if tree is None else tree.data_ptr())
+        lib = runtime.lib()
+        # The form, and with it the workspace, goes by sizes and by whether rows are read in 16-byte pieces.
+        key = (sizes, tree is None, (pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15)
+        room = _pages_rooms.get(key)
+        if room is None:
+            call = _CALL.pack(*pointers, *sizes, scale, 0, 0, error_word, stream)
+            room = lib.llmx_pages_workspace(call)
+            if runtime.bind_missing():
+                room = lib.llmx_pages_workspace(call)
+            if len(_pages_rooms) > 4096:
+                _pages_rooms.clear()
+            _pages_rooms[key] = room
+        workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+        call = _CALL.pack(*pointers, *sizes, scale, 0 if workspace is None else workspace.data_ptr(), room, error_word, stream)
+        if lib.llmx_pages_attention(call):
+            raise KernelError(f"{what}: {runtime.last_error()}")
     return out
-
-
-def _pages_attention(what: str, call, device: torch.device, stream) -> None:
-    lib = runtime.lib()
-    room = lib.llmx_pages_workspace(call)
-    if runtime.bind_missing():
-        room = lib.llmx_pages_workspace(call)
-    workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    call.workspace, call.workspace_bytes = None if workspace is None else workspace.data_ptr(), room
-    call.error_word, call.stream = runtime.error_word(device).data_ptr(), stream
-    runtime.check(lib.llmx_pages_attention(call), what)
 
 
 def attention_quantized(q: torch.Tensor, cache: QuantizedPages, out: torch.Tensor, row_start: torch.Tensor, row_count: torch.Tensor,

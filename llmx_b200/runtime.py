@@ -63,15 +63,7 @@ class LayerStepStruct(ctypes.Structure):
     _fields_ = [("block", _i), ("cache_entry", _i), ("write_cache", _i)]
 
 
-class PagesCall(ctypes.Structure):
-    _fields_ = [("q", _p), ("out", _p), ("cache", _p), ("exponents", _p), ("row_start", _p), ("row_count", _p), ("history", _p), ("tables", _p),
-                ("tree", _p), ("q_dtype", _i), ("cache_dtype", _i), ("table_stride", _i), ("tree_words", _i), ("requests", _i), ("total_rows", _i),
-                ("max_rows", _i), ("max_context", _i), ("total_context", _ll), ("pages", _i), ("heads", _i), ("kv_heads", _i), ("head_dim", _i),
-                ("page_size", _i), ("window", _i), ("scale", _f), ("workspace", _p), ("workspace_bytes", _sz), ("error_word", _p), ("stream", _p)]
-
-
 _SP = ctypes.POINTER(StepStruct)
-_PCP = ctypes.POINTER(PagesCall)
 _SIGNATURES = {
     "llmx_rt_version": (_i, []),
     "llmx_rt_bind": (_i, [ctypes.c_char_p, _p]),
@@ -128,8 +120,8 @@ _SIGNATURES = {
     "llmx_paged_attention": (_i, [_SP, _p, _i, _i, _p, _i, _i, _i, _i, _f]),
     "llmx_paged_attention_workspace": (_sz, [_SP, _i, _i, _i, _i, _i]),
     "llmx_decode_from_qkv": (_i, [_SP, _p, _i, _p, _p, _f, _p, _p, _i, _p, _i, _i, _i, _i, _f]),
-    "llmx_pages_attention": (_i, [_PCP]),
-    "llmx_pages_workspace": (_sz, [_PCP]),
+    "llmx_pages_attention": (_i, [ctypes.c_char_p]),
+    "llmx_pages_workspace": (_sz, [ctypes.c_char_p]),
     "llmx_model_create": (_p, [_p, _p, _i, _p, _i, _p, _i, _i]),
     "llmx_model_destroy": (None, [_p]),
     "llmx_model_workspace": (_sz, [_p, _SP]),
@@ -252,7 +244,7 @@ _ERROR_NAMES = {101: "the TMA producer waited for a free stage", 102: "the MMA i
 
 def error_word(device) -> torch.Tensor:
     """The device int a kernel records a failed (bounded) wait in, one per device."""
-    idx = torch.device(device).index or 0
+    idx = (device if isinstance(device, torch.device) else torch.device(device)).index or 0
     w = _error_words.get(idx)
     if w is None:
         w = _error_words[idx] = torch.zeros(1, dtype=torch.int32, device=device)
