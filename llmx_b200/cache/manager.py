@@ -96,6 +96,7 @@ class CacheGroup:
         self.page_size = page_size
         self.pool = PagePool(num_pages)
         self.storage = None               # torch tensor [len(members), num_pages, 2, G, page, D] once allocated
+        self.exponents = None             # in eight bits: [len(members), num_pages, 2, G, page]
 
     def bytes_per_page(self, element_size: int) -> int:
         return len(self.members) * self.spec.planes * self.spec.kv_heads * self.page_size * self.spec.head_dim * element_size
@@ -231,6 +232,14 @@ class CacheManager:
         import torch
         for g in self.groups:
             s = g.spec
+            if self.kv_dtype is torch.float8_e4m3fn:
+                if s.planes != 2:
+                    raise ValueError("a cache in eight bits holds keys and values in planes of their own")
+                # Codes and exponents (ops.QuantizedPages), rows of zeros: 127 is an exponent of nought.
+                shape = (len(g.members), g.pool.num_pages, 2, s.kv_heads, g.page_size)
+                g.storage = torch.zeros((*shape, s.head_dim), dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
+                g.exponents = torch.full(shape, 127, dtype=torch.uint8, device=self.device)
+                continue
             # Zero-filled: a kernel may load (and mask) slots of a page that were never written.
             g.storage = torch.zeros((len(g.members), g.pool.num_pages, s.planes, s.kv_heads, g.page_size, s.head_dim),
                                     dtype=self.kv_dtype, device=self.device)
@@ -295,13 +304,19 @@ class CacheManager:
         for g in self.groups:
             if g.storage is not None:
                 total += g.storage.numel() * g.storage.element_size()
+            if g.exponents is not None:
+                total += g.exponents.numel()
         return total
 
     def entry_storage(self, entry: int):
-        """(group index, this entry's [num_pages, 2, G, page, D] storage) or the state tensor."""
+        """(group index, this entry's [num_pages, 2, G, page, D] storage, in eight bits its `ops.QuantizedPages`) or the state tensor."""
         if entry in self.group_of_entry:
             gi, mi = self.group_of_entry[entry]
-            return gi, self.groups[gi].storage[mi]
+            g = self.groups[gi]
+            if g.exponents is not None:
+                from ..ops import QuantizedPages
+                return gi, QuantizedPages(g.storage[mi], g.exponents[mi])
+            return gi, g.storage[mi]
         return -1, self.state_storage[entry]
 
     def check(self) -> None:

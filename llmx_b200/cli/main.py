@@ -82,16 +82,16 @@ def _dtype(value: str) -> str:
 
 def _cache_type(given) -> Optional[str]:
     """The cache's element type from --cache-type-k / --cache-type-v (the reference's flags, src/cli/main.cpp:2018-2038),
-    or None for the path's own.  Keys and values lie in one storage here, so the two must agree; bf16 and f32 are
-    what the kernels take (the reference's f16 default has no kernel in this engine and is refused by name)."""
+    or None for the path's own.  Keys and values lie in one storage here, so the two must agree; bf16, f32 and f8 (e4m3 with an
+    exponent a row) are what the kernels take (the reference's f16 default has no kernel in this engine and is refused by name)."""
     k, v = given.get("--cache-type-k"), given.get("--cache-type-v")
     for f, t in (("--cache-type-k", k), ("--cache-type-v", v)):
-        if t is not None and t not in ("bf16", "f32"):
-            raise UsageError(f"{f} {t}: the cache is bf16 or f32 here (no kernel reads a cache of another type)")
+        if t is not None and t not in ("bf16", "f32", "f8"):
+            raise UsageError(f"{f} {t}: the cache is bf16, f32 or f8 here (no kernel reads a cache of another type)")
     if k is not None and v is not None and k != v:
         raise UsageError("--cache-type-k and --cache-type-v must agree: keys and values share their pages here")
     t = k if k is not None else v
-    return None if t is None else {"bf16": "bfloat16", "f32": "float32"}[t]
+    return None if t is None else {"bf16": "bfloat16", "f32": "float32", "f8": "float8_e4m3"}[t]
 
 
 def _yarn(given: Dict[str, str]) -> Tuple[Optional[float], Optional[int]]:

@@ -136,8 +136,9 @@ struct FewPlan {
 };
 
 FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads, int head_dim, int page_size,
-                 int window) {
+                 int window, int general) {
     FewPlan p;
+    if (general) return p;
     const bool types = cache_dtype == LLMX_E4M3 || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
@@ -206,21 +207,21 @@ int tensor_rows(const FewPlan& p, const void* q, const void* cache, const void* 
 
 // The bytes that `workspace` needs.
 LLMX_EXPORT int llmx_attention_pages_workspace(int q_dtype, int cache_dtype, int requests, int max_rows, int max_context, int heads, int kv_heads,
-                                               int head_dim, int page_size, int window, long long* bytes) {
+                                               int head_dim, int page_size, int window, int general, long long* bytes) {
     *bytes = 0;
     if (requests <= 0 || max_rows <= 0 || kv_heads <= 0 || page_size <= 0) return 0;
-    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
+    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window, general);
     if (p.rows) *bytes = p.bytes(head_dim);
     return 0;
 }
 
 // q/out [total_rows, heads, head_dim] of `q_dtype`; the cache [pages, 2, kv_heads, page_size, head_dim] of `cache_dtype`, with `exponents`
 // [pages, 2, kv_heads, page_size] where that is LLMX_E4M3.  Requests of more than `max_rows` rows are left out; none has more than
-// `max_context` keys (which only chooses the form).  Rows that no request names are left as they are.
+// `max_context` keys.  `general`: the general form, whose sums do not depend on what a row is batched with.  Rows that no request names are left as they are.
 LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cache, const void* exponents, int cache_dtype, void* out,
                                      const int* row_start, const int* row_count, const int* history, const int* tables, int table_stride,
                                      const void* tree, int tree_words, int requests, int total_rows, int max_rows, int max_context, int pages,
-                                     int heads, int kv_heads, int head_dim, int page_size, int window, float scale, void* workspace,
+                                     int heads, int kv_heads, int head_dim, int page_size, int window, int general, float scale, void* workspace,
                                      long long workspace_bytes, int* error_word, cudaStream_t stream) {
     if (requests <= 0 || total_rows <= 0 || max_rows <= 0) return 0;
     if (head_dim <= 0 || head_dim > 32 * MAX_PER_LANE || kv_heads <= 0 || heads % kv_heads || heads > 65535 || requests > 65535 || page_size <= 0)
@@ -228,7 +229,7 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
     Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words,
                     ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), 0, max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
-    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window);
+    const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window, general);
     a.max_tiles = p.max_tiles;
     if (p.rows && pages > 0 && (long long)total_rows * heads < (1ll << 31) && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&
         (long long)pages * 2 * kv_heads * page_size < (1ll << 31)) {

@@ -107,6 +107,159 @@ quantize_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict
     }
 }
 
+// ---- writing a step's rows as the q/k/v product leaves them: per-head norm, rotation, queries out, keys and values into their slots ----
+// The arithmetic of head_norm_rope_kernel (rowwise.cu), operation for operation, with a head's row in registers at its end, where it is
+// given its exponent.  One warp a (row, head): a query head, or a key head with its value.
+struct HeadsIn {
+    const float* qkv;                 // [rows, stride]: q heads, then k heads at k_offset, v heads at v_offset
+    int stride, k_offset, v_offset;
+    const float* q_weight;            // [head_dim] or null
+    const float* k_weight;
+    float eps;
+    const float* cos_table;           // [positions, rot_half] or null
+    const float* sin_table;
+    int rot_half;
+    const int* positions;
+    const int* slots;
+    int rows, heads, kv_heads, head_dim, page_size;
+    long long total_slots;
+};
+__device__ __forceinline__ void write4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void write4(__nv_bfloat16* p, float4 v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+
+template <typename QT>
+__global__ void __launch_bounds__(WARPS * 32)
+head_norm_rope_kernel(HeadsIn a, QT* __restrict__ q_out, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float smem[WARPS][MAX_WIDTH];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_row = a.heads + a.kv_heads, D = a.head_dim;
+    const long long item = (long long)blockIdx.x * WARPS + warp;
+    if (item >= (long long)a.rows * per_row) return;
+    const int row = (int)(item / per_row), j = (int)(item % per_row);
+    const bool is_q = j < a.heads;
+    const int g = is_q ? 0 : j - a.heads;
+    const int slot = is_q ? 0 : a.slots[row];
+    if (slot < 0 || (!is_q && slot >= a.total_slots)) return;
+    float* buf = smem[warp];
+    const float* src = a.qkv + (size_t)row * a.stride + (is_q ? j * D : a.k_offset + g * D);
+    const float* weight = is_q ? a.q_weight : a.k_weight;
+    float s = 0.0f;
+    for (int d = lane; d < D; d += 32) {
+        const float v = src[d];
+        buf[d] = v;
+        s = fmaf(v, v, s);
+    }
+    if (weight) {
+        s = warp_sum(s);
+        const float rr = 1.0f / sqrtf(s / (float)D + a.eps);
+        __syncwarp();
+        for (int d = lane; d < D; d += 32) buf[d] = buf[d] * (rr * weight[d]);
+    }
+    __syncwarp();
+    const float* cs = a.cos_table ? a.cos_table + (size_t)a.positions[row] * a.rot_half : nullptr;
+    const float* sn = a.cos_table ? a.sin_table + (size_t)a.positions[row] * a.rot_half : nullptr;
+    float x[MAX_WIDTH / 32];
+#pragma unroll
+    for (int i = 0; i < MAX_WIDTH / 32; ++i) {
+        const int d = lane + 32 * i;
+        x[i] = 0.0f;
+        if (d >= D) continue;
+        if (cs && d < 2 * a.rot_half) {
+            const int p = d < a.rot_half ? d : d - a.rot_half;
+            const float u = buf[p], v = buf[p + a.rot_half];
+            x[i] = d < a.rot_half ? fmaf(-v, sn[p], u * cs[p]) : fmaf(u, sn[p], v * cs[p]);
+        } else {
+            x[i] = buf[d];
+        }
+        if (is_q) q_out[(size_t)row * a.heads * D + j * D + d] = from_float<QT>(x[i]);
+    }
+    if (is_q) return;
+    const float* value = a.qkv + (size_t)row * a.stride + a.v_offset + g * D;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+        unsigned peak = 0;
+#pragma unroll
+        for (int i = 0; i < MAX_WIDTH / 32; ++i) {
+            if (plane) x[i] = lane + 32 * i < D ? value[lane + 32 * i] : 0.0f;
+            peak = max(peak, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        }
+        const unsigned byte = e4m3::exponent_byte(__reduce_max_sync(0xffffffffu, peak));
+        const size_t at = (((size_t)(slot / a.page_size) * 2 + plane) * a.kv_heads + g) * a.page_size + slot % a.page_size;
+        if (lane == 0) exponents[at] = (uint8_t)byte;
+        const float f = e4m3::down(byte);
+#pragma unroll
+        for (int i = 0; i < MAX_WIDTH / 32; ++i)
+            if (lane + 32 * i < D) codes[at * D + lane + 32 * i] = byte == e4m3::NOT_NUMBERS ? 0 : (uint8_t)e4m3::pack2(x[i] * f, 0.0f);
+    }
+}
+
+// Heads of 128 rotated whole or not at all: four values a lane, a pair's partner 16 lanes away (head_norm_rope_128_kernel's arithmetic).
+template <typename QT>
+__global__ void __launch_bounds__(WARPS * 32)
+head_norm_rope_128_kernel(HeadsIn a, QT* __restrict__ q_out, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int D = 128;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_row = a.heads + a.kv_heads;
+    const unsigned item = blockIdx.x * WARPS + warp;
+    if (item >= (unsigned)a.rows * (unsigned)per_row) return;
+    const int row = (int)(item / (unsigned)per_row), j = (int)(item - (unsigned)row * (unsigned)per_row);
+    const bool is_q = j < a.heads;
+    const int g = is_q ? 0 : j - a.heads;
+    const int slot = is_q ? 0 : a.slots[row];
+    if (slot < 0 || (!is_q && slot >= a.total_slots)) return;
+    const float* row_src = a.qkv + (size_t)row * a.stride;
+    float4 x = reinterpret_cast<const float4*>(row_src + (is_q ? j * D : a.k_offset + g * D))[lane], value = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!is_q) value = reinterpret_cast<const float4*>(row_src + a.v_offset + g * D)[lane];
+    float4 c, sn;
+    if (a.cos_table) {
+        const size_t base = (size_t)a.positions[row] * 64 + 4 * (lane & 15);
+        c = *reinterpret_cast<const float4*>(a.cos_table + base);
+        sn = *reinterpret_cast<const float4*>(a.sin_table + base);
+    }
+    const float* weight = is_q ? a.q_weight : a.k_weight;
+    if (weight) {
+        float s = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, x.w * x.w)));
+        s = warp_sum(s);
+        const float rr = 1.0f / sqrtf(s / (float)D + a.eps);
+        const float4 w4 = reinterpret_cast<const float4*>(weight)[lane];
+        x.x *= rr * w4.x; x.y *= rr * w4.y; x.z *= rr * w4.z; x.w *= rr * w4.w;
+    }
+    if (a.cos_table) {
+        float4 o;
+        o.x = __shfl_xor_sync(0xffffffffu, x.x, 16); o.y = __shfl_xor_sync(0xffffffffu, x.y, 16);
+        o.z = __shfl_xor_sync(0xffffffffu, x.z, 16); o.w = __shfl_xor_sync(0xffffffffu, x.w, 16);
+        if (lane < 16) {
+            x.x = fmaf(-o.x, sn.x, x.x * c.x); x.y = fmaf(-o.y, sn.y, x.y * c.y);
+            x.z = fmaf(-o.z, sn.z, x.z * c.z); x.w = fmaf(-o.w, sn.w, x.w * c.w);
+        } else {
+            x.x = fmaf(o.x, sn.x, x.x * c.x); x.y = fmaf(o.y, sn.y, x.y * c.y);
+            x.z = fmaf(o.z, sn.z, x.z * c.z); x.w = fmaf(o.w, sn.w, x.w * c.w);
+        }
+    }
+    if (is_q) {
+        write4(q_out + ((size_t)row * a.heads + j) * D + 4 * lane, x);
+        return;
+    }
+    const int page = slot / a.page_size;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+        const float4 y = plane ? value : x;
+        const unsigned peak = max(max(__float_as_uint(y.x) & 0x7FFFFFFFu, __float_as_uint(y.y) & 0x7FFFFFFFu),
+                                  max(__float_as_uint(y.z) & 0x7FFFFFFFu, __float_as_uint(y.w) & 0x7FFFFFFFu));
+        const unsigned byte = e4m3::exponent_byte(__reduce_max_sync(0xffffffffu, peak));
+        const float f = e4m3::down(byte);
+        const size_t at = (((size_t)page * 2 + plane) * a.kv_heads + g) * a.page_size + (slot - page * a.page_size);
+        if (lane == 0) exponents[at] = (uint8_t)byte;
+        reinterpret_cast<unsigned*>(codes + at * D)[lane] =
+            byte == e4m3::NOT_NUMBERS ? 0u : e4m3::pack2(y.x * f, y.y * f) | e4m3::pack2(y.z * f, y.w * f) << 16;
+    }
+}
+
 // ---- reading back: bound by the bytes written ----
 // 16 bytes of the output a thread (8 codes, or 4), four of them 256 pieces apart, whose loads are all asked for before the first is used; a
 // block has up to 1024 pieces of a page.
@@ -363,5 +516,32 @@ LLMX_EXPORT int llmx_expand_requests(const void* codes, const void* exponents, c
     launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(READERS), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_count, history,
                   tables, table_stride, requests, rows_over, window, pages, kv_heads, page_size, (__nv_bfloat16*)out, out_table, out_stride,
                   out_count, out_list);
+    return launch_status();
+}
+
+// Per-head norm, rotation, queries out and keys and values into their slots, as llmx_head_norm_rope_kv (rowwise.cu) for a cache in eight bits.
+LLMX_EXPORT int llmx_head_norm_rope_e4m3(const float* qkv, int qkv_stride, int k_offset, int v_offset, const float* q_weight, const float* k_weight,
+                                         float eps, const float* cos_table, const float* sin_table, int rot_half, const int* positions,
+                                         const int* slots, void* q_out, int q_dtype, void* codes, void* exponents, long long pages, int rows, int heads,
+                                         int kv_heads, int head_dim, int page_size, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (head_dim <= 0 || rot_half < 0 || 2 * rot_half > head_dim || page_size <= 0 || (q_dtype != LLMX_F32 && q_dtype != LLMX_BF16)) return LLMX_ERR_BAD_ARGUMENT;
+    const long long blocks = ((long long)rows * (heads + kv_heads) + WARPS - 1) / WARPS;
+    if (head_dim > MAX_WIDTH || blocks >= (1ll << 29)) return LLMX_ERR_UNSUPPORTED;
+    const HeadsIn a = {qkv, qkv_stride, k_offset, v_offset, q_weight, k_weight, eps, cos_table, sin_table, rot_half, positions, slots,
+                       rows, heads, kv_heads, head_dim, page_size, pages * page_size};
+    const bool fast = head_dim == 128 && (!cos_table || rot_half == 64) && !((qkv_stride | k_offset | v_offset) % 4) &&
+                      !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)codes | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
+                         (uintptr_t)sin_table) & 15);
+#define LLMX_HEADS(KERNEL, QT) \
+    launch_kernel(KERNEL<QT>, dim3((unsigned)blocks), dim3(WARPS * 32), 0, stream, a, (QT*)q_out, (uint8_t*)codes, (uint8_t*)exponents)
+    if (q_dtype == LLMX_BF16) {
+        if (fast) LLMX_HEADS(head_norm_rope_128_kernel, __nv_bfloat16);
+        else LLMX_HEADS(head_norm_rope_kernel, __nv_bfloat16);
+    } else {
+        if (fast) LLMX_HEADS(head_norm_rope_128_kernel, float);
+        else LLMX_HEADS(head_norm_rope_kernel, float);
+    }
+#undef LLMX_HEADS
     return launch_status();
 }

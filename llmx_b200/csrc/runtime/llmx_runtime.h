@@ -82,6 +82,9 @@ void llmx_caches_destroy(llmx_caches*);
 // A key/value entry: storage [pages, 2, kv_heads, page_size, head_dim] of `dtype`, in cache group `group`.
 int llmx_caches_set_kv(llmx_caches*, int entry, int group, void* storage, int dtype, long long pages, int kv_heads,
                        int page_size, int head_dim);
+// The same in eight bits: codes [pages, 2, kv_heads, page_size, head_dim] and exponents [pages, 2, kv_heads, page_size] (e4m3.cuh).
+int llmx_caches_set_kv_e4m3(llmx_caches*, int entry, int group, void* codes, void* exponents, long long pages, int kv_heads, int page_size,
+                            int head_dim);
 // A state entry: `slots` tensors of `bytes_per_slot` bytes each.
 int llmx_caches_set_state(llmx_caches*, int entry, void* storage, long long slots, long long bytes_per_slot);
 
@@ -224,6 +227,7 @@ typedef struct llmx_pages_call {
     int max_rows, max_context;        // the most rows a request brings, the most keys one has
     long long total_context;          // the most keys of all requests together (0: requests * max_context)
     int pages, heads, kv_heads, head_dim, page_size, window;
+    int general;                      // the form whose sums do not depend on what a row is batched with, whatever the sizes
     float scale;
     void* workspace;                  // llmx_pages_workspace bytes, 256-byte aligned
     size_t workspace_bytes;

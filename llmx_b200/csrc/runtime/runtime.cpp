@@ -45,8 +45,10 @@ typedef cudaStream_t S;
     X(llmx_attention_plain, (const void*, int, const void*, int, void*, const int*, const int*, const int*, int, int,     \
                              int, int, int, int, int, float, S))                                                          \
     X(llmx_attention_pages, (const void*, int, const void*, const void*, int, void*, const int*, const int*, const int*, const int*,  \
-                             int, const void*, int, int, int, int, int, int, int, int, int, int, int, float, void*, long long, int*, S)) \
-    X(llmx_attention_pages_workspace, (int, int, int, int, int, int, int, int, int, int, long long*))                         \
+                             int, const void*, int, int, int, int, int, int, int, int, int, int, int, int, float, void*, long long, int*, S)) \
+    X(llmx_attention_pages_workspace, (int, int, int, int, int, int, int, int, int, int, int, long long*))                         \
+    X(llmx_head_norm_rope_e4m3, (const float*, int, int, int, const float*, const float*, float, const float*, const float*,      \
+                                 int, const int*, const int*, void*, int, void*, void*, long long, int, int, int, int, int, S))   \
     X(llmx_expand_requests, (const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, int, int,    \
                              void*, int, int*, int, int*, int*, S))                                                       \
     X(llmx_gemm_tc_weight_map, (void*, const void*, int, int))                                                            \
@@ -441,15 +443,16 @@ int pages_attention(Ctx& c, const llmx_pages_call& p) {
         }
         long long room = 0;
         kern.llmx_attention_pages_workspace(p.q_dtype, p.cache_dtype, p.requests, max_rows, p.max_context, p.heads, p.kv_heads, p.head_dim, p.page_size,
-                                            p.window, &room);
+                                            p.window, p.general, &room);
+        if (((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.cache | (uintptr_t)p.exponents) & 15) room = 0;      // (the general form)
         void* at = room ? c.alloc((size_t)room) : nullptr;
         CALL(c, llmx_attention_pages, room ? 2 : 1, p.q, p.q_dtype, p.cache, p.exponents, p.cache_dtype, p.out, p.row_start, p.row_count, p.history,
              p.tables, p.table_stride, p.tree, p.tree_words, p.requests, p.total_rows, max_rows, p.max_context, p.pages, p.heads, p.kv_heads,
-             p.head_dim, p.page_size, p.window, p.scale, at, room, p.error_word, c.stream);
+             p.head_dim, p.page_size, p.window, p.general, p.scale, at, room, p.error_word, c.stream);
     };
     // Many rows: their keys and values become bfloat16 once (exact), and the prompt kernel runs over them.  Its tiles of 128 pairs are
     // half empty below FEW_PAIRS.
-    const bool many = p.cache_dtype == LLMX_DT_E4M3 && p.q_dtype == LLMX_DT_BF16 && !p.tree && (long long)p.max_rows * ratio > FEW_PAIRS &&
+    const bool many = p.cache_dtype == LLMX_DT_E4M3 && p.q_dtype == LLMX_DT_BF16 && !p.tree && !p.general && (long long)p.max_rows * ratio > FEW_PAIRS &&
                       tensor_core_prefill(p.heads, p.kv_heads, p.head_dim, ATTN_PAGE) &&
                       !(((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.cache) & 15);
     if (!many) {
@@ -494,6 +497,7 @@ struct CacheEntry {
     int kind = 0;          // 0 none, 1 keys and values, 2 state
     int group = 0, dtype = 0, kv_heads = 0, page_size = 0, head_dim = 0;
     void* storage = nullptr;
+    void* exponents = nullptr;      // beside codes (LLMX_DT_E4M3)
     long long pages = 0, slots = 0, bytes_per_slot = 0;
     alignas(64) mutable unsigned char map[128];         // the decode / warp-level prefill kernels' TMA descriptor
     alignas(64) mutable unsigned char half_map[128];    // the tcgen05 prefill kernel's
@@ -516,6 +520,7 @@ struct AttnPlan {
     std::vector<int> order;            // requests: those with few rows first, then the others
     int n_small = 0, n_large = 0, rows_small = 0, rows_large = 0;
     int ctx_small = 0, ctx_large = 0;
+    long long all_large = 0;           // keys of the requests with more rows, together
     int splits = 1, chunk = 64;        // key ranges of the split-KV kernel
     bool chunk_on_device = false;      // a recorded step: the keys per range are read from the plan's ints
     int tiles = 2, psplits = 1;        // item shape of the tcgen05 prefill kernel
@@ -748,6 +753,22 @@ struct Attention : Mixer {
     int attend(Ctx& c, const void* q, const CacheEntry& e, void* out, int rows, int group) {
         const llmx_step& s = *c.s;
         const int* tables = c.meta(s.block_tables[group]);
+        if (e.dtype == LLMX_DT_E4M3) {
+            const AttnPlan* p = plan_of(c);
+            llmx_pages_call call = {};
+            call.q = q, call.out = out, call.cache = e.storage, call.exponents = e.exponents, call.row_start = c.meta(s.row_start),
+            call.row_count = c.meta(s.row_count), call.history = c.meta(s.history), call.tables = tables, call.q_dtype = qkv.dtype,
+            call.cache_dtype = e.dtype, call.table_stride = s.table_stride[group], call.requests = s.requests, call.total_rows = rows;
+            // Bounds: of a recorded step its room, else what the block tables hold; the rows that the requests leave one another.
+            call.max_rows = p ? std::max(p->rows_small, p->rows_large) : rows - s.requests + 1;
+            call.max_context = s.room > 0 ? s.room : s.table_stride[group] * e.page_size;
+            call.total_context = p ? p->all_large : 0;
+            call.pages = (int)e.pages, call.heads = d.heads, call.kv_heads = d.kv_heads, call.head_dim = d.head_dim, call.page_size = e.page_size,
+            call.window = d.window, call.scale = d.scale, call.error_word = s.error_word;
+            // (The 32-bit path's attention goes by sizes alone, as that over any other cache does.)
+            call.general = invariant() || qkv.dtype == LLMX_DT_F32;
+            return pages_attention(c, call);
+        }
         if (!tiled(e))
             return CALL(c, llmx_attention_plain, 1, q, qkv.dtype, (const void*)e.storage, e.dtype, out, c.meta(s.row_request),
                         c.meta(s.positions) + (size_t)d.position_stream * s.rows, tables, s.table_stride[group], rows, d.heads,
@@ -823,9 +844,14 @@ struct Attention : Mixer {
         if (!from_qkv(c, qkv_out, e, o_buf, rows, slots, g)) {
             if (c.status) return c.status;
             void* q = c.alloc((size_t)rows * q_width * elem(act));
-            CALL(c, llmx_head_norm_rope_kv, 1, (const float*)qkv_out, qkv.N, q_width, q_width + kv_width, d.q_norm, d.k_norm,
-                 d.qk_norm_eps, d.cos, d.sin, d.cos ? d.rot_half : 0, positions, slots, q, act, (void*)e.storage, e.dtype, rows, d.heads,
-                 d.kv_heads, d.head_dim, e.page_size, c.stream);
+            if (e.dtype == LLMX_DT_E4M3)
+                CALL(c, llmx_head_norm_rope_e4m3, 1, (const float*)qkv_out, qkv.N, q_width, q_width + kv_width, d.q_norm, d.k_norm, d.qk_norm_eps,
+                     d.cos, d.sin, d.cos ? d.rot_half : 0, positions, slots, q, act, e.storage, e.exponents, e.pages, rows, d.heads, d.kv_heads,
+                     d.head_dim, e.page_size, c.stream);
+            else
+                CALL(c, llmx_head_norm_rope_kv, 1, (const float*)qkv_out, qkv.N, q_width, q_width + kv_width, d.q_norm, d.k_norm,
+                     d.qk_norm_eps, d.cos, d.sin, d.cos ? d.rot_half : 0, positions, slots, q, act, (void*)e.storage, e.dtype, rows, d.heads,
+                     d.kv_heads, d.head_dim, e.page_size, c.stream);
             attend(c, q, e, o_buf, rows, g);
         }
         return o.forward(c, o_buf, rows, residual, true, false);
@@ -1120,6 +1146,17 @@ LLMX_API int llmx_caches_set_kv(llmx_caches* c, int entry, int group, void* stor
     e.head_dim = head_dim;
     return 0;
 }
+LLMX_API int llmx_caches_set_kv_e4m3(llmx_caches* c, int entry, int group, void* codes, void* exponents, long long pages, int kv_heads,
+                                     int page_size, int head_dim) {
+    if (!c || entry < 0 || entry >= (int)c->entries.size() || group < 0 || group >= LLMX_MAX_GROUPS || !codes || !exponents || pages < 0 ||
+        pages >= (1ll << 31) || kv_heads <= 0 || page_size <= 0 || head_dim <= 0)
+        return fail(LLMX_RT_ERR_BAD_ARGUMENT, "llmx_caches_set_kv_e4m3: bad entry, group, storage or geometry");
+    CacheEntry& e = c->entries[entry];
+    e = CacheEntry();
+    e.kind = 1, e.group = group, e.storage = codes, e.exponents = exponents, e.dtype = LLMX_DT_E4M3, e.pages = pages, e.kv_heads = kv_heads,
+    e.page_size = page_size, e.head_dim = head_dim;
+    return 0;
+}
 LLMX_API int llmx_caches_set_state(llmx_caches* c, int entry, void* storage, long long slots, long long bytes_per_slot) {
     if (!c || entry < 0 || entry >= (int)c->entries.size() || !storage || slots < 0 || bytes_per_slot < 0)
         return fail(LLMX_RT_ERR_BAD_ARGUMENT, "llmx_caches_set_state: bad entry or storage");
@@ -1137,6 +1174,7 @@ void plan_attention(llmx_plan& plan, AttnPlan& a, const int* histories) {
     a.max_rows = std::max(16 / ratio, 1);
     a.order.clear();
     a.n_small = a.n_large = a.rows_small = a.rows_large = a.ctx_small = a.ctx_large = 0;
+    a.all_large = 0;
     for (int r = 0; r < n; ++r)
         if (plan.counts[r] <= a.max_rows) a.order.push_back(r);
     a.n_small = (int)a.order.size();
@@ -1150,7 +1188,7 @@ void plan_attention(llmx_plan& plan, AttnPlan& a, const int* histories) {
         // of speed only: the prefill kernels take any history under any item shape) is the context it was made at.
         const int likely = plan.room > 0 && plan.typical_context > 0 ? std::max(std::min(plan.typical_context, plan.room), c) : ctx;
         if (c <= a.max_rows) a.rows_small = std::max(a.rows_small, c), a.ctx_small = std::max(a.ctx_small, ctx);
-        else a.rows_large = std::max(a.rows_large, c), a.ctx_large = std::max(a.ctx_large, likely);
+        else a.rows_large = std::max(a.rows_large, c), a.ctx_large = std::max(a.ctx_large, likely), a.all_large += ctx;
     }
     a.chunk_on_device = plan.room > 0;
     if (a.n_small) decode_schedule(a.n_small, a.key.kv_heads, a.ctx_small, a.key.head_dim, nullptr, &a.splits, &a.chunk);

@@ -48,11 +48,12 @@ class StepEntry:
 @dataclass
 class EngineOptions:
     dtype: str = "bfloat16"
-    kv_dtype: Optional[str] = None   # the cache's element type, "bfloat16" or "float32" (default: the path's).  The
+    kv_dtype: Optional[str] = None   # the cache's element type, "bfloat16", "float32" or "float8_e4m3" (default: the path's).  The
     #                                  reference's cache types are its own options too (ModelOptions.kv_k / kv_v,
     #                                  src/model/runtime.hpp:80-84): bfloat16 products over a float32 cache separate the
     #                                  products' rounding from the cache's; a cache the tiled kernels do not take
-    #                                  (anything but bfloat16) runs the plain attention kernel
+    #                                  (float32) runs the plain attention kernel.  "float8_e4m3": eight bits and an
+    #                                  exponent a row (ops.QuantizedPages), for models whose mixers all are `Attention`
     kv_tokens: int = 8192            # tokens the cache pool is made for
     window_kv_tokens: Optional[int] = None   # ... the pools of layer groups that keep only a window (default: as many)
     page_size: int = 16
@@ -77,6 +78,24 @@ def _scaled(config, options: "EngineOptions"):
     return config.with_yarn(options.yarn, options.yarn_original_ctx)
 
 
+EIGHT_BITS = ("float8_e4m3", "e4m3", "f8")      # names of the cache's type of eight bits
+
+
+def _need_eight_bits(model, specs) -> None:
+    """Refuses a cache in eight bits for a model with mixers that do not read one."""
+    from ..cache.manager import KVSpec
+
+    def mixers(part):
+        below = [m for c in part.children().values() for m in mixers(c)]
+        return below or ([part] if getattr(part, "cache_spec", None) is not None and part.cache_spec() is not None else [])
+    others = sorted({type(m).__name__ for b in model.blocks for m in mixers(b) if not m.eight_bit_cache})
+    if model.embedding_entry is not None:
+        others.append(type(model.embedding).__name__)
+    if others or not any(isinstance(s, KVSpec) for s in specs):
+        raise StepError("a cache in eight bits holds the keys and values of attention mixers alone"
+                        + (f"; this model has {', '.join(others)}" if others else ""))
+
+
 ROOM_STEP = 2048           # a recording's room for context is a multiple of this
 
 
@@ -98,8 +117,12 @@ class Engine:
         if model.precision is None or model.precision.act is not self.precision.act:
             raise ValueError("the model was not loaded in the engine's dtype")
         self.max_positions = model.max_positions
-        kv_dtype = Precision.of(options.kv_dtype).act if options.kv_dtype else self.precision.act
         specs = model.cache_entry_specs()
+        if options.kv_dtype in EIGHT_BITS:
+            kv_dtype = torch.float8_e4m3fn
+            _need_eight_bits(model, specs)
+        else:
+            kv_dtype = Precision.of(options.kv_dtype).act if options.kv_dtype else self.precision.act
         self.cache = CacheManager(specs, options.page_size, options.kv_tokens, options.max_requests, kv_dtype=kv_dtype,
                                   device=self.device, window_kv_tokens=options.window_kv_tokens)
         # Position tables reach as far as a request can: the pool's size where every request's keys all lie in it,

@@ -50,7 +50,7 @@ class LLM:
     reserve:          "full" or "prompt" (see llmx_b200.engine.scheduler)
     yarn, yarn_original_ctx:  the rope scaled by YaRN at this factor over this trained length (the reference's
                       --yarn and --yarn-original-ctx); the context becomes factor x length
-    kv_dtype:         the cache's element type when it is not the path's ("bfloat16" or "float32"; the reference's
+    kv_dtype:         the cache's element type when it is not the path's ("bfloat16", "float32" or "float8_e4m3"; the reference's
                       --cache-type-k / --cache-type-v)
     invariant:        schedules chosen by sizes alone, so that a request's reply does not depend on what it was
                       batched with, bit for bit (slower; see parts.base.Precision)
@@ -82,10 +82,11 @@ class LLM:
         entry, config = config_from_dir(model_dir)
         model = entry.build(config)
         per_token = 0
-        width = 2 if dtype in ("bfloat16", "bf16") else 4
+        from .engine import EIGHT_BITS
+        width = 1 if dtype in EIGHT_BITS else 2 if dtype in ("bfloat16", "bf16") else 4
         for spec in model.cache_entry_specs():
             if hasattr(spec, "kv_heads"):
-                per_token += getattr(spec, "planes", 2) * spec.kv_heads * spec.head_dim * width
+                per_token += getattr(spec, "planes", 2) * spec.kv_heads * (spec.head_dim * width + (width == 1))
         free, _ = torch.cuda.mem_get_info(torch.device(device))
         by_memory = (free // 3) // max(per_token, 1)
         tokens = int(min(model.max_positions, by_memory))

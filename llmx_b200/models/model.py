@@ -278,8 +278,7 @@ class Model:
         if self.native is not None:
             rt = runtime.lib()
             probe = step.struct_for(self)
-            need = rt.llmx_model_workspace(self.native, ctypes.byref(probe))
-            runtime.bind_missing()
+            need = runtime.sized(lambda: rt.llmx_model_workspace(self.native, ctypes.byref(probe)))
             s = step.struct_for(self, need)
             logits = torch.empty((wanted, self.vocab_size), dtype=torch.float32, device=step.token_ids.device) if wanted else None
             runtime.check(rt.llmx_model_forward(self.native, ctypes.byref(s), runtime.ptr(logits)), "forward")

@@ -155,6 +155,7 @@ _SIGNATURES = {
                                                  _i, _p, _p],
     ("latent_prompt_tc", "llmx_latent_prompt"): [_p, _i, _p, _i, _p, _p, _i, _p, _i, _i, _f, _p, _i, _i, _i, _i, _i, _f, _p, _p],
     ("cache_e4m3", "llmx_quantize_kv"): [_p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    ("cache_e4m3", "llmx_head_norm_rope_e4m3"): [_p, _i, _i, _i, _p, _p, _f, _p, _p, _i, _p, _p, _p, _i, _p, _p, ctypes.c_longlong, _i, _i, _i, _i, _i, _p],
     ("cache_e4m3", "llmx_dequantize_pages"): [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
     ("gemm_plain", "llmx_gemm_plain"): [_p, _i, _p, _i, _p, _i, _i, _i, _i, _p],
     ("attention_plain", "llmx_attention_plain"): [_p, _i, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _p],
@@ -294,14 +295,16 @@ def rmsnorm_pair(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, eps: float
 def head_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
                       q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
                       cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
-                      slots: torch.Tensor, q_out: torch.Tensor, cache: torch.Tensor) -> None:
+                      slots: torch.Tensor, q_out: torch.Tensor, cache) -> None:
     """Per-head norm, rotation and the cache write for one layer.
 
     qkv float32 [rows, (heads + 2 kv_heads) * head_dim] (queries, keys, values);
-    q_out [rows, heads * head_dim]; cache [pages, 2, kv_heads, page_size, head_dim];
+    q_out [rows, heads * head_dim]; cache [pages, 2, kv_heads, page_size, head_dim], or `QuantizedPages` of those sizes;
     cos/sin float32 [positions, rot_half] or None (no rotation); slots int32 [rows],
     negative to skip a row's cache write.
     """
+    eight = isinstance(cache, QuantizedPages)
+    quantized, cache = (cache, cache.codes) if eight else (None, cache)
     _cuda(qkv, q_weight, k_weight, cos, sin, positions, slots, q_out, cache)
     rows = qkv.shape[0]
     q_w, kv_w = heads * head_dim, kv_heads * head_dim
@@ -320,6 +323,13 @@ def head_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: in
     for w in (q_weight, k_weight):
         _need(w is None or (w.dtype == torch.float32 and w.numel() == head_dim), "head_norm_rope_kv: norm weight")
     page_size = cache.shape[3]
+    if eight:
+        _need(head_dim <= 256, "head_norm_rope_kv: heads of 256 values at most in eight bits")
+        _check(_fn("cache_e4m3", "llmx_head_norm_rope_e4m3")(
+            _ptr(qkv), qkv.shape[1], q_w, q_w + kv_w, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rot_half, _ptr(positions),
+            _ptr(slots), _ptr(q_out), _code(q_out), _ptr(cache), _ptr(quantized.exponents), cache.shape[0], rows, heads, kv_heads, head_dim,
+            page_size, _stream()), "head_norm_rope_kv")
+        return
     _check(_fn("rowwise", "llmx_head_norm_rope_kv")(
         _ptr(qkv), qkv.shape[1], q_w, q_w + kv_w, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
         rot_half, _ptr(positions), _ptr(slots), _ptr(q_out), _code(q_out), _ptr(cache), _code(cache), rows, heads,
@@ -1396,7 +1406,7 @@ def tree_bits(parents: Sequence[Sequence[int]]) -> np.ndarray:
     return bits.view(np.int32)
 
 
-_CALL = struct.Struct("@9P8iq6if1PN2P")       # llmx_pages_call (csrc/runtime/llmx_runtime.h)
+_CALL = struct.Struct("@9P8iq7if1PN2P")       # llmx_pages_call (csrc/runtime/llmx_runtime.h)
 _pages_rooms = {}                             # what the sizes of calls ask for as a workspace
 
 
@@ -1423,7 +1433,7 @@ def _attention_pages(what: str, q, cache, out, row_start, row_count, history, bl
         raise KernelError(f"{what}: bounds of at least 0, a window of at least 1, a scale above 0")
     q_code, code, device = _code(q), E4M3 if eight else _code(stored), q.device
     sizes = (q_code, code, block_tables.shape[1], 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), int(max_context), 0, at[0], heads,
-             kv_heads, head_dim, at[3], int(window or 0))
+             kv_heads, head_dim, at[3], int(window or 0), 0)
     with _on(what, device, out, stored, row_start, row_count, history, block_tables, tree) as stream:
         error_word = runtime.error_word(device).data_ptr()
         pointers = (q.data_ptr(), out.data_ptr(), stored.data_ptr(), cache.exponents.data_ptr() if eight else 0, row_start.data_ptr(),
@@ -1434,9 +1444,7 @@ def _attention_pages(what: str, q, cache, out, row_start, row_count, history, bl
         room = _pages_rooms.get(key)
         if room is None:
             call = _CALL.pack(*pointers, *sizes, scale, 0, 0, error_word, stream)
-            room = lib.llmx_pages_workspace(call)
-            if runtime.bind_missing():
-                room = lib.llmx_pages_workspace(call)
+            room = runtime.sized(lambda: lib.llmx_pages_workspace(call))
             if len(_pages_rooms) > 4096:
                 _pages_rooms.clear()
             _pages_rooms[key] = room

@@ -78,7 +78,7 @@ def cache_map(cache: torch.Tensor) -> CacheMap:
 class OneEntryCache:
     """A cache of one key/value entry, as the runtime wants to see it (for tests that bring their own storage)."""
 
-    def __init__(self, storage: torch.Tensor):
+    def __init__(self, storage):          # a tensor [pages, 2, kv_heads, page_size, head_dim], or ops.QuantizedPages
         self.storage = storage
         self.views = runtime.CacheViews(1)
         self.views.set_kv(0, 0, storage)
@@ -102,8 +102,7 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, step, cache_entry: int, 
     _need(q.shape == out.shape and q.shape[1] == heads * head_dim and q.dtype == out.dtype, "attention: q and out shapes do not fit")
     rt = runtime.lib()
     probe = _struct(step, cache)
-    need = rt.llmx_paged_attention_workspace(ctypes.byref(probe), cache_entry, heads, kv_heads, head_dim, int(window or 0))
-    runtime.bind_missing()
+    need = runtime.sized(lambda: rt.llmx_paged_attention_workspace(ctypes.byref(probe), cache_entry, heads, kv_heads, head_dim, int(window or 0)))
     s = _struct(step, cache, need)
     runtime.check(rt.llmx_paged_attention(ctypes.byref(s), q.data_ptr(), runtime.code(q.dtype), cache_entry, out.data_ptr(),
                                           heads, kv_heads, head_dim, int(window or 0), float(scale)), "attention")
@@ -123,8 +122,7 @@ def decode_from_qkv(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k_weigh
           "attention: the product's output and the attention output do not fit the head counts")
     rt = runtime.lib()
     probe = _struct(step, cache)
-    need = rt.llmx_paged_attention_workspace(ctypes.byref(probe), cache_entry, heads, kv_heads, head_dim, int(window or 0))
-    runtime.bind_missing()
+    need = runtime.sized(lambda: rt.llmx_paged_attention_workspace(ctypes.byref(probe), cache_entry, heads, kv_heads, head_dim, int(window or 0)))
     s = _struct(step, cache, need)
     status = rt.llmx_decode_from_qkv(ctypes.byref(s), qkv.data_ptr(), cache_entry, runtime.ptr(q_weight), runtime.ptr(k_weight),
                                      float(eps), runtime.ptr(cos), runtime.ptr(sin), 0 if cos is None else cos.shape[1],

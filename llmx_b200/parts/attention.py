@@ -58,6 +58,8 @@ class AttentionShape(Part):
 
 
 class Attention(Part):
+    eight_bit_cache = True
+
     def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, position_encoding: Part,
                  qk_norm_eps: Optional[float] = None, window: Optional[int] = None,
                  scale: Optional[float] = None, position_stream: int = 0):

@@ -120,6 +120,7 @@ class Part:
     """
     recordable = True
     position_streams = 1
+    eight_bit_cache = False      # whether a mixer's keys and values may lie in eight bits (ops.QuantizedPages)
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         return {}
@@ -238,7 +239,7 @@ class StepBatch:
     _keep: List[Any] = field(default_factory=list)
 
     def kv(self, cache_entry: int):
-        """(group view, this entry's storage [pages, 2, G, page, D])."""
+        """(group view, this entry's storage [pages, 2, G, page, D], or in eight bits its `ops.QuantizedPages`)."""
         gi, storage = self.caches.entry_storage(cache_entry)
         return self.groups[gi], storage
 

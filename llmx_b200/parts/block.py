@@ -65,8 +65,7 @@ class PreNormBlock(Part):
         if self.native is not None:
             rt = runtime.lib()
             probe = step.struct_for(self)
-            need = rt.llmx_part_workspace(self.native, ctypes.byref(probe), rows, -1 if cache_entry is None else int(cache_entry))
-            runtime.bind_missing()
+            need = runtime.sized(lambda: rt.llmx_part_workspace(self.native, ctypes.byref(probe), rows, -1 if cache_entry is None else int(cache_entry)))
             s = step.struct_for(self, need)
             runtime.check(rt.llmx_block_forward(self.native, ctypes.byref(s), x.data_ptr(), rows,
                                                 -1 if cache_entry is None else int(cache_entry), 1 if write_cache else 0), "block")

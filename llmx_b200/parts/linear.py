@@ -35,8 +35,7 @@ def call_struct(step, part, device, workspace_of):
     for (the dry run that sizes it also names the kernel libraries still to be bound).  `step` may be None for a part
     that needs no cache and no plan.  Returns (struct, what must stay alive until the call is enqueued)."""
     probe = step.struct_for(part) if step is not None else bare_step(device)
-    need = int(workspace_of(probe))
-    runtime.bind_missing()
+    need = runtime.sized(lambda: workspace_of(probe))
     if step is not None:
         return step.struct_for(part, need), None
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=device)

@@ -85,6 +85,7 @@ _SIGNATURES = {
     "llmx_caches_create": (_p, [_i]),
     "llmx_caches_destroy": (None, [_p]),
     "llmx_caches_set_kv": (_i, [_p, _i, _i, _p, _i, _ll, _i, _i, _i]),
+    "llmx_caches_set_kv_e4m3": (_i, [_p, _i, _i, _p, _p, _ll, _i, _i, _i]),
     "llmx_caches_set_state": (_i, [_p, _i, _p, _ll, _ll]),
     "llmx_plan_make": (_p, [_p, _p, _i, _p, _p, _i, _i, _i]),
     "llmx_plan_ints": (_i, [_p]),
@@ -141,7 +142,7 @@ KERNEL_LIBS: Dict[str, str] = {
     "llmx_attn_prefill_tc_cache_map": "attention_prefill_tc", "llmx_attn_prefill_tc": "attention_prefill_tc",
     "llmx_attn_prefill": "attention_prefill",
     "llmx_attention_pages": "attention_pages", "llmx_attention_pages_workspace": "attention_pages",
-    "llmx_expand_requests": "cache_e4m3",
+    "llmx_expand_requests": "cache_e4m3", "llmx_head_norm_rope_e4m3": "cache_e4m3",
     "llmx_sample": "sampling", "llmx_penalize": "sampling",
 }
 
@@ -196,6 +197,13 @@ def bind_missing() -> bool:
     if names:
         rt.llmx_rt_reset_caches()
     return bool(names)
+
+
+def sized(workspace_of) -> int:
+    """`workspace_of()`, a dry run's workspace, with every entry point that it would call bound (one that says how much another
+    needs says so only once it is)."""
+    need = workspace_of()
+    return int(workspace_of() if bind_missing() else need)
 
 
 def fail_call(name: Optional[str], nth: int = 1) -> None:
@@ -358,7 +366,13 @@ class CacheViews:
         self.handle = lib().llmx_caches_create(entries)
         self._keep: List[torch.Tensor] = []
 
-    def set_kv(self, entry: int, group: int, storage: torch.Tensor) -> None:
+    def set_kv(self, entry: int, group: int, storage) -> None:
+        if hasattr(storage, "exponents"):          # ops.QuantizedPages
+            pages, _, kv_heads, page_size, head_dim = storage.codes.shape
+            check(lib().llmx_caches_set_kv_e4m3(self.handle, entry, group, storage.codes.data_ptr(), storage.exponents.data_ptr(), pages, kv_heads,
+                                                page_size, head_dim), "cache entry")
+            self._keep += [storage.codes, storage.exponents]
+            return
         pages, _, kv_heads, page_size, head_dim = storage.shape
         check(lib().llmx_caches_set_kv(self.handle, entry, group, storage.data_ptr(), code(storage.dtype), pages, kv_heads,
                                        page_size, head_dim), "cache entry")

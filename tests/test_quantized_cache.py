@@ -136,3 +136,32 @@ def test_tree_bits_name_a_token_and_what_it_continues():
 def test_tree_bits_refuse_what_no_tree_is(parents):
     with pytest.raises(KernelError, match="no earlier token"):
         ops.tree_bits(parents)
+
+
+def test_a_cache_of_one_plane_is_refused_eight_bits():
+    from llmx_b200.cache.manager import CacheManager, KVSpec
+    with pytest.raises(ValueError, match="planes of their own"):
+        CacheManager([KVSpec(2, 64, planes=1)], 16, 64, 2, kv_dtype=torch.float8_e4m3fn, device="cpu")
+
+
+def test_the_managers_eight_bits():
+    from llmx_b200.cache.manager import CacheManager, KVSpec
+    m = CacheManager([KVSpec(2, 64), KVSpec(2, 64), KVSpec(2, 64, window=32)], 16, 64, 2, kv_dtype=torch.float8_e4m3fn, device="cpu")
+    gi, entry = m.entry_storage(1)
+    assert isinstance(entry, ops.QuantizedPages) and gi == 0 and (entry.pages, entry.kv_heads, entry.page_size, entry.head_dim) == (4, 2, 16, 64)
+    assert m.storage_bytes() == 3 * 4 * 2 * 2 * 16 * 65
+
+
+def test_models_with_other_mixers_are_refused_eight_bits():
+    from configs import TINY_E
+    from llmx_b200.engine.engine import StepError, _need_eight_bits
+    from llmx_b200.registry import architecture_of
+    from test_zamizen_config import CFG
+    for config, refused in ((TINY_E, None), (CFG, "LatentAttention, MaskedAttention")):
+        entry = architecture_of(config)
+        model = entry.build(entry.config_cls.from_dict(config))
+        if refused is None:
+            _need_eight_bits(model, model.cache_entry_specs())
+        else:
+            with pytest.raises(StepError, match=refused):
+                _need_eight_bits(model, model.cache_entry_specs())

@@ -485,3 +485,104 @@ def test_written_attended_and_read_back():
         c.requests, c.starts, c.rows, c.q = [(n, at)], [0], n, q[at:at + n]
         c.check()
         at += n
+
+
+# ---- as a step writes it, and in an engine ------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads, g, dim, page, rot_half, normed", [(8, 2, 128, 16, 64, True), (8, 8, 128, 32, 0, False), (6, 2, 64, 16, 32, True), (3, 1, 48, 8, 12, True),
+                                                                   (5, 1, 128, 16, 48, True)])
+def test_a_steps_rows_go_in_as_their_32_bit_ones_would(dtype, heads, g, dim, page, rot_half, normed):
+    """Queries have the bits that they have over a cache of another type; keys and values are the 32-bit cache's, quantized."""
+    gen = torch.Generator().manual_seed(dim)
+    rows, n_pages = 37, 8
+    qkv = torch.randn(rows, (heads + 2 * g) * dim, generator=gen).to(DEV)
+    qkv[3, heads * dim + 5], qkv[4, -1] = math.inf, math.nan
+    qw, kw = ((1 + 0.1 * torch.randn(dim, generator=gen)).to(DEV) for _ in range(2)) if normed else (None, None)
+    angle = torch.rand(64, max(rot_half, 1), generator=gen).to(DEV) * 6
+    cos, sin = (angle.cos().contiguous(), angle.sin().contiguous()) if rot_half else (None, None)
+    positions = torch.randint(0, 64, (rows,), generator=gen).int().to(DEV)
+    slots = torch.randperm(n_pages * page, generator=gen)[:rows].int().to(DEV)
+    slots[7] = -1
+    q32, q = torch.zeros(rows, heads * dim, device=DEV), torch.zeros(rows, heads * dim, dtype=dtype, device=DEV)
+    plain, cache = torch.zeros(n_pages, 2, g, page, dim, device=DEV), ops.QuantizedPages.zeros(n_pages, g, page, dim, DEV)
+    for out, store in ((q32, plain), (q, cache)):
+        ops.head_norm_rope_kv(qkv, heads, g, dim, qw, kw, 1e-6, cos, sin, positions, slots, out, store)
+    assert torch.equal(q, q32.to(dtype))
+    values, b = quantized(plain.cpu().double().numpy())
+    assert np.array_equal(cache.exponents.cpu().numpy(), b)
+    want = np.where(b[..., None] == 255, np.nan, values * np.exp2(b[..., None] - 127.0))
+    assert np.array_equal(decoded(cache.codes, cache.exponents), want, equal_nan=True)
+
+
+@gpu
+@pytest.mark.parametrize("requests", [[(1, 300), (1, 5), (1, 77)], [(200, 33), (1, 100), (3, 0)]])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_paged_kernels_entry_takes_eight_bits(requests, dtype):
+    from llmx_b200 import ops_attn
+    c = Case(requests, 8, 2, 128, 16, dtype, seed=14, spare_rows=0)
+    step = ops_attn.attention_step(DEV, [(h, n) for n, h in requests], c.tables.clamp(min=0).numpy(), 8, 2, 128, None)
+
+    class Same(Case):
+        def run(self, window=None, out=None):
+            out = torch.zeros_like(self.q.to(DEV))
+            ops_attn.paged_attention(self.q.to(DEV), out, step, 0, 8, 2, 128, window, self.scale, cache=ops_attn.OneEntryCache(self.cache))
+            return out.double().cpu()
+    c.__class__ = Same
+    c.check()
+
+
+def _plain_logits(folder, ids, bf16):
+    import helpers
+    import plain_qwen3 as plain
+    cfg, w = helpers._folder(folder)
+
+    def in_eight_bits(x):
+        values, b = quantized(np.asarray(x, dtype=np.float64))
+        return (values * np.exp2(b[..., None] - 127.0)).astype(np.float32)
+    return plain.forward(cfg, w, list(ids), act_round=plain.round_bf16 if bf16 else None, cache_round=in_eight_bits)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["A", "B", "C", "D", "E"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("record", [False, True])
+def test_an_engine_over_eight_bits(model_dirs, name, dtype, record):
+    """Logits against the plain implementation that quantizes the same keys and values.  A key that falls on the other side of a
+    rounding border moves a logit by 2e-3 of the scale where steps are bfloat16's (test_a_cache_type_of_its_own); a code's
+    steps are 16 times as wide."""
+    import helpers
+    from configs import BF16_BUDGET, CONFIGS
+    from llmx_b200.engine import Engine, EngineOptions
+    d16, d32, page = model_dirs[name]
+    folder = d32 if dtype == "float32" else d16
+    vocab = CONFIGS[name][0]["vocab_size"]
+    requests = {f"k{i}": helpers.random_ids(vocab, n, seed=90 + i) for i, n in enumerate([70, 9, 133, 33, 1])}
+    steps = helpers.trace_tail_decoded(requests, 20) if record else helpers.trace_mixed(requests)
+    engine = Engine.from_dir(folder, EngineOptions(dtype=dtype, kv_dtype="float8_e4m3", kv_tokens=helpers.tokens_needed(steps), page_size=page, max_requests=4,
+                                                   record_after=3))
+    assert engine.cache.groups[0].storage.dtype is torch.float8_e4m3fn
+    got = helpers.run_trace(engine, steps, record=record)
+    assert not record or engine.step_recordings
+    engine.cache.check()
+    for rid, ids in requests.items():
+        ref = _plain_logits(folder, ids, dtype == "bfloat16")
+        scale = float(np.abs(ref).max())
+        worst = max(float(np.abs(got[(rid, p)] - ref[p]).max()) for p in range(len(ids)) if (rid, p) in got)
+        assert worst <= (3.2e-2 + (BF16_BUDGET[name] if dtype == "bfloat16" else 0)) * scale, (rid, worst / scale)
+
+
+@gpu
+def test_generation_over_eight_bits(model_dirs):
+    """The command's entry: greedy tokens with recorded decoding steps, the cache at an eighth of 32 bits and an exponent a row."""
+    from llmx_b200.engine.generate import LLM
+    from llmx_b200.sampling import SamplingParams
+    folder = model_dirs["E"][1]
+    prompts = [[3, 5, 7, 11] * 12, [9], [2, 4] * 50]
+    outs = [LLM(folder, dtype="float32", kv_dtype=t, kv_tokens=1024).generate(prompts, SamplingParams(max_tokens=24, temp=0.0, top_k=0, top_p=1.0, ignore_eos=True))
+            for t in ("float8_e4m3", "float8_e4m3", None)]
+    assert [o.tokens for o in outs[0]] == [o.tokens for o in outs[1]]
+    assert all(len(o.tokens) == 24 for o in outs[0])
+    llm, wide = LLM(folder, dtype="float32", kv_dtype="f8", kv_tokens=1024), LLM(folder, dtype="float32", kv_tokens=1024)
+    d = wide.engine.model.cache_entry_specs()[0].head_dim
+    assert llm.engine.cache.storage_bytes() * 4 * d == wide.engine.cache.storage_bytes() * (d + 1)
