@@ -661,6 +661,7 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
 template <typename QT, bool EIGHT, int D, int TILE_ROWS, int KEYS, int OPEN, int RUNS>
 __global__ void __launch_bounds__(128)
 merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, int requests, int heads, int kv_heads, int grid) {
+    pdl_trigger();
     constexpr int ROWF = D + PART, LANES = D / 4, EACH = 128 / LANES;
     const int r = blockIdx.y, ratio = heads / kv_heads;
     // The kernel before let this one start when the kernels before it had ended: the requests' counts stand.  Every thread waits before

@@ -488,18 +488,22 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 const uint32_t use = before + i;
                 const int stage = use % STAGES, s_buffer = mine & 1;
                 const int t0 = (sg.from + i) * KEYS, t = t0 + key;
-                // The tile's copies, its scores, and that the weights' buffer is free again: asked for together, since an answer takes long.
-                const bool reused = mine > 0;
-                const uint32_t w_parity = (mine & 1u) ^ 1u;
+                // The tile's copies, its scores, and whether the weights' place is free again (which is not needed yet): asked for together,
+                // since an answer takes long.
+                bool free_again = mine == 0;
                 if (ok) {
-                    const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u),
-                               a2 = !reused || is_done(&o_done[unit], w_parity);
-                    if (!__all_sync(0xffffffffu, a0 && a1 && a2)) {
+                    const bool a0 = is_done(&full[stage], (use / STAGES) & 1u), a1 = is_done(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u);
+                    free_again = __all_sync(0xffffffffu, free_again || is_done(&o_done[unit], (mine & 1u) ^ 1u));
+                    if (!__all_sync(0xffffffffu, a0 && a1)) {
                         ok = tc::mbar_wait_warp(&full[stage], (use / STAGES) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                         if (ok) ok = tc::mbar_wait_warp(&s_full[2 * unit + s_buffer], (mine >> 1) & 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
-                        if (ok && reused) ok = tc::mbar_wait_warp(&o_done[unit], w_parity, abort_flag, error_word, ERR_PAGES_SOFTMAX);
                     }
                 }
+                auto weights_place = [&]() {                     // every O^T that has been asked for has been made
+                    if (!free_again && ok) ok = tc::mbar_wait_warp(&o_done[unit], (mine & 1u) ^ 1u, abort_flag, error_word, ERR_PAGES_SOFTMAX);
+                    free_again = true;
+                    tc::tc_fence_after();
+                };
                 tc::tc_fence_after();
                 int runs;
                 asm volatile("ld.shared.s32 %0, [%1];" : "=r"(runs) : "r"(live_at + 4 * stage) : "memory");
@@ -631,7 +635,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     }
                     weights();
                     if (!opening) {
-                        // (Every O^T that has been asked for has been made: the weights' buffer is free.)
+                        weights_place();
 #pragma unroll
                         for (int n = 0; n < R; ++n) sum[n] *= fade_sum[n];
 #pragma unroll
@@ -650,6 +654,7 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s_free[2 * unit + s_buffer]);
                 // ---- the weights to shared memory
+                weights_place();
                 constexpr int SKIP = S::HALVES ? 4 : 0;          // pieces of 16 bytes to the second unit's half
 #pragma unroll
                 for (int n = 0; n < R; ++n) sum[n] += x[n];
