@@ -4,7 +4,7 @@
 // and values follow them there.  Row i sees the keys t with
 //     t <= history + i,  t > history + i - window (window > 0)         or, with a tree,
 //     t < history  or  bit (t - history) of its words is set (t < history + row_count)
-// and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key.
+// and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key (or only such with scores of -inf).
 // Query head h reads key/value head h / (heads / kv_heads).  A page that is not in the cache reads as zeros.
 //
 // Two forms.  Heads of 64 or 128 in pages of 16 to 512 slots by 16 run on the matrix instruction (attention_pages_mma.cuh): queries of either type
@@ -81,9 +81,9 @@ attention_pages_kernel(const QT* __restrict__ q, const void* __restrict__ cache,
             vf = e4m3::up(exponents[v_slot]);
         }
         s *= scale;
-        const float m_new = fmaxf(m, s);
-        const float corr = expf(m - m_new);  // exp(-inf) = 0 on the first key
-        const float e = expf(s - m_new);
+        const float m_new = fmaxf(m, s), base = m_new == -INFINITY ? 0.0f : m_new;      // (a score of -inf weighs nothing, before the first key too)
+        const float corr = expf(m - base);   // exp(-inf) = 0 on the first key
+        const float e = expf(s - base);
         l = l * corr + e;
 #pragma unroll
         for (int j = 0; j < MAX_PER_LANE; ++j) {
@@ -109,7 +109,7 @@ attention_pages_kernel(const QT* __restrict__ q, const void* __restrict__ cache,
     for (int w = 0; w < WARPS; ++w) {
         // A warp without keys has a sum of zero and says nothing; one whose scores are NaN has a NaN there.
         const float lw = smem[w * (head_dim + 2) + head_dim + 1], mw = smem[w * (head_dim + 2) + head_dim];
-        f[w] = lw == 0.0f ? 0.0f : expf(mw - mm);
+        f[w] = lw == 0.0f ? 0.0f : expf(mw - (mm == -INFINITY ? 0.0f : mm));
         ll = fmaf(lw, f[w], ll);
     }
     QT* orow = out + ((size_t)row * heads + h) * head_dim;
@@ -139,7 +139,7 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
                  int window, int general) {
     FewPlan p;
     if (general) return p;
-    const bool types = cache_dtype == LLMX_E4M3 || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
+    const bool types = (cache_dtype == LLMX_E4M3 && (q_dtype == LLMX_BF16 || q_dtype == LLMX_F32)) || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
     p.tensor = head_dim == 128 && q_dtype == LLMX_BF16;

@@ -344,28 +344,37 @@ constexpr int EXPANDED = 16, ROW_PIECES = 16;         // slots of an expanded pa
 // A value row that is no numbers comes as zeros with its key as NaN: the attention's mask then keeps it from the rows that do
 // not see it (a weight of zero would not), and makes NaN of those that do, as it has to.
 __global__ void __launch_bounds__(READERS)
-expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ row_count,
-              const int* __restrict__ history, const int* __restrict__ tables, int table_stride, int requests, int rows_over, int window, int pages,
+expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, const int* __restrict__ row_start,
+              const int* __restrict__ row_count, const int* __restrict__ history, const int* __restrict__ tables, int table_stride, int requests,
+              int total_rows, int rows_over, int max_rows, int window, int pages,
               int kv_heads, int page_size, __nv_bfloat16* __restrict__ out, int* __restrict__ out_table, int out_stride,
               int* __restrict__ out_count, int* __restrict__ out_list) {
     pdl_trigger();
     pdl_wait();
+    // A request's rows, none where it is left out: its reader trusts what it gets, so rows must lie in the output, and keys (up to the
+    // end of the last stage of 128) in the request's part of the table.
+    auto rows_of = [&](int r) {
+        const int n = row_count[r], h = history[r], start = row_start[r];
+        return n > rows_over && n <= max_rows && h >= 0 && start >= 0 && (long long)h + n <= (long long)(out_stride - 8) * EXPANDED
+                   ? max(min(n, total_rows - start), 0) : 0;
+    };
     __shared__ int owner, page_of_owner;
     if (threadIdx.x == 0) owner = -1;
     __syncthreads();
     if (blockIdx.x == 0)
         for (int r = threadIdx.x; r < requests; r += blockDim.x) {
             out_list[r] = r;
-            out_count[r] = row_count[r] > rows_over ? row_count[r] : 0;
+            out_count[r] = rows_of(r);
         }
     if (threadIdx.x < 32) {
         const int f = blockIdx.x;
         int before = 0;
         for (int r0 = 0; r0 < requests && before <= f; r0 += 32) {
             const int r = r0 + threadIdx.x;
+            const int rows = r < requests ? rows_of(r) : 0;
             int n = 0, first = 0;
-            if (r < requests && row_count[r] > rows_over) {
-                const int keys = history[r] + row_count[r];
+            if (rows > 0) {
+                const int keys = history[r] + rows;
                 // The reader starts at a whole stage of 128 keys.
                 first = window > 0 ? max(0, history[r] - window + 1) / 128 * (128 / EXPANDED) : 0;
                 n = max(0, min((keys + EXPANDED - 1) / EXPANDED, out_stride) - first);
@@ -384,7 +393,7 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
     const int r = owner, j = page_of_owner;
     if (r < 0) return;
     if (threadIdx.x == 0) out_table[(size_t)r * out_stride + j] = blockIdx.x;
-    const int keys = min(history[r] + row_count[r], table_stride * page_size);
+    const int keys = (int)min((long long)history[r] + rows_of(r), (long long)table_stride * page_size);
     const int total = 2 * kv_heads * EXPANDED * ROW_PIECES, low = window > 0 ? max(0, history[r] - window + 1) : 0;
     const int* table = tables + (size_t)r * table_stride;
     const size_t plane = (size_t)kv_heads * page_size;
@@ -506,15 +515,16 @@ LLMX_EXPORT int llmx_dequantize_pages(const void* codes, const void* exponents, 
     return launch_status();
 }
 
-// Requests of more than `rows_over` rows, their keys and values as bfloat16 pages out[0 .. capacity) of [2, kv_heads, 16, 128]: all of
+// Requests of more than `rows_over` rows (and at most `max_rows`), their keys and values as bfloat16 pages out[0 .. capacity) of [2, kv_heads, 16, 128]: all of
 // them, or under a window those from the stage of 128 that the first row's window starts in.  `capacity` pages must hold them.
-LLMX_EXPORT int llmx_expand_requests(const void* codes, const void* exponents, const int* row_count, const int* history, const int* tables,
-                                     int table_stride, int requests, int rows_over, int window, int pages, int kv_heads, int head_dim, int page_size,
+LLMX_EXPORT int llmx_expand_requests(const void* codes, const void* exponents, const int* row_start, const int* row_count, const int* history,
+                                     const int* tables, int table_stride, int requests, int total_rows, int rows_over, int max_rows, int window, int pages,
+                                     int kv_heads, int head_dim, int page_size,
                                      void* out, int capacity, int* out_table, int out_stride, int* out_count, int* out_list, cudaStream_t stream) {
     if (requests <= 0 || capacity <= 0) return 0;
     if (kv_heads <= 0 || head_dim != 8 * ROW_PIECES || page_size <= 0 || (((uintptr_t)codes | (uintptr_t)out) & 15)) return LLMX_ERR_UNSUPPORTED;
-    launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(READERS), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_count, history,
-                  tables, table_stride, requests, rows_over, window, pages, kv_heads, page_size, (__nv_bfloat16*)out, out_table, out_stride,
+    launch_kernel(expand_kernel, dim3((unsigned)capacity), dim3(READERS), 0, stream, (const uint8_t*)codes, (const uint8_t*)exponents, row_start,
+                  row_count, history, tables, table_stride, requests, total_rows, rows_over, max_rows, window, pages, kv_heads, page_size, (__nv_bfloat16*)out, out_table, out_stride,
                   out_count, out_list);
     return launch_status();
 }

@@ -49,8 +49,8 @@ typedef cudaStream_t S;
     X(llmx_attention_pages_workspace, (int, int, int, int, int, int, int, int, int, int, int, long long*))                         \
     X(llmx_head_norm_rope_e4m3, (const float*, int, int, int, const float*, const float*, float, const float*, const float*,      \
                                  int, const int*, const int*, void*, int, void*, void*, long long, int, int, int, int, int, S))   \
-    X(llmx_expand_requests, (const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, int, int,    \
-                             void*, int, int*, int, int*, int*, S))                                                       \
+    X(llmx_expand_requests, (const void*, const void*, const int*, const int*, const int*, const int*, int, int, int, int, int,       \
+                             int, int, int, int, int, void*, int, int*, int, int*, int*, S))                              \
     X(llmx_gemm_tc_weight_map, (void*, const void*, int, int))                                                            \
     X(llmx_gemm_tc_weight_map_box, (void*, const void*, int, int, int))                                                   \
     X(llmx_gemm_tc, (const void*, const void*, float*, int, int, int, int, int, int, int, int*, S))                       \
@@ -432,8 +432,9 @@ namespace {
 constexpr int FEW_PAIRS = 64;             // (row, head) pairs of a group up to which a request's rows read the pages as they are
 constexpr int EXPANDED_PAGE = 16;
 
-int pages_attention(Ctx& c, const llmx_pages_call& p) {
+int pages_attention(Ctx& c, llmx_pages_call p) {
     if (p.requests <= 0 || p.total_rows <= 0 || p.max_rows <= 0) return 0;
+    p.max_rows = std::min(p.max_rows, p.total_rows);          // (no request has more)
     const int ratio = p.heads / p.kv_heads;
     auto few = [&](int max_rows) {
         if (!kern.llmx_attention_pages_workspace) {
@@ -469,7 +470,8 @@ int pages_attention(Ctx& c, const llmx_pages_call& p) {
     int* table = c.alloc_n<int>((size_t)p.requests * stride);
     int* count = c.alloc_n<int>(p.requests);
     int* list = c.alloc_n<int>(p.requests);
-    CALL(c, llmx_expand_requests, 1, p.cache, p.exponents, p.row_count, p.history, p.tables, p.table_stride, p.requests, rows_few, p.window, p.pages,
+    CALL(c, llmx_expand_requests, 1, p.cache, p.exponents, p.row_start, p.row_count, p.history, p.tables, p.table_stride, p.requests, p.total_rows,
+         rows_few, p.max_rows, p.window, p.pages,
          p.kv_heads, p.head_dim, p.page_size, expanded, (int)capacity, table, stride, count, list, c.stream);
     int tiles = 2, splits = 1;
     prefill_shape(p.requests, p.kv_heads, ratio, p.max_rows, p.max_context, p.window, sms(), &tiles, &splits);

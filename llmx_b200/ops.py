@@ -1427,10 +1427,10 @@ def _attention_pages(what: str, q, cache, out, row_start, row_count, history, bl
             raise KernelError(f"{what}: int32 first rows, row counts and histories, one per request")
     if not (block_tables.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests and block_tables.is_contiguous()):
         raise KernelError(f"{what}: int32 block tables [requests, pages]")
-    if tree is not None and not (tree.dtype is torch.int32 and tree.dim() == 2 and tree.shape[0] == rows and tree.is_contiguous()):
-        raise KernelError(f"{what}: int32 words of bits, [rows, words]")
-    if not (0 <= max_rows < 2 ** 31 and 0 <= max_context < 2 ** 31 and (window is None or 0 < window < 2 ** 31) and scale > 0):
-        raise KernelError(f"{what}: bounds of at least 0, a window of at least 1, a scale above 0")
+    if tree is not None and not (tree.dtype is torch.int32 and tree.dim() == 2 and tree.shape[0] == rows and tree.shape[1] > 0 and tree.is_contiguous()):
+        raise KernelError(f"{what}: int32 words of bits, [rows, words], one at least")
+    if not (0 <= max_rows < 2 ** 31 and 0 <= max_context < 2 ** 31 and (window is None or 0 < window < 2 ** 31) and 0 < scale < 2.0 ** 127):
+        raise KernelError(f"{what}: bounds of at least 0, a window of at least 1, a scale above 0 that 32 bits hold")
     q_code, code, device = _code(q), E4M3 if eight else _code(stored), q.device
     sizes = (q_code, code, block_tables.shape[1], 0 if tree is None else tree.shape[1], requests, rows, int(max_rows), int(max_context), 0, at[0], heads,
              kv_heads, head_dim, at[3], int(window or 0), 0)
@@ -1475,7 +1475,7 @@ def attention_tree(q: torch.Tensor, cache, out: torch.Tensor, row_start: torch.T
                    max_context: int) -> torch.Tensor:
     """`attention_quantized` for rows that are drafted tokens: a row sees its request's whole history, and key history[r] + j, that
     of the request's j-th row, where bit j % 32 of word j // 32 of its words in `tree` (int32 [rows, words], `tree_bits`) is set:
-    rows may see rows behind them, and not themselves; one that sees no key is zeros.  `cache`: `QuantizedPages`, or bfloat16 or
+    rows may see rows behind them, and not themselves; one that sees no key, or only keys with scores of -inf, is zeros.  `cache`: `QuantizedPages`, or bfloat16 or
     float32 [pages, 2, kv_heads, page size, head_dim].  Where the drafted tokens' rotations stand is the queries' and keys' own
     business."""
     return _attention_pages("attention_tree", q, cache, out, row_start, row_count, history, block_tables, tree, heads, kv_heads, head_dim, None, scale,

@@ -94,6 +94,8 @@ REFUSED = [
     ("scale above 0", dict(scale=0.0)),
     ("scale above 0", dict(scale=-1.0)),
     ("scale above 0", dict(scale=float("nan"))),
+    ("scale above 0", dict(scale=float("inf"))),
+    ("scale above 0", dict(scale=1e39)),
     ("CUDA tensors", dict()),
 ]
 
@@ -112,6 +114,7 @@ def test_attention_quantized_refuses(what, changes):
     ("words", dict(tree=torch.zeros(2, 1, dtype=torch.int32))),
     ("words", dict(tree=torch.zeros(3, 1, dtype=torch.int64))),
     ("words", dict(tree=torch.zeros(3, dtype=torch.int32))),
+    ("words", dict(tree=torch.zeros(3, 0, dtype=torch.int32))),
     ("not one the kernels take", dict(cache=torch.zeros(4, 2, 2, 16, 64, dtype=torch.float16))),
 ])
 def test_attention_tree_refuses(what, changes):

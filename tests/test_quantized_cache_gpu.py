@@ -356,6 +356,45 @@ def test_rows_that_do_not_see_a_drafted_token_do_not_meet_its_infinities(store, 
 
 
 @gpu
+@pytest.mark.parametrize("store, dtype, heads, g, dim", [("bfloat16", BF16, 4, 2, 128), ("bfloat16", BF16, 4, 2, 64), ("bfloat16", BF16, 4, 2, 96),
+                                                         ("bfloat16", F32, 4, 2, 128), ("float32", F32, 4, 2, 64)])
+@pytest.mark.parametrize("h", [0, 130])
+def test_a_key_with_a_score_of_minus_infinity_weighs_nothing(store, dtype, heads, g, dim, h):
+    """The first drafted token's keys give every row -inf: as if no row saw it.  Rows that see only such keys are zeros."""
+    requests = [(6, h), (3, 10)]
+    c = Case(requests, heads, g, dim, 16, dtype, store, seed=11, spare_rows=0)
+    x = c.q.view(-1, heads, dim)
+    x[..., 3] = x[..., 3].abs() + 0.25
+    c.cache[int(c.tables[0][h // 16]), 0, :, h % 16, 3] = -math.inf
+    c.tree = ops.tree_bits([[-1, 0, 0, 1, 2, 2], [-1, 0, 1]])
+    got = c.run()
+    c.tree[:6] &= ~1
+    assert torch.equal(got, c.run()) and bool(got.isfinite().all())
+    assert bool((got[0] == 0).all()) == (h == 0)
+
+
+@gpu
+@pytest.mark.parametrize("n, h, claimed", [(100, 40, 100), (30, 500, 30), (100, 40, 101), (30, 500, 400)])
+def test_rows_and_keys_beyond_what_was_said(n, h, claimed):
+    """Counts on the device that the call's bounds do not cover: rows beyond the output's are not written, a request of more rows than
+    `max_rows` is left alone, the others are what they were."""
+    c = Case([(n, h), (2, 9)], 8, 2, 128, 16, BF16, seed=12, spare_rows=0)
+    want, q = c.run(), c.q.to(DEV)
+    for counts, max_rows, same in (([n, claimed], n, slice(0, n)), ([claimed, 2], n, slice(n, n + 2))):
+        out = torch.full_like(q, 7.0)
+        starts, _, histories, tables = c.device()
+        ops.attention_quantized(q, c.cache, out, starts, torch.tensor(counts, dtype=torch.int32, device=DEV), histories, tables, c.heads, c.g, c.dim,
+                                None, c.scale, max_rows, c.bounds()[1])
+        assert torch.equal(out[same].double().cpu(), want[same])
+        if claimed > max_rows:
+            other = slice(n, n + 2) if counts[0] == n else slice(0, n)
+            assert bool((out[other] == 7.0).all())
+    out = torch.full_like(q, 7.0)
+    ops.attention_quantized(q, c.cache, out, *c.device(), c.heads, c.g, c.dim, None, c.scale, n, max(h - 1, 20))      # fewer keys than there are
+    assert torch.equal(out[n:].double().cpu(), want[n:])
+
+
+@gpu
 @pytest.mark.parametrize("heads, g, dim", [(8, 2, 128), (4, 2, 64)])
 @pytest.mark.parametrize("n, h", [(5, 300), (200, 100), (300, 3000)])
 @pytest.mark.parametrize("plane", [0, 1])
