@@ -7,10 +7,11 @@
 // and   o = sum_t e_t v_t / sum_t e_t,   e_t = exp(scale q . k_t - max),  zeros where a row sees no key (or only such with scores of -inf).
 // Query head h reads key/value head h / (heads / kv_heads).  A page that is not in the cache reads as zeros.
 //
-// Two forms.  Heads of 64 or 128 in pages of 16 to 512 slots by 16 run on the matrix instruction (attention_pages_mma.cuh): queries of either type
-// over eight bits, bfloat16 over bfloat16.  The general form takes any width to 256, any page size and any types, one block a
-// (row, head): each warp walks every fourth key in increasing order
-// with a running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone.
+// Three forms.  Heads of 64 or 128 in pages of 16 to 512 slots by 16 run on matrix instructions, the warps' (attention_pages_mma.cuh) or
+// tcgen05's (attention_pages_tc.cuh): queries of either type over eight bits, bfloat16 over bfloat16.  The general form takes any
+// width to 256, any page size and any types, one block a (row, head): each warp walks every fourth key in increasing order with a
+// running maximum and sum; the four states are merged in warp order, so a row's sums depend on its own keys alone (3.5 ms where the
+// warps' form takes 33 us: 8 rows after 8,192 keys, 32 heads of 128 over 8).
 #include "attention_pages_mma.cuh"
 #include "attention_pages_tc.cuh"
 
@@ -142,7 +143,13 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
     const bool types = (cache_dtype == LLMX_E4M3 && (q_dtype == LLMX_BF16 || q_dtype == LLMX_F32)) || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
-    p.tensor = head_dim == 128 && q_dtype == LLMX_BF16;
+    // Over eight bits the warps' form is as fast up to 32 pairs and simpler to feed (us; warps against tcgen05 with tiles as high as the
+    // pairs ask for: 1 x 32,768 keys of 4 pairs 25.6 / 26.6, 8 x 8,192 32.6 / 34.3, 64 requests of 2 pairs 63 / 70, 8 x 4,096 of 32 pairs
+    // 33.2 / 34.4); from 33 on a tile's keys are turned into halves for too many warps (8 x 4,096 of 64 pairs 57.6 / 52.4, 1 x 8,191 of
+    // 252 54.3 / 43.6; 32 x 1,024 of 64 71 / 74).
+    p.tensor = head_dim == 128 && q_dtype == LLMX_BF16 && (cache_dtype == LLMX_BF16 || pairs > 32);
+    // As few rows a tile as hold a request's: bfloat16, 8 x 4,096 keys, tiles of 16 / 32 / 64 rows: of 16 pairs 39 / 45 / 49 us, of 32 60 /
+    // 46 / 51, of 64 106 / 72 / 54.
     p.rows = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
     // As many blocks as find an SM at one time.  The kernel leaves some of them without work where there is too little.
     const long long items = (pairs + p.rows - 1) / p.rows * kv_heads * requests;
@@ -236,11 +243,7 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
         if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes(head_dim)) return LLMX_ERR_BAD_ARGUMENT;
 #define LLMX_FEW_ARGS p, q, cache, exponents, out, (float*)workspace, a, requests, max_rows, heads, kv_heads, scale
         if (p.tensor) {
-            if (cache_dtype == LLMX_E4M3) {
-                if (p.rows == 16) return tensor_rows<true, true, 16>(LLMX_FEW_ARGS, error_word, stream);
-                if (p.rows == 32) return tensor_rows<true, true, 32>(LLMX_FEW_ARGS, error_word, stream);
-                return tensor_rows<true, false, 32>(LLMX_FEW_ARGS, error_word, stream);
-            }
+            if (cache_dtype == LLMX_E4M3) return tensor_rows<true, false, 32>(LLMX_FEW_ARGS, error_word, stream);
             if (p.rows == 16) return tensor_rows<false, true, 16>(LLMX_FEW_ARGS, error_word, stream);
             if (p.rows == 32) return tensor_rows<false, true, 32>(LLMX_FEW_ARGS, error_word, stream);
             return tensor_rows<false, false, 32>(LLMX_FEW_ARGS, error_word, stream);
@@ -252,7 +255,9 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
         return few_rows<QT, EIGHT, D, 4>(LLMX_FEW_ARGS, stream);                            \
     } while (0)
         if (cache_dtype == LLMX_BF16) LLMX_FEW_ROWS(__nv_bfloat16, false, 64);
-        if (q_dtype == LLMX_BF16) LLMX_FEW_ROWS(__nv_bfloat16, true, 64);
+        if (q_dtype == LLMX_BF16 && head_dim == 64) LLMX_FEW_ROWS(__nv_bfloat16, true, 64);
+        if (q_dtype == LLMX_BF16 && p.rows == 16) return few_rows<__nv_bfloat16, true, 128, 1>(LLMX_FEW_ARGS, stream);
+        if (q_dtype == LLMX_BF16) return few_rows<__nv_bfloat16, true, 128, 2>(LLMX_FEW_ARGS, stream);
         if (head_dim == 64) LLMX_FEW_ROWS(float, true, 64);
         LLMX_FEW_ROWS(float, true, 128);
 #undef LLMX_FEW_ARGS

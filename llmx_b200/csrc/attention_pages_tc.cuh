@@ -1,7 +1,8 @@
-// Attention over pages on the tensor cores of tcgen05: few rows a request (decoding, drafts), heads of 128.
+// Attention over pages on the tensor cores of tcgen05: few rows a request, heads of 128; all of bfloat16 pages (decoding, drafts), and
+// over eight bits more than 32 (row, head) pairs (trees of drafts).
 //
-// The warp form (attention_pages_mma.cuh) spends its time on turning codes into halves and moving them through registers.  Here neither
-// keys nor values pass through registers at all: TMA brings 128 keys of a head to shared memory as they lie in their pages, and the
+// The warp form (attention_pages_mma.cuh) spends its time on turning codes into halves, again for every 16 rows, and moving them through
+// registers.  Here neither keys nor values pass through registers at all: TMA brings 128 keys of a head to shared memory as they lie in their pages, and the
 // matrix instruction reads codes (kind::f8f6f4; bfloat16 pages: kind::f16) from there, keys and values on its 128-row side:
 //     S^T [128 keys, rows] = K Q^T           K as it lies, K-major
 //     O^T [128 values, rows] += V^T W^T      V as it lies, MN-major; W^T [keys, rows] written by the softmax warps, MN-major
@@ -55,10 +56,11 @@ struct Shape {
     static constexpr int HALF = 2 * KEYS * 128, STAGE = EIGHT ? HALF : 2 * HALF;
     // As many stages as there is room for: a stage is taken for some 5,000 clocks, a third of them until its copies have come, and
     // memory gives one in 1,000.
-    static constexpr int STAGES = !EIGHT ? 2 : R == 16 ? 6 : 5;
-    // A tile's weights: rows of 128 bytes a key, of which a unit has one half, or all.
+    static constexpr int STAGES = EIGHT ? 5 : 2;
+    // A tile's weights: rows of 128 bytes a key, of which a unit has one half (bfloat16), or all.
     static constexpr int WEIGHTS = KEYS * 128;
-    static constexpr bool HALVES = !EIGHT || R == 16;
+    static constexpr bool HALVES = !EIGHT;
+    static_assert(!EIGHT || !SHARED, "few rows over eight bits are the warp form's");
     static constexpr int ROWS = SHARED ? R : U * R;             // of an item
     static constexpr int Q_BYTES = 2 * R * D;                   // R rows' queries: two codes each, or bfloat16
     static constexpr int Q_BUFFERS = SHARED ? 2 : 1;            // (two would not fit)

@@ -429,7 +429,13 @@ bool tensor_core_prefill(int heads, int kv_heads, int head_dim, int page_size) {
 // Attention over pages of any cache type.
 // ---------------------------------------------------------------------------------------------------------------
 namespace {
-constexpr int FEW_PAIRS = 64;             // (row, head) pairs of a group up to which a request's rows read the pages as they are
+// (Row, head) pairs of a group up to which a request's rows read the pages as they are.  Beyond, their keys and values become bfloat16
+// once (exact), and the prompt kernel runs over them: that reads and writes some 1.7 us' worth a thousand keys of 8 heads and takes 20 us
+// besides, but a tile of 64 pairs more costs next to nothing.  In us, as they are / expanded, 32 heads over 8: one request of 1,024 keys,
+// 64 pairs 21 / 25, 256 22 / 26; of 8,192 keys, 64 26 / 39, 128 31 / 41, 256 43 / 42; 8 requests of 1,024, 64 28 / 33, 96 39 / 33, 128
+// 41 / 34; of 4,096, 64 50 / 76, 128 81 / 78, 192 115 / 86.  So a tile for every request, or up to four where the tiles of all heads
+// leave most of the SMs idle.
+int few_pairs(long long requests, int kv_heads) { return 64 * (int)std::min(4ll, std::max(1ll, 32 / std::max(requests * kv_heads, 1ll))); }
 constexpr int EXPANDED_PAGE = 16;
 
 int pages_attention(Ctx& c, llmx_pages_call p) {
@@ -451,16 +457,15 @@ int pages_attention(Ctx& c, llmx_pages_call p) {
              p.tables, p.table_stride, p.tree, p.tree_words, p.requests, p.total_rows, max_rows, p.max_context, p.pages, p.heads, p.kv_heads,
              p.head_dim, p.page_size, p.window, p.general, p.scale, at, room, p.error_word, c.stream);
     };
-    // Many rows: their keys and values become bfloat16 once (exact), and the prompt kernel runs over them.  Its tiles of 128 pairs are
-    // half empty below FEW_PAIRS.
-    const bool many = p.cache_dtype == LLMX_DT_E4M3 && p.q_dtype == LLMX_DT_BF16 && !p.tree && !p.general && (long long)p.max_rows * ratio > FEW_PAIRS &&
+    const int most_pairs = few_pairs(p.requests, p.kv_heads);
+    const bool many = p.cache_dtype == LLMX_DT_E4M3 && p.q_dtype == LLMX_DT_BF16 && !p.tree && !p.general && (long long)p.max_rows * ratio > most_pairs &&
                       tensor_core_prefill(p.heads, p.kv_heads, p.head_dim, ATTN_PAGE) &&
                       !(((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.cache) & 15);
     if (!many) {
         few(p.max_rows);
         return c.status;
     }
-    const int rows_few = std::max(FEW_PAIRS / ratio, 0);
+    const int rows_few = most_pairs / ratio;
     const long long most = p.window > 0 ? std::min((long long)p.max_context, (long long)p.window + p.max_rows + 128) : p.max_context;
     long long capacity = (long long)p.requests * (most / EXPANDED_PAGE + 2);
     if (p.total_context > 0) capacity = std::min(capacity, p.total_context / EXPANDED_PAGE + 2ll * p.requests);
@@ -487,7 +492,7 @@ int pages_attention(Ctx& c, llmx_pages_call p) {
     CALL(c, llmx_attn_prefill_tc, splits > 1 ? 2 : 1, (const void*)map, p.q, p.out, p.total_rows, (const int*)list, p.requests, p.row_start,
          (const int*)count, p.history, (const int*)table, stride, p.heads, p.kv_heads, p.head_dim, EXPANDED_PAGE, p.window, p.scale, p.max_rows, tiles,
          splits, partial, p.error_word, c.stream);
-    if (p.requests > 1 && rows_few > 0) few(std::min(p.max_rows, rows_few));
+    if (p.requests > 1) few(std::min(p.max_rows, rows_few));
     return c.status;
 }
 }  // namespace

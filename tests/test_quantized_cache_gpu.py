@@ -211,7 +211,8 @@ class Case:
         for r, (n, h) in enumerate(self.requests):
             if n == 0:
                 continue
-            prompt = self.tree is None and self.dim == 128 and n * self.heads // self.g > 64
+            most = 64 * min(4, max(1, 32 // (len(self.requests) * self.g)))       # pairs of a request whose weights are not rounded to bfloat16
+            prompt = self.tree is None and self.dim == 128 and n * self.heads // self.g > most
             weight_step = 2.0 ** -21 if self.dtype is F32 else 2.0 ** -8 if self.store == "bfloat16" or prompt else 2.0 ** -11
             kv, ok = self.keys(r), self.seen(r, window)
             for head in range(self.heads):
@@ -374,7 +375,7 @@ def test_a_key_with_a_score_of_minus_infinity_weighs_nothing(store, dtype, heads
 
 
 @gpu
-@pytest.mark.parametrize("n, h, claimed", [(100, 40, 100), (30, 500, 30), (100, 40, 101), (30, 500, 400)])
+@pytest.mark.parametrize("n, h, claimed", [(100, 40, 100), (90, 500, 90), (100, 40, 101), (90, 500, 400)])
 def test_rows_and_keys_beyond_what_was_said(n, h, claimed):
     """Counts on the device that the call's bounds do not cover: rows beyond the output's are not written, a request of more rows than
     `max_rows` is left alone, the others are what they were."""
