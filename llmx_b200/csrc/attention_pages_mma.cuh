@@ -686,32 +686,48 @@ merge_kernel(const float* __restrict__ partial, QT* __restrict__ out, Rows a, in
     const int slot0 = 2 * b0 + (share_begins(all, blocks, b0) > x0 ? 0 : 1);
     const float* base = partial + (size_t)(pair % TILE_ROWS) * ROWF;
     auto state = [&](int b) { return base + (size_t)(b == b0 ? slot0 : 2 * b) * TILE_ROWS * ROWF; };
-    float t = -INFINITY, most = -INFINITY;
-    for (int b = b0; b <= b1; b += 8) {
-        float4 m[8];
+    // A lane has the maxima and sum of one of LANES states, and its four values of all of them, AT_ONCE asked for at one time: what this
+    // takes is the trips to memory.  Sixteen where few rows share many blocks (37 states a row of 1 x 32,768 keys: the call 23.5 us,
+    // with eight 24.3, with every lane reading all states' maxima first 26.0), but their registers cost where many rows share a few
+    // (8 x 4,096 keys of 64 pairs: 56 us, with eight 52.5).
+    constexpr int AT_ONCE = TILE_ROWS == 16 ? 16 : 8;
+    const int lane = threadIdx.x % LANES;
+    const unsigned together = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    float4 v[AT_ONCE];
+    auto ask = [&](int b) {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) m[n] = *reinterpret_cast<const float4*>(state(min(b + n, b1)) + D);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) t = fmaxf(t, m[n].x), most = fmaxf(most, m[n].y);
+        for (int n = 0; n < AT_ONCE; ++n)
+            if (b + n <= b1) v[n] = *reinterpret_cast<const float4*>(state(b + n) + d);
+    };
+    auto ends = [&](int b) { return b + lane <= b1 ? *reinterpret_cast<const float4*>(state(b + lane) + D) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f); };
+    const float4 mine = ends(b0);
+    ask(b0);
+    float t = mine.x, most = mine.y;
+    for (int b = b0 + LANES; b <= b1; b += LANES) {
+        const float4 m = ends(b);
+        t = fmaxf(t, m.x), most = fmaxf(most, m.y);
     }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) t = fmaxf(t, __shfl_xor_sync(together, t, o)), most = fmaxf(most, __shfl_xor_sync(together, most, o));
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f;
-    for (int b = b0; b <= b1; b += 8) {
-        float4 v[8], m[8];
+    for (int b = b0; b <= b1; b += LANES) {
+        const float4 m = b == b0 ? mine : ends(b);
+        const float f = share(m.x, t);
+        l = fmaf(m.z, share(m.y, most), l);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const float* s = state(min(b + n, b1));
-            v[n] = *reinterpret_cast<const float4*>(s + d);
-            m[n] = *reinterpret_cast<const float4*>(s + D);
-        }
+        for (int k = 0; k < LANES; k += AT_ONCE) {
+            if (b + k > b1) break;
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (b + n <= b1) {
-                const float f = share(m[n].x, t);
-                acc.x = fmaf(v[n].x, f, acc.x); acc.y = fmaf(v[n].y, f, acc.y); acc.z = fmaf(v[n].z, f, acc.z); acc.w = fmaf(v[n].w, f, acc.w);
-                l = fmaf(m[n].z, share(m[n].y, most), l);
+            for (int n = 0; n < AT_ONCE; ++n) {
+                const float fn = __shfl_sync(together, f, k + n, LANES);
+                if (b + k + n <= b1) acc.x = fmaf(v[n].x, fn, acc.x), acc.y = fmaf(v[n].y, fn, acc.y), acc.z = fmaf(v[n].z, fn, acc.z), acc.w = fmaf(v[n].w, fn, acc.w);
             }
+            ask(b + k + AT_ONCE);
+        }
     }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) l += __shfl_xor_sync(together, l, o);
     write4(out + ((size_t)(rq.start + row) * heads + head) * D + d, finished<EIGHT>(acc, t, most, l));
 }
 
