@@ -262,7 +262,8 @@ head_norm_rope_128_kernel(HeadsIn a, QT* __restrict__ q_out, uint8_t* __restrict
 
 // ---- reading back: bound by the bytes written ----
 // 16 bytes of the output a thread (8 codes, or 4), four of them 256 pieces apart, whose loads are all asked for before the first is used; a
-// block has up to 1024 pieces of a page.
+// block has up to 1024 pieces of a page.  Pages of 8 heads of 128 and 16 slots as bfloat16: 512 in 11.7 us, 4,096 in 75 (5.4 TB/s; a copy of what
+// is written takes 82); 512 as float32 in 19.
 __device__ __forceinline__ float code_value(unsigned halves, bool upper) {
     return __half2float(__ushort_as_half((unsigned short)(upper ? halves >> 16 : halves & 0xffffu)));
 }
@@ -340,7 +341,7 @@ constexpr int EXPANDED = 16, ROW_PIECES = 16;         // slots of an expanded pa
 
 // Requests' keys and values as bfloat16 pages of 16 slots, for a kernel that reads those: the requests of more than `rows_over` rows, one
 // after another without gaps, a block a page.  `out_table` names a request's pages, `out_count` has its rows (none for the requests
-// that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value.
+// that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value (8,192 keys of 8 heads: 12 us).
 // A value row that is no numbers comes as zeros with its key as NaN: the attention's mask then keeps it from the rows that do
 // not see it (a weight of zero would not), and makes NaN of those that do, as it has to.
 __global__ void __launch_bounds__(READERS)
@@ -446,12 +447,14 @@ LLMX_EXPORT int llmx_quantize_kv(const void* k, long long k_stride, const void* 
     const long long items = (long long)rows * 2 * kv_heads, blocks = (items + WARPS - 1) / WARPS;
     if (blocks >= (1ll << 31)) return LLMX_ERR_UNSUPPORTED;
     // Rows in 16-byte pieces where they lie so and a warp's lanes are whole rows.  Few items: one at a time a warp, so that they find more
-    // of the device's warps (8 rows of 16 heads of 128 float32: 1.7 us either way); many: four, for their loads' latency.
+    // of the device's warps; many: two, for their loads' latency.  In us with one / two / four, rows of 8 heads of 128: 8 of float32 1.3 /
+    // 1.5 / 2.0, 256 2.3 / 2.9 / 3.0, 1,024 4.9 / 4.5 / 5.1, 8,192 34 / 23 / 22, 40,000 of bfloat16 84 / 68 / 80.  Warps that stay and ask for
+    // the next rows before these are written are no faster (26 and 76).
     const int size = dtype == LLMX_F32 ? 4 : 2, lanes = head_dim * size / 16;
     const bool wide = head_dim * size % 16 == 0 && (lanes == 8 || lanes == 16 || lanes == 32) && !((k_stride | v_stride) * size % 16) &&
                       !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)codes) & 15) && items < (1ll << 30);
     if (wide) {
-        const int each = items * lanes >= 148ll * 32 * 64 ? 4 : 1;
+        const int each = items * lanes >= 148ll * 32 * 64 ? 2 : 1;
         const long long per = (long long)WARPS * (32 / lanes) * each;
 #define LLMX_QUANTIZE(T, LANES, EACH)                                                                                                  \
     launch_kernel(quantize_wide_kernel<T, LANES, EACH>, dim3((unsigned)((items + per - 1) / per)), dim3(WARPS * 32), 0, stream, (const T*)k,  \
@@ -459,7 +462,7 @@ LLMX_EXPORT int llmx_quantize_kv(const void* k, long long k_stride, const void* 
                   (long long)pages * page_size)
 #define LLMX_QUANTIZE_EACH(T, LANES)                   \
     do {                                               \
-        if (each == 4) LLMX_QUANTIZE(T, LANES, 4);     \
+        if (each == 2) LLMX_QUANTIZE(T, LANES, 2);     \
         else LLMX_QUANTIZE(T, LANES, 1);               \
     } while (0)
         if (dtype == LLMX_F32) {
