@@ -27,8 +27,9 @@
 // Work is cut evenly as in the warp form, one block an SM, tiles of 128 keys.
 //
 // Measured with the kernel that adds up (32 heads over 8): trees of 16 tokens for 8 requests after 4,096 keys of eight bits 52.5 us, one of 63 after
-// 8,191 of bfloat16 46, decoding 8 x 8,192 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows takes a unit some 3,500 clocks: 1,000 until its scores
-// are there, 600 to read them, 730 for exponentials and weights, 500 to store these; the tensor pipe is 8 % busy.
+// 8,191 of bfloat16 46, decoding 8 x 8,192 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows takes 3,300 clocks: 500 until a unit
+// has begun, 650 to read scores, 800 for exponentials and weights, 1,000 to store these; the tensor pipe is 8 % busy, and two softmax warps a
+// scheduler are what registers allow (four units of 16 rows, 96 registers a thread: 57 and 52 us).
 #pragma once
 #include "attention_pages_mma.cuh"
 #include "attn_common.cuh"
