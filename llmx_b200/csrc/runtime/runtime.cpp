@@ -465,7 +465,9 @@ int pages_attention(Ctx& c, llmx_pages_call p) {
         few(p.max_rows);
         return c.status;
     }
-    const int rows_few = most_pairs / ratio;
+    // One request's rows are the prompt kernel's whatever their number, which only the device knows (`max_rows` bounds it): there is nothing
+    // else for the few-row form to do, and to launch it besides would take 5 us of every prompt.
+    const int rows_few = p.requests == 1 ? 0 : most_pairs / ratio;
     const long long most = p.window > 0 ? std::min((long long)p.max_context, (long long)p.window + p.max_rows + 128) : p.max_context;
     long long capacity = (long long)p.requests * (most / EXPANDED_PAGE + 2);
     if (p.total_context > 0) capacity = std::min(capacity, p.total_context / EXPANDED_PAGE + 2ll * p.requests);
@@ -492,7 +494,7 @@ int pages_attention(Ctx& c, llmx_pages_call p) {
     CALL(c, llmx_attn_prefill_tc, splits > 1 ? 2 : 1, (const void*)map, p.q, p.out, p.total_rows, (const int*)list, p.requests, p.row_start,
          (const int*)count, p.history, (const int*)table, stride, p.heads, p.kv_heads, p.head_dim, EXPANDED_PAGE, p.window, p.scale, p.max_rows, tiles,
          splits, partial, p.error_word, c.stream);
-    if (p.requests > 1) few(std::min(p.max_rows, rows_few));
+    if (rows_few > 0) few(std::min(p.max_rows, rows_few));
     return c.status;
 }
 }  // namespace
