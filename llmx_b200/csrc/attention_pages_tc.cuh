@@ -20,8 +20,9 @@
 //   warps 2 .. 9    two units of four warps: exponentials, weights to shared memory.  A tile takes a unit much longer than it takes to
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
 //                   tile's rows are R; their states meet at the item's end), or half of the rows each (2 R)
-// The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^8 of them has the unit
-// raise them, and its sums and outputs (in tensor memory) scaled.  Every wait is bounded; the softmax warps go on through their
+// The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^8 of them (or a sum's exponential
+// 2^100, where values are so small that its weight does not) has the unit raise them, and its sums and outputs (in tensor memory)
+// scaled.  Every wait is bounded; the softmax warps go on through their
 // barriers without waiting once one has run out.
 //
 // Work is cut evenly as in the warp form, one block an SM, tiles of 128 keys.
@@ -73,9 +74,10 @@ struct Shape {
     static constexpr int TMEM = U * U_COLS <= 64 ? 64 : U * U_COLS <= 128 ? 128 : U * U_COLS <= 256 ? 256 : 512;
     static constexpr int AT_WEIGHTS = STAGES * STAGE, AT_QUERIES = AT_WEIGHTS + (HALVES ? 1 : U) * WEIGHTS, AT_EXPONENTS = AT_QUERIES + Q_BUFFERS * (ROWS / R) * Q_BYTES;
     // What a unit's threads tell each other, in floats: minus the sum's reference, the weights' beside it, what raising scales the two by,
-    // what the item's end scales its outputs and the other unit's by, 2^(the second) [R]; maxima and sums of warps [2][4][R].
-    static constexpr int UNIT_FLOATS = 7 * R + 2 * UNIT_WARPS * R;
-    static constexpr float LIMIT = EIGHT ? 256.0f : 0x1p60f;
+    // what the item's end scales its outputs and the other unit's by, 2^(the second) [R]; maxima and sums of warps [2][4][R]; the least
+    // 2^(the second) (and three unused).
+    static constexpr int UNIT_FLOATS = 7 * R + 2 * UNIT_WARPS * R + 4;
+    static constexpr float LIMIT = EIGHT ? 256.0f : 0x1p60f, SUM_LIMIT = 0x1p100f;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
     // What the queries' warp tells, of an item's rows: factors, positions, rows of the output (-1: none).
     static constexpr int AT_ROWS = AT_FLOATS + U * UNIT_FLOATS * 4;
@@ -119,6 +121,11 @@ __device__ __forceinline__ bool is_done(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ float warp_most(float v) {            // NaN aside
     float r;
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_least(float v) {
+    float r;
+    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
 // A barrier of a unit's threads; true for all if it is for one.
@@ -463,7 +470,8 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
         const uint32_t s_at = tmem + unit * S::U_COLS + lanes, o_at = s_at + 2 * S::S_COLS;
         float* shared = reinterpret_cast<float*>(smem + S::AT_FLOATS) + unit * S::UNIT_FLOATS;
         float *minus_peak = shared, *shift = shared + R, *fade_sum = shared + 2 * R, *fade_o = shared + 3 * R, *own_scale = shared + 4 * R,
-              *given_scale = shared + 5 * R, *power = shared + 6 * R, *warp_peak = shared + 7 * R, *warp_top = warp_peak + UNIT_WARPS * R;             // [4][R]
+              *given_scale = shared + 5 * R, *power = shared + 6 * R, *warp_peak = shared + 7 * R, *warp_top = warp_peak + UNIT_WARPS * R,             // [4][R]
+              *least_power = warp_top + UNIT_WARPS * R;
         float* strays = reinterpret_cast<float*>(smem + S::AT_STRAY) + unit * R * D;
         const uint32_t live_at = tc::smem_u32((const void*)live), rows_at = tc::smem_u32(shared), exponents_at = tc::smem_u32(smem + S::AT_EXPONENTS);
         const uint32_t weights_at = tc::smem_u32(smem + S::AT_WEIGHTS + (S::HALVES ? 0 : unit * S::WEIGHTS)) + key * 128;
@@ -612,7 +620,12 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 };
                 bool raise = opening;
                 if (!opening) {
-                    raise = unit_any(unit, weights() > S::LIMIT);
+                    bool over = weights() > S::LIMIT;
+                    // (Weights up to the limit are of exponentials up to the sums' wherever their factor is no less than the limits' ratio.)
+                    if (EIGHT && v_power * *least_power < S::LIMIT / S::SUM_LIMIT)
+#pragma unroll
+                        for (int n = 0; n < R; ++n) over |= x[n] > S::SUM_LIMIT;
+                    raise = unit_any(unit, over);
                     if (raise) scores(true);
                 }
                 if (raise) {
@@ -633,6 +646,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                         fade_sum[n] = exp2_fast(old - now);
                         fade_o[n] = EIGHT ? exp2_fast(top_old - top_now) : fade_sum[n];
                         minus_peak[n] = -now, shift[n] = now - top_now, power[n] = exp2_fast(now - top_now);
+                        if constexpr (EIGHT) {
+                            static_assert(R == 32, "one warp has a unit's rows");
+                            const float least = warp_least(power[n]);
+                            if (lane == 0) *least_power = least;
+                        }
                     }
                     unit_barrier(unit);
 #pragma unroll

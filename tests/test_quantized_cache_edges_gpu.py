@@ -1,12 +1,13 @@
-"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts.  Tolerances count the
-roundings that test_quantized_cache_gpu.py names."""
+"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts, scores
+and values far apart.  Tolerances count the roundings that test_quantized_cache_gpu.py names."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from llmx_b200 import ops
-from test_quantized_cache_gpu import BF16, DEV, Case, gpu
+from test_quantized_cache_gpu import BF16, DEV, F32, Case, gpu, quantized
 
 
 def close(c, got, r, weight_step, least, window=None):
@@ -64,3 +65,41 @@ def test_one_request_recorded_at_the_bound_and_replayed_with_fewer_rows(window):
         assert bool((out[n:] == 7.0).all())
         c.requests = [(n, h)]
         close(c, out.double().cpu(), 0, 2.0 ** -8, 0.0, window)
+
+
+# ---- scores and values far apart ----------------------------------------------------------------------------------------------------------
+# Heads of 64 and 128, queries of both types, up to 16, 32 and more (row, head) pairs (those of bfloat16 over heads of 128 by tcgen05), many rows.
+FORMS = [(BF16, 4, 2, 128, 1), (BF16, 8, 1, 128, 3), (BF16, 8, 2, 128, 20), (BF16, 4, 2, 64, 3), (F32, 4, 2, 128, 2), (F32, 4, 2, 64, 30), (BF16, 8, 2, 128, 90),
+         (BF16, 6, 3, 96, 3)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS[:6])
+@pytest.mark.parametrize("at", [40, 200])
+@pytest.mark.parametrize("apart", [60, 104])
+def test_scores_that_rise_where_values_fall(dtype, heads, g, dim, n, at, apart):
+    """Keys from `at` on have scores higher by `apart` (to base 2) and values smaller by as many powers: what they weigh together is
+    much alike, and the sums of weights are not."""
+    c = Case([(n, 500)], heads, g, dim, 16, dtype, seed=27, spread=0.0)
+    c.scale = 1.0
+    c.q.zero_()
+    c.q.view(-1, heads, dim)[:, :, 0] = 1.0
+    codes, b = c.cache.codes.view(torch.uint8), c.cache.exponents
+    # A key's first value is its score: eighths around nought, from `at` on eights up to what `apart` is to base e.
+    steps = round(apart * math.log(2) / 8.0)
+    t = torch.arange(n + 500)
+    page, place = c.tables[0].long()[t // 16], t % 16
+    key = torch.zeros(len(t), dim)
+    key[:, 0] = torch.randn(len(t), generator=torch.Generator().manual_seed(3)).mul(4).round().clamp(-7, 7) / 8
+    key[at:, 0] = 8.0 * steps
+    values, e = quantized(key.double().numpy())
+    raw = torch.from_numpy(values).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    low = round(apart / 2)
+    for head in range(g):
+        codes[page.to(DEV), 0, head, place.to(DEV)] = raw.to(DEV)
+        b[page.to(DEV), 0, head, place.to(DEV)] = torch.from_numpy(e).to(torch.uint8).to(DEV)
+        c.values[page, 0, head, place] = torch.from_numpy(values * np.exp2(e[:, None] - 127.0))
+        for part, by in ((t < at, low), (t >= at, -low)):
+            b[page[part].to(DEV), 1, head, place[part].to(DEV)] = (b[page[part].to(DEV), 1, head, place[part].to(DEV)].int() + by).to(torch.uint8)
+            c.values[page[part], 1, head, place[part]] *= 2.0 ** by
+    c.check()
