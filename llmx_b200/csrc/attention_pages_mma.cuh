@@ -14,7 +14,8 @@
 // is exact that is not 2^-28 of the row's largest; a key's power of two multiplies its finished score.  A value's power joins its
 // key's score instead, before the exponential: with s the scores and n the values' exponents (both to base 2)
 //     w = 2^(s + n - max (s + n)),   o = sum w code / sum 2^(s - max s) * 2^(max (s + n) - max s),
-// so that weights fit halves whatever the values' sizes, with both maxima and the sum in 32 bits.  Queries in
+// so that weights fit halves whatever the values' sizes, with both maxima and the sum in 32 bits.  A row of zeros, whose power is 1, would
+// set that maximum and leave small values no bits: it counts with 2^-127, as a page that is not there.  Queries in
 // 32 bits, and their weights, are two halves each.  Over bfloat16 pages queries, keys, values and weights are bfloat16.
 //
 // Measured with the kernel that adds up (32 heads of 128 over 8, bfloat16 queries): 8 x 8,192 keys 32 us, 4.2 TB/s (33 alone and cold: 245 registers,
@@ -143,6 +144,18 @@ __device__ __forceinline__ float4 finished(float4 acc, float top, float peak, fl
     if (sum == 0.0f) return make_float4(0.f, 0.f, 0.f, 0.f);
     const float f = (EIGHT ? exp2f(top - peak) : 1.0f) / sum;
     return make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+}
+
+// Which of a stage's rows, a lane each, at `at` are zeros (of either sign) throughout.
+template <int ROW>
+__device__ __forceinline__ unsigned rows_of_zeros(uint32_t at) {
+    uint32_t any = 0;
+#pragma unroll 1
+    for (int piece = 0; piece < ROW / 16; ++piece) {
+        const uint4 v = read16(at + place<ROW>(threadIdx.x & 31, piece));
+        any |= v.x | v.y | v.z | v.w;
+    }
+    return __ballot_sync(0xffffffffu, (any & 0x7F7F7F7Fu) == 0);
 }
 
 // bfloat16 values that are no numbers, of keys that not every row sees: their products are added one by one for the rows that do, and
@@ -503,10 +516,22 @@ few_rows_kernel(const QT* __restrict__ q, const uint8_t* __restrict__ cache, con
                         w[n >> 1][2 * u + (n & 1)] = fmaf(z, factor[u], v);
                     }
                 }
-                if (__any_sync(0xffffffffu, __vcmpeq4(vb[0], 0xffffffffu) | __vcmpeq4(vb[1], 0xffffffffu)))
+                // Values that have the byte of a row of zeros, 127, or of one that is no numbers, 255.
+                if (__any_sync(0xffffffffu, __vcmpeq4(vb[0] | 0x80808080u, 0xffffffffu) | __vcmpeq4(vb[1] | 0x80808080u, 0xffffffffu))) {
+                    const unsigned zeros = rows_of_zeros<S::ROW>(stage + S::PLANE) >> (8 * c);
 #pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        if ((vb[n >> 2] >> (8 * (n & 3)) & 255u) == e4m3::NOT_NUMBERS) w[n >> 1][n & 1] = w[n >> 1][2 + (n & 1)] = NAN;
+                    for (int n = 0; n < 8; ++n) {
+                        const unsigned byte = vb[n >> 2] >> (8 * (n & 3)) & 255u;
+                        const bool nothing = byte == 127u && (zeros >> n & 1u);
+                        if (nothing) vb[n >> 2] &= ~(255u << (8 * (n & 3)));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            float& x = w[n >> 1][2 * u + (n & 1)];
+                            if (byte == e4m3::NOT_NUMBERS) x = NAN;
+                            else if (nothing) x = fmaf(s[n >> 1][2 * u + (n & 1)], factor[u], -127.0f);
+                        }
+                    }
+                }
             }
             // Who sees what, where that is not everyone everything.
             const bool whole = t0 >= all_from && t0 + TILE <= all_to;

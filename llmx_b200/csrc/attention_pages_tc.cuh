@@ -11,7 +11,8 @@
 //
 // Eight bits on both sides: a query is two codes that add up to it, q = (q1 + q2 / 32) 2^e (bfloat16 has 8 bits, a code 4: exact down
 // to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 32 + w3 / 1024 (12 bits, down to 2^-20 of the largest): columns of their
-// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two belongs to its key's weight.
+// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two belongs to its key's weight; a row of zeros and a page
+// that is not there count with 2^-126.
 //
 //   warps 0, 10     page lookups and copies, STAGES tiles ahead, every other tile each: 16 keys and their values a copy (a warp issues
 //                   one in some 100 clocks, which by itself would be less than memory gives)
@@ -21,7 +22,7 @@
 //                   copy, most of it in waits for one thing after another, so the units have every other tile each (SHARED: a
 //                   tile's rows are R; their states meet at the item's end), or half of the rows each (2 R)
 // The maxima that the exponentials use are those of the first tile; a tile in which some weight would pass 2^8 of them (or a sum's exponential
-// 2^100, where values are so small that its weight does not) has the unit raise them, and its sums and outputs (in tensor memory)
+// 2^96, where values are so small that its weight does not) has the unit raise them, and its sums and outputs (in tensor memory)
 // scaled.  Every wait is bounded; the softmax warps go on through their
 // barriers without waiting once one has run out.
 //
@@ -47,10 +48,13 @@ constexpr int KEYS = 128, D = 128;
 constexpr int OPEN = 5;                 // tiles that an item's beginning and end take as long as
 constexpr int UNIT_WARPS = 4, LOADER = 10, QUERIES = 11;
 // The exponentials' references.  A weight is 1 at the maximum, and up to 2^8 before that is raised (what a code leaves of it is then 8 at
-// most, of which 32 is a code again); over bfloat16, which has the exponents, up to 2^60.  The sum's exponentials are 2^24 at the
+// most, of which 32 is a code again); over bfloat16, which has the exponents, up to 2^60.  The sum's exponentials are 2^64 at the
 // maximum: a weight is made from one by its value's power and its row's, which may be 2^120 apart, and must not be lost before.
-constexpr float ROOM = 24.0f;
+constexpr float ROOM = 64.0f;
 constexpr float NONE = -1.0e30f;        // a maximum of no keys
+// What values of nothing count as, to base 2, in the weights' reference: little enough to leave values their bits beside a key of zeros that
+// is 2^(126 - 60) times as heavy, and a row's power (up to 2^(126 - ROOM)) times a key's (up to 2^60) is within 32 bits.
+constexpr int NOTHING = -126;
 enum : int { ERR_PAGES_PRODUCER = 501, ERR_PAGES_MMA = 502, ERR_PAGES_SOFTMAX = 503 };
 
 template <bool EIGHT, bool SHARED, int R>
@@ -77,7 +81,7 @@ struct Shape {
     // what the item's end scales its outputs and the other unit's by, 2^(the second) [R]; maxima and sums of warps [2][4][R]; the least
     // 2^(the second) (and three unused).
     static constexpr int UNIT_FLOATS = 7 * R + 2 * UNIT_WARPS * R + 4;
-    static constexpr float LIMIT = EIGHT ? 256.0f : 0x1p60f, SUM_LIMIT = 0x1p100f;
+    static constexpr float LIMIT = EIGHT ? 256.0f : 0x1p60f, SUM_LIMIT = 0x1p96f;
     static constexpr int AT_FLOATS = AT_EXPONENTS + STAGES * 256;
     // What the queries' warp tells, of an item's rows: factors, positions, rows of the output (-1: none).
     static constexpr int AT_ROWS = AT_FLOATS + U * UNIT_FLOATS * 4;
@@ -527,10 +531,21 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                 if constexpr (EIGHT) {
                     const uint32_t b = exponents_at + stage * 256 + key;
                     const unsigned kb = shared_byte(b), vb = shared_byte(b + KEYS);
+                    bool nothing = dead;
+                    if (!dead && vb == 127) {                    // the byte of a row of zeros
+                        unsigned any = 0;
+#pragma unroll 1
+                        for (int n = 0; n < 8; ++n) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(smem + stage * S::STAGE + (key >> 3) * 2048 + 1024 + (key & 7) * 128 + n * 16);
+                            any |= v.x | v.y | v.z | v.w;
+                        }
+                        nothing = !(any & 0x7F7F7F7Fu);
+                    }
                     // A value that is no number makes its key none: NaN for the rows that see it.
                     k_power = dead ? 0.0f : vb == e4m3::NOT_NUMBERS ? NAN : e4m3::up(kb);
-                    v_power = dead || vb == e4m3::NOT_NUMBERS ? 1.0f : e4m3::up(vb);
-                    v_exponent = dead || vb == e4m3::NOT_NUMBERS ? 0.0f : (float)((int)vb - 127);
+                    const int n = nothing ? NOTHING : vb == e4m3::NOT_NUMBERS ? 0 : (int)vb - 127;
+                    v_power = __uint_as_float((unsigned)(n + 127) << 23);
+                    v_exponent = (float)n;
                 }
                 const bool whole = t0 >= all_from && t0 + KEYS <= all_to && runs == 0xff;
                 const bool in_reach = t >= sg.rq.low && t < sg.rq.end;

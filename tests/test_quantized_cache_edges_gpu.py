@@ -1,5 +1,5 @@
-"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts, scores
-and values far apart.  Tolerances count the roundings that test_quantized_cache_gpu.py names."""
+"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts, values of
+nothing beside small ones, scores and values far apart.  Tolerances count the roundings that test_quantized_cache_gpu.py names."""
 import math
 
 import numpy as np
@@ -7,7 +7,12 @@ import pytest
 import torch
 
 from llmx_b200 import ops
-from test_quantized_cache_gpu import BF16, DEV, F32, Case, gpu, quantized
+from test_quantized_cache_gpu import BF16, DEV, F32, Case, gpu, quantized, random_tree
+
+
+# Heads of 64 and 128, queries of both types, up to 16, 32 and more (row, head) pairs (those of bfloat16 over heads of 128 by tcgen05), many rows.
+FORMS = [(BF16, 4, 2, 128, 1), (BF16, 8, 1, 128, 3), (BF16, 8, 2, 128, 20), (BF16, 4, 2, 64, 3), (F32, 4, 2, 128, 2), (F32, 4, 2, 64, 30), (BF16, 8, 2, 128, 90),
+         (BF16, 6, 3, 96, 3)]
 
 
 def close(c, got, r, weight_step, least, window=None):
@@ -67,12 +72,69 @@ def test_one_request_recorded_at_the_bound_and_replayed_with_fewer_rows(window):
         close(c, out.double().cpu(), 0, 2.0 ** -8, 0.0, window)
 
 
+# ---- values of nothing beside small ones --------------------------------------------------------------------------------------------------
+def shift_values(c, by):
+    c.cache.exponents[:, 1] = (c.cache.exponents[:, 1].int() + by).to(torch.uint8)
+    c.values[:, 1] *= 2.0 ** by
+
+
+def clear_values(c, where, negative=False):
+    """Zeros (of either sign, as a row of them is written) as the values of slots `where` [pages, page], all heads."""
+    at = where[:, None, :].expand(-1, c.g, -1)
+    codes = c.cache.codes.view(torch.uint8)[:, 1]
+    codes[at.to(DEV)] = 0x80 if negative else 0
+    c.cache.exponents[:, 1][at.to(DEV)] = 127
+    c.values[:, 1][at] = 0.0
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+@pytest.mark.parametrize("by", [-8, -20, -38])
+@pytest.mark.parametrize("negative", [False, True])
+def test_values_that_are_zeros_leave_the_others_their_bits(dtype, heads, g, dim, n, by, negative):
+    c = Case([(n, 700), (1, 40)], heads, g, dim, 16, dtype, seed=23)
+    shift_values(c, by)
+    clear_values(c, torch.rand(c.pages, 16, generator=torch.Generator().manual_seed(1)) < 0.2, negative)
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+@pytest.mark.parametrize("by", [-8, -38])
+def test_pages_that_are_not_there_leave_the_others_their_bits(dtype, heads, g, dim, n, by):
+    c = Case([(n, 700), (1, 40)], heads, g, dim, 16, dtype, seed=24)
+    shift_values(c, by)
+    c.tables[0, 3], c.tables[0, 0], c.tables[0, 40] = -1, c.pages, -7
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+def test_tiles_of_zeros_before_values(dtype, heads, g, dim, n):
+    """The first 300 keys' values are zeros, and all of the second request's: zeros, whatever the scores."""
+    c = Case([(n, 700), (2, 40)], heads, g, dim, 16, dtype, seed=25)
+    shift_values(c, -30)
+    where = torch.zeros(c.pages, 16, dtype=torch.bool)
+    for r, t in ((0, torch.arange(300)), (1, torch.arange(42))):
+        where[c.tables[r].long()[t // 16], t % 16] = True
+    clear_values(c, where)
+    got = c.run()
+    assert bool((got[n:] == 0).all())
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS[:6])
+def test_trees_over_values_that_are_zeros(dtype, heads, g, dim, n):
+    requests = [(n, 300), (5, 0), (2, 40)]
+    c = Case(requests, heads, g, dim, 16, dtype, seed=26)
+    c.tree = random_tree(requests, 26)
+    shift_values(c, -30)
+    clear_values(c, torch.rand(c.pages, 16, generator=torch.Generator().manual_seed(2)) < 0.3)
+    c.check()
+
+
 # ---- scores and values far apart ----------------------------------------------------------------------------------------------------------
-# Heads of 64 and 128, queries of both types, up to 16, 32 and more (row, head) pairs (those of bfloat16 over heads of 128 by tcgen05), many rows.
-FORMS = [(BF16, 4, 2, 128, 1), (BF16, 8, 1, 128, 3), (BF16, 8, 2, 128, 20), (BF16, 4, 2, 64, 3), (F32, 4, 2, 128, 2), (F32, 4, 2, 64, 30), (BF16, 8, 2, 128, 90),
-         (BF16, 6, 3, 96, 3)]
-
-
 @gpu
 @pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS[:6])
 @pytest.mark.parametrize("at", [40, 200])
