@@ -338,10 +338,11 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
 }
 
 constexpr int EXPANDED = 16, ROW_PIECES = 16;         // slots of an expanded page; pieces of eight of a head's 128 values
+constexpr int MOST_PAGES = (1 << 25) - 1;             // of a request (256 GB of one head's)
 
 // Requests' keys and values as bfloat16 pages of 16 slots, for a kernel that reads those: the requests of more than `rows_over` rows, one
-// after another without gaps, a block a page.  `out_table` names a request's pages, `out_count` has its rows (none for the requests
-// that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value (8,192 keys of 8 heads: 12 us).
+// after another without gaps, a block a page, as far as the pages reach (a request whose keys no longer fit is left out).  `out_table` names
+// a request's pages, `out_count` has its rows (none for the requests that are left out), `out_list` the requests.  Bound by the bytes: a byte read and two written for each value (8,192 keys of 8 heads: 12 us).
 // A value row that is no numbers comes as zeros with its key as NaN: the attention's mask then keeps it from the rows that do
 // not see it (a weight of zero would not), and makes NaN of those that do, as it has to.
 __global__ void __launch_bounds__(READERS)
@@ -362,15 +363,11 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
     __shared__ int owner, page_of_owner;
     if (threadIdx.x == 0) owner = -1;
     __syncthreads();
-    if (blockIdx.x == 0)
-        for (int r = threadIdx.x; r < requests; r += blockDim.x) {
-            out_list[r] = r;
-            out_count[r] = rows_of(r);
-        }
     if (threadIdx.x < 32) {
-        const int f = blockIdx.x;
+        // (Counts that overlap may claim more pages than there are: sums stay below 2^31.  The first block walks all requests, for their counts.)
+        const int f = blockIdx.x, capacity = gridDim.x;
         int before = 0;
-        for (int r0 = 0; r0 < requests && before <= f; r0 += 32) {
+        for (int r0 = 0; r0 < requests && (before <= f || f == 0); r0 += 32) {
             const int r = r0 + threadIdx.x;
             const int rows = r < requests ? rows_of(r) : 0;
             int n = 0, first = 0;
@@ -378,7 +375,7 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
                 const int keys = history[r] + rows;
                 // The reader starts at a whole stage of 128 keys.
                 first = window > 0 ? max(0, history[r] - window + 1) / 128 * (128 / EXPANDED) : 0;
-                n = max(0, min((keys + EXPANDED - 1) / EXPANDED, out_stride) - first);
+                n = min(max(0, min((keys + EXPANDED - 1) / EXPANDED, out_stride) - first), MOST_PAGES);
             }
             int upto = n;
 #pragma unroll
@@ -386,8 +383,11 @@ expand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exp
                 const int x = __shfl_up_sync(0xffffffffu, upto, o);
                 if ((int)threadIdx.x >= o) upto += x;
             }
-            if (f >= before + upto - n && f < before + upto) owner = r, page_of_owner = first + f - (before + upto - n);
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            const int end = before + upto, begin = end - n;
+            const bool fits = end <= capacity;
+            if (fits && f >= begin && f < end) owner = r, page_of_owner = first + f - begin;
+            if (f == 0 && r < requests) out_list[r] = r, out_count[r] = fits ? rows : 0;
+            before = min(before + __shfl_sync(0xffffffffu, upto, 31), 32 * MOST_PAGES);
         }
     }
     __syncthreads();

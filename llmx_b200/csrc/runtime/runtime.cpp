@@ -469,8 +469,10 @@ int pages_attention(Ctx& c, llmx_pages_call p) {
     // else for the few-row form to do, and to launch it besides would take 5 us of every prompt.
     const int rows_few = p.requests == 1 ? 0 : most_pairs / ratio;
     const long long most = p.window > 0 ? std::min((long long)p.max_context, (long long)p.window + p.max_rows + 128) : p.max_context;
-    long long capacity = (long long)p.requests * (most / EXPANDED_PAGE + 2);
-    if (p.total_context > 0) capacity = std::min(capacity, p.total_context / EXPANDED_PAGE + 2ll * p.requests);
+    // Requests of more than rows_few rows, each with rows of its own: no more of them than the rows make, and one whose last rows lie beyond.
+    const long long prompts = std::min<long long>(p.requests, p.total_rows / (rows_few + 1) + 1);
+    long long capacity = prompts * (most / EXPANDED_PAGE + 2);
+    if (p.total_context > 0) capacity = std::min(capacity, p.total_context / EXPANDED_PAGE + 2 * prompts);
     if (capacity >= (1ll << 31)) return c.status = fail(LLMX_RT_ERR_BAD_ARGUMENT, "attention over pages: more keys than 2^31 pages hold");
     const int stride = p.max_context / EXPANDED_PAGE + 9;
     void* expanded = c.alloc((size_t)capacity * 2 * p.kv_heads * EXPANDED_PAGE * p.head_dim * 2);

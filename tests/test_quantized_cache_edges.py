@@ -1,0 +1,37 @@
+"""What the host decides for calls at the edges of attention over pages (no GPU): the workspace, calls that are refused."""
+import pytest
+import torch
+
+from llmx_b200 import ops, runtime
+
+
+def call(requests=1, rows=1, max_rows=1, max_context=64, heads=32, kv_heads=8, dim=128, page=16, window=0, q=ops.BF16, cache=ops.E4M3, tree_words=0, pages=4096,
+         total_context=0):
+    """A call of the sizes named, its pointers aligned and of nothing."""
+    pointers = [256] * 8 + [256 if tree_words else 0]
+    return ops._CALL.pack(*pointers, q, cache, -(-max_context // page), tree_words, requests, rows, max_rows, max_context, total_context, pages, heads, kv_heads,
+                          dim, page, window, 0, 1.0, 0, 0, 0, 0)
+
+
+def room(**sizes):
+    packed = call(**sizes)
+    return runtime.sized(lambda: runtime.lib().llmx_pages_workspace(packed))
+
+
+EXPANDED = 2 * 8 * 16 * 128 * 2          # bytes of an expanded page of 8 heads
+
+
+# ---- prompts' pages -----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("context", [32768, 131072])
+def test_room_for_prompts_goes_by_the_rows_that_there_are(context):
+    """One prompt among 63 requests of a row each: requests of more than 16 rows are expanded (64 pairs of 4 heads), and 363 rows are
+    at most 21 of those."""
+    most = room(requests=64, rows=363, max_rows=300, max_context=context)
+    assert 21 * (context // 16) * EXPANDED <= most <= 22 * (context // 16 + 32) * EXPANDED
+
+
+def test_room_for_prompts_alone_is_theirs():
+    assert room(requests=4, rows=4 * 512, max_rows=512, max_context=8192) >= 4 * 512 * EXPANDED
+    one = room(requests=1, rows=512, max_rows=512, max_context=8192)
+    assert 512 * EXPANDED <= one <= 600 * EXPANDED + 32 * 512 * 132 * 4 * 8
+    assert room(requests=1, rows=512, max_rows=512, max_context=131072, window=1024) <= 200 * EXPANDED + 32 * 512 * 132 * 4 * 8

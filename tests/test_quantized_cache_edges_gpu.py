@@ -1,5 +1,5 @@
-"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts, values of
-nothing beside small ones, scores and values far apart.  Tolerances count the roundings that test_quantized_cache_gpu.py names."""
+"""Calls at the edges of what the operators of the cache in eight bits allow: bounds that lie above the counts, as many
+prompts as there can be, values of nothing beside small ones, scores and values far apart.  Tolerances count the roundings that test_quantized_cache_gpu.py names."""
 import math
 
 import numpy as np
@@ -70,6 +70,25 @@ def test_one_request_recorded_at_the_bound_and_replayed_with_fewer_rows(window):
         assert bool((out[n:] == 7.0).all())
         c.requests = [(n, h)]
         close(c, out.double().cpu(), 0, 2.0 ** -8, 0.0, window)
+
+
+# ---- as many prompts as the rows make -----------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("requests", [[(17, 400)] * 20, [(300, 500)] + [(1, 700)] * 40, [(1, 90)] * 20 + [(17, 30), (0, 9), (19, 600)], [(16, 100)] * 20 + [(17, 0)] * 3])
+@pytest.mark.parametrize("window", [None, 70])
+def test_prompts_of_as_few_rows_as_are_expanded(requests, window):
+    """64 pairs, of 4 heads, are the few-row form's; 17 rows are a prompt, and the room is for as many of them as there are rows."""
+    Case(requests, 8, 2, 128, 16, BF16, seed=31, spare_rows=0).check(window)
+
+
+@gpu
+def test_prompts_that_name_the_same_rows():
+    """More of them than their rows make: what does not fit is left out, and the rows are those of one that does."""
+    c = Case([(70, 400)], 8, 2, 128, 16, BF16, seed=32, spare_rows=0)
+    q, out = c.q.to(DEV), torch.full_like(c.q.to(DEV), 7.0)
+    start, count, history, tables = (x.repeat_interleave(3, dim=0) for x in c.device())
+    ops.attention_quantized(q, c.cache, out, start, count, history, tables, c.heads, c.g, c.dim, None, c.scale, 70, 470)
+    close(c, out.double().cpu(), 0, 2.0 ** -8, 0.0)
 
 
 # ---- values of nothing beside small ones --------------------------------------------------------------------------------------------------
