@@ -1,4 +1,4 @@
-// Softmax attention of requests' new rows over pages, in any of the cache's types, under a window or a tree's bits.
+// Softmax attention of requests' new rows over pages: of eight bits, under a window or a tree's bits; of bfloat16 and float32 under a tree's.
 //
 // Request r brings row_count[r] rows, row_start[r] the first, after history[r] keys that the cache holds already; the rows' own keys
 // and values follow them there.  Row i sees the keys t with
@@ -236,6 +236,7 @@ LLMX_EXPORT int llmx_attention_pages(const void* q, int q_dtype, const void* cac
     Rows a = {row_start, row_count, history, tables, table_stride, total_rows, pages, page_size, window, (const unsigned*)tree, tree_words,
                     ((1u << 31) + (unsigned)max(page_size / 16, 1) - 1) / (unsigned)max(page_size / 16, 1), 0, max_rows};
     if (!(scale > 0.0f)) return LLMX_ERR_BAD_ARGUMENT;
+    if (!tree && cache_dtype != LLMX_E4M3) return LLMX_ERR_UNSUPPORTED;      // (the forms over bfloat16 look among drafted tokens alone for infinities)
     const FewPlan p = few_plan(q_dtype, cache_dtype, requests, max_rows, max_context, heads, kv_heads, head_dim, page_size, window, general);
     a.max_tiles = p.max_tiles;
     if (p.rows && pages > 0 && (long long)total_rows * heads < (1ll << 31) && !(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)exponents) & 15) &&

@@ -1,5 +1,5 @@
-// Attention over pages on the tensor cores of tcgen05: few rows a request, heads of 128; all of bfloat16 pages (decoding, drafts), and
-// over eight bits more than 32 (row, head) pairs (trees of drafts).
+// Attention over pages on the tensor cores of tcgen05: few rows a request, heads of 128; trees of drafted tokens over bfloat16 pages, and
+// over eight bits more than 32 (row, head) pairs.
 //
 // The warp form (attention_pages_mma.cuh) spends its time on turning codes into halves, again for every 16 rows, and moving them through
 // registers.  Here neither keys nor values pass through registers at all: TMA brings 128 keys of a head to shared memory as they lie in their pages, and the
@@ -29,7 +29,7 @@
 // Work is cut evenly as in the warp form, one block an SM, tiles of 128 keys.
 //
 // Measured with the kernel that adds up (32 heads over 8): trees of 16 tokens for 8 requests after 4,096 keys of eight bits 52.5 us, one of 63 after
-// 8,191 of bfloat16 46, decoding 8 x 8,192 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows takes 3,300 clocks: 500 until a unit
+// 8,191 of bfloat16 46, one token each after 8 x 8,191 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows takes 3,300 clocks: 500 until a unit
 // has begun, 650 to read scores, 800 for exponentials and weights, 1,000 to store these; the tensor pipe is 8 % busy, and two softmax warps a
 // scheduler are what registers allow (four units of 16 rows, 96 registers a thread: 57 and 52 us).
 #pragma once

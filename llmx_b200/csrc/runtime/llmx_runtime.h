@@ -210,9 +210,10 @@ int llmx_decode_from_qkv(const llmx_step*, const float* qkv, int entry, const fl
                          float eps, const float* cos, const float* sin, int rot_half, void* out, int heads, int kv_heads,
                          int head_dim, int window, float scale);
 
-// Attention of requests' rows over pages of any cache type (llmx_attention_pages, attention_pages.cu, has the formulas): over keys and
-// values in eight bits, and for rows that are drafted tokens.  Requests of many rows over eight bits (heads of 128, bfloat16
-// queries, no tree) have their pages expanded and run the tcgen05 kernel.
+// Attention of requests' rows over pages (llmx_attention_pages, attention_pages.cu, has the formulas): over keys and values in eight bits,
+// and over any cache type for rows that are drafted tokens (other calls over bfloat16 or float32 are refused: llmx_paged_attention
+// takes them).  Requests of many rows over eight bits (heads of 128, bfloat16 queries, no tree) have their pages expanded and run the
+// tcgen05 kernel.
 typedef struct llmx_pages_call {
     const void* q;                    // [total_rows, heads, head_dim] of q_dtype, like out
     void* out;

@@ -1510,6 +1510,8 @@ bool good_call(const llmx_pages_call* p) {
     return p && p->requests >= 0 && p->total_rows >= 0 && p->max_rows >= 0 && p->max_context >= 0 && p->heads > 0 && p->kv_heads > 0 &&
            p->heads % p->kv_heads == 0 && p->head_dim > 0 && p->page_size > 0 && p->table_stride >= 0 && p->window >= 0 && p->scale > 0.0f;
 }
+// Without a tree only pages of eight bits: the forms over bfloat16 pages look among drafted tokens alone for values that are no numbers.
+bool has_form(const llmx_pages_call* p) { return p->cache_dtype == LLMX_DT_E4M3 || p->tree; }
 llmx_step step_of(const llmx_pages_call& p) {
     llmx_step s = {};
     s.workspace = p.workspace, s.workspace_bytes = p.workspace_bytes, s.error_word = p.error_word, s.stream = p.stream;
@@ -1517,7 +1519,7 @@ llmx_step step_of(const llmx_pages_call& p) {
 }
 }  // namespace
 LLMX_API size_t llmx_pages_workspace(const llmx_pages_call* p) {
-    if (!good_call(p)) return 0;
+    if (!good_call(p) || !has_form(p)) return 0;
     const llmx_step s = step_of(*p);
     Ctx c(&s, true);
     pages_attention(c, *p);
@@ -1525,6 +1527,7 @@ LLMX_API size_t llmx_pages_workspace(const llmx_pages_call* p) {
 }
 LLMX_API int llmx_pages_attention(const llmx_pages_call* p) {
     if (!good_call(p)) return fail(LLMX_RT_ERR_BAD_ARGUMENT, "attention over pages: sizes that do not fit each other");
+    if (!has_form(p)) return fail(LLMX_RT_ERR_UNSUPPORTED, "attention over pages: bfloat16 and float32 pages are attended under a tree alone");
     const llmx_step s = step_of(*p);
     Ctx c(&s, false);
     pages_attention(c, *p);

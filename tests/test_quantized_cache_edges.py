@@ -1,6 +1,5 @@
 """What the host decides for calls at the edges of attention over pages (no GPU): the workspace, calls that are refused."""
 import pytest
-import torch
 
 from llmx_b200 import ops, runtime
 
@@ -35,3 +34,13 @@ def test_room_for_prompts_alone_is_theirs():
     one = room(requests=1, rows=512, max_rows=512, max_context=8192)
     assert 512 * EXPANDED <= one <= 600 * EXPANDED + 32 * 512 * 132 * 4 * 8
     assert room(requests=1, rows=512, max_rows=512, max_context=131072, window=1024) <= 200 * EXPANDED + 32 * 512 * 132 * 4 * 8
+
+
+# ---- calls without a form -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cache", [ops.BF16, ops.F32])
+@pytest.mark.parametrize("window", [0, 70])
+def test_pages_of_other_types_are_attended_under_a_tree_alone(cache, window):
+    packed = call(requests=2, rows=20, max_rows=10, cache=cache, window=window)
+    assert runtime.lib().llmx_pages_attention(packed) != 0 and "under a tree alone" in runtime.last_error()
+    assert runtime.lib().llmx_pages_workspace(packed) == 0
+    assert cache == ops.F32 or room(requests=2, rows=20, max_rows=10, cache=cache, tree_words=1) > 0
