@@ -184,3 +184,98 @@ def test_scores_that_rise_where_values_fall(dtype, heads, g, dim, n, at, apart):
             b[page[part].to(DEV), 1, head, place[part].to(DEV)] = (b[page[part].to(DEV), 1, head, place[part].to(DEV)].int() + by).to(torch.uint8)
             c.values[page[part], 1, head, place[part]] *= 2.0 ** by
     c.check()
+
+
+# ---- sizes beside the usual ones ----------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("heads, g, dim", [(8, 2, 128), (4, 2, 64), (5, 1, 64)])
+@pytest.mark.parametrize("requests", [[(300, 0)], [(300, 200), (1, 90), (40, 33)]])
+@pytest.mark.parametrize("window", [None, 70])
+def test_prompts_with_queries_of_32_bits(heads, g, dim, requests, window):
+    Case(requests, heads, g, dim, 16, F32, seed=41).check(window)
+
+
+@gpu
+@pytest.mark.parametrize("page", [48, 112, 512, 528])
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS[:7])
+def test_pages_of_other_sizes(page, dtype, heads, g, dim, n):
+    Case([(n, 1100), (1, 3), (2, page)], heads, g, dim, page, dtype, seed=page).check()
+
+
+@gpu
+@pytest.mark.parametrize("page", [48, 512])
+@pytest.mark.parametrize("heads, g, dim, n", [(8, 2, 128, 1), (8, 2, 128, 6), (8, 2, 128, 20), (4, 2, 64, 9)])
+def test_trees_over_bfloat16_pages_of_other_sizes(page, heads, g, dim, n):
+    requests = [(n, 1100), (3, 0), (2, page)]
+    c = Case(requests, heads, g, dim, page, BF16, "bfloat16", seed=page)
+    c.tree = random_tree(requests, page, words=3)
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+@pytest.mark.parametrize("tree", [False, True])
+def test_bounds_far_above_what_there_is(dtype, heads, g, dim, n, tree):
+    """As a program says them that records one call for all that may come."""
+    class Loose(Case):
+        def bounds(self):
+            return 150, 20000
+    c = Loose([(n, 300), (0, 9), (1, 40), (2, 0)], heads, g, dim, 16, dtype, seed=42, spare_rows=200)
+    if tree:
+        c.tree = np.concatenate([random_tree(c.requests, 42, words=5), np.zeros((198, 5), dtype=np.int32)])
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 3])
+def test_many_requests(n):
+    """More than a warp's lanes, of all lengths, none among them."""
+    gen = np.random.default_rng(43)
+    requests = [(int(gen.integers(0, n + 1)), int(gen.integers(0, 90))) for _ in range(300)]
+    Case(requests, 4, 2, 128, 16, BF16, seed=43).check()
+    Case(requests, 4, 2, 64, 16, F32, seed=44).check()
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    cases = [Case([(1, 3000), (2, 700)], 8, 2, 128, 16, BF16, seed=45), Case([(20, 900)], 8, 2, 128, 16, BF16, seed=46), Case([(200, 700)], 8, 2, 128, 16, BF16, seed=47),
+             Case([(2, 900)], 4, 2, 64, 16, F32, seed=48)]
+    wants = [c.run() for c in cases]
+    ready = [(c, c.q.to(DEV), c.device()) for c in cases]
+    outs = [torch.full_like(q, 7.0) for _ in range(2) for _, q, _ in ready]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i in range(len(outs)):
+            c, q, rows = ready[i % len(ready)]
+            with torch.cuda.stream(streams[(i + i // len(ready)) % 2]):
+                ops.attention_quantized(q, c.cache, outs[i], *rows, c.heads, c.g, c.dim, None, c.scale, *c.bounds())
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        c = cases[i % len(cases)]
+        assert torch.equal(out[:c.rows].double().cpu(), wants[i % len(cases)])
+
+
+# ---- an invariant engine ------------------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("name", ["A", "D", "E"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_an_invariant_engine_over_eight_bits_gives_a_row_the_same_bits_in_any_batch(model_dirs, name, dtype):
+    import helpers
+    from configs import CONFIGS
+    from llmx_b200.engine import Engine, EngineOptions
+    d16, d32, page = model_dirs[name]
+    requests = {f"i{i}": helpers.random_ids(CONFIGS[name][0]["vocab_size"], n, seed=80 + i) for i, n in enumerate([70, 9, 40, 33, 81])}
+    base = None
+    for make in (helpers.trace_whole, helpers.trace_tail_decoded, helpers.trace_portions, helpers.trace_mixed):
+        steps = make(requests)
+        engine = Engine.from_dir(d32 if dtype == "float32" else d16,
+                                 EngineOptions(dtype=dtype, kv_dtype="float8_e4m3", kv_tokens=helpers.tokens_needed(steps), page_size=page, max_requests=4,
+                                               invariant=True))
+        got = helpers.run_trace(engine, steps)
+        del engine
+        base = base or got
+        assert got.keys() == base.keys()
+        moved = [k for k in base if not np.array_equal(base[k], got[k])]
+        assert not moved, (make.__name__, len(moved), moved[:5])
