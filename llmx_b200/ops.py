@@ -1439,8 +1439,8 @@ def _attention_pages(what: str, q, cache, out, row_start, row_count, history, bl
         pointers = (q.data_ptr(), out.data_ptr(), stored.data_ptr(), cache.exponents.data_ptr() if eight else 0, row_start.data_ptr(),
                     row_count.data_ptr(), history.data_ptr(), block_tables.data_ptr(), 0 if tree is None else tree.data_ptr())
         lib = runtime.lib()
-        # The form, and with it the workspace, goes by sizes and by whether rows are read in 16-byte pieces.
-        key = (sizes, tree is None, (pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15)
+        # The form, and with it the workspace, goes by sizes and by what is read in 16-byte pieces: rows, and exponents (a prompt's are not).
+        key = (sizes, tree is None, (pointers[0] | pointers[1] | pointers[2]) & 15 == 0, pointers[3] & 15 == 0)
         room = _pages_rooms.get(key)
         if room is None:
             call = _CALL.pack(*pointers, *sizes, scale, 0, 0, error_word, stream)

@@ -15,6 +15,12 @@ FORMS = [(BF16, 4, 2, 128, 1), (BF16, 8, 1, 128, 3), (BF16, 8, 2, 128, 20), (BF1
          (BF16, 6, 3, 96, 3)]
 
 
+class Done(Case):
+    """A case whose outputs are there already."""
+    def run(self, window=None):
+        return self.done
+
+
 def close(c, got, r, weight_step, least, window=None):
     """Request r's rows of `got` (float64) against 64 bits: a weight's rounding is `weight_step` of it, and `least` of the largest product
     of a row and head for each key that it sees."""
@@ -279,3 +285,99 @@ def test_an_invariant_engine_over_eight_bits_gives_a_row_the_same_bits_in_any_ba
         assert got.keys() == base.keys()
         moved = [k for k in base if not np.array_equal(base[k], got[k])]
         assert not moved, (make.__name__, len(moved), moved[:5])
+
+
+# ---- places and rows anywhere -------------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+def test_a_cache_beyond_32_bits_of_bytes(dtype, heads, g, dim, n):
+    """The same pages at the far end of a cache of more than 2^32 bytes: the same bits; written there, and read back."""
+    c = Case([(n, 300), (1, 40)], heads, g, dim, 16, dtype, seed=51)
+    want = c.run()
+    pages = 2 ** 32 // (2 * g * 16 * dim) + c.pages + 5
+    far = pages - c.pages
+    large = ops.QuantizedPages.zeros(pages, g, 16, dim, DEV)
+    large.codes[far:], large.exponents[far:] = c.cache.codes, c.cache.exponents
+    small, c.cache = c.cache, large
+    tables = c.tables
+    c.tables = torch.where(tables >= 0, tables + far, tables)
+    assert torch.equal(c.run(), want)
+    ids = torch.tensor([pages - 1, far], dtype=torch.int32, device=DEV)
+    for t in (F32, BF16):
+        out = [torch.empty(2, 2, g, 16, dim, dtype=t, device=DEV) for _ in range(2)]
+        ops.dequantize_pages(large, ids, out[0])
+        ops.dequantize_pages(small, ids - far, out[1])
+        assert torch.equal(*out)
+    k, v = (torch.randn(40, g, dim, device=DEV) for _ in range(2))
+    slots = torch.randperm(c.pages * 16, device=DEV)[:40].int()
+    ops.quantize_kv(k, v, slots, small)
+    ops.quantize_kv(k, v, slots + far * 16, large)
+    assert torch.equal(large.codes[far:].view(torch.uint8), small.codes.view(torch.uint8)) and torch.equal(large.exponents[far:], small.exponents)
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+def test_storage_that_starts_anywhere(dtype, heads, g, dim, n):
+    """Calls of one size whose queries, outputs, codes and exponents begin off their 16 bytes, in turn."""
+    def moved(x, by):
+        raw = torch.empty(x.numel() * x.element_size() + 64, dtype=torch.uint8, device=DEV)
+        y = raw[by:by + x.numel() * x.element_size()].view(x.dtype).view(x.shape)
+        y.copy_(x)
+        return y
+
+    c = Done([(n, 300), (1, 40)], heads, g, dim, 16, dtype, seed=52, spare_rows=0)
+    codes, exponents = c.cache.codes, c.cache.exponents
+    for what in ("q", "out", "codes", "exponents", ""):
+        q, out = c.q.to(DEV), torch.zeros_like(c.q.to(DEV))
+        if what == "q":
+            q = moved(q, q.element_size())
+        if what == "out":
+            out = moved(out, out.element_size())
+        cache = ops.QuantizedPages(moved(codes.view(torch.uint8), 1).view(torch.float8_e4m3fn) if what == "codes" else codes,
+                                   moved(exponents, 1) if what == "exponents" else exponents)
+        ops.attention_quantized(q, cache, out, *c.device(), c.heads, c.g, c.dim, None, c.scale, *c.bounds())
+        c.done = out.double().cpu()
+        c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, heads, g, dim, n", FORMS)
+def test_rows_in_any_order_with_others_between(dtype, heads, g, dim, n):
+    c = Case([(n, 300), (2, 40), (0, 7), (1, 20)], heads, g, dim, 16, dtype, seed=53, spare_rows=0)
+    want = c.run()
+    starts, at = [0] * 4, 3
+    for r in (3, 1, 0, 2):
+        starts[r] = at
+        at += c.requests[r][0] + 2
+    q, out = torch.randn(at, heads * dim, device=DEV).to(dtype), torch.full((at, heads * dim), 7.0, dtype=dtype, device=DEV)
+    mine = torch.zeros(at, dtype=torch.bool)
+    for r, (rows, _) in enumerate(c.requests):
+        q[starts[r]:starts[r] + rows] = c.q[c.starts[r]:c.starts[r] + rows].to(DEV)
+        mine[starts[r]:starts[r] + rows] = True
+    _, count, history, tables = c.device()
+    ops.attention_quantized(q, c.cache, out, torch.tensor(starts, dtype=torch.int32, device=DEV), count, history, tables, heads, g, dim, None, c.scale, *c.bounds())
+    assert bool((out[~mine.to(DEV)] == 7.0).all())
+    for r, (rows, _) in enumerate(c.requests):
+        assert torch.equal(out[starts[r]:starts[r] + rows].double().cpu(), want[c.starts[r]:c.starts[r] + rows])
+
+
+@gpu
+@pytest.mark.parametrize("store", ["e4m3", "bfloat16"])
+@pytest.mark.parametrize("dtype, heads, g, dim, n", [f for f in FORMS if f[-1] > 1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_row_of_queries_that_are_no_numbers_is_its_own(store, dtype, heads, g, dim, n, bad):
+    requests = [(n, 300), (2, 40)]
+    c = Case(requests, heads, g, dim, 16, dtype, store, seed=54, spare_rows=0)
+    if store == "bfloat16":
+        c.tree = random_tree(requests, 54)[:n + 2]
+        c.tree[1] = 1                                    # (sees something)
+    want, q = c.run(), c.q.clone()
+    c.q[1, :2 * dim] = bad
+    got, c.q = c.run(), q
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[1, :2 * dim] = True
+    assert bool(got[hit].isnan().all())
+    # (Not the same bits: a warp's rows are given new references together, when one of them needs it.)
+    c.done = torch.where(hit, want, got)
+    c.__class__ = Done
+    c.check()
