@@ -146,16 +146,19 @@ __device__ __forceinline__ float4 finished(float4 acc, float top, float peak, fl
     return make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 }
 
-// Which of a stage's rows, a lane each, at `at` are zeros (of either sign) throughout.
+// Which of a stage's rows, a lane each, at `at` are zeros (of either sign) throughout; it stops at the piece that says so.  (8 x 8,192 keys
+// whose values all have a row of zeros' byte 32.0 -> 35.0 us, 39.3 without stopping; all of zeros 41.4.)
 template <int ROW>
 __device__ __forceinline__ unsigned rows_of_zeros(uint32_t at) {
     uint32_t any = 0;
+    unsigned zeros = 0xffffffffu;
 #pragma unroll 1
-    for (int piece = 0; piece < ROW / 16; ++piece) {
+    for (int piece = 0; piece < ROW / 16 && zeros; ++piece) {
         const uint4 v = read16(at + place<ROW>(threadIdx.x & 31, piece));
-        any |= v.x | v.y | v.z | v.w;
+        any |= (v.x | v.y | v.z | v.w) & 0x7F7F7F7Fu;
+        zeros = __ballot_sync(0xffffffffu, any == 0);
     }
-    return __ballot_sync(0xffffffffu, (any & 0x7F7F7F7Fu) == 0);
+    return zeros;
 }
 
 // bfloat16 values that are no numbers, of keys that not every row sees: their products are added one by one for the rows that do, and

@@ -535,11 +535,11 @@ pages_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __res
                     if (!dead && vb == 127) {                    // the byte of a row of zeros
                         unsigned any = 0;
 #pragma unroll 1
-                        for (int n = 0; n < 8; ++n) {
+                        for (int n = 0; n < 8 && !any; ++n) {
                             const uint4 v = *reinterpret_cast<const uint4*>(smem + stage * S::STAGE + (key >> 3) * 2048 + 1024 + (key & 7) * 128 + n * 16);
-                            any |= v.x | v.y | v.z | v.w;
+                            any = (v.x | v.y | v.z | v.w) & 0x7F7F7F7Fu;
                         }
-                        nothing = !(any & 0x7F7F7F7Fu);
+                        nothing = !any;
                     }
                     // A value that is no number makes its key none: NaN for the rows that see it.
                     k_power = dead ? 0.0f : vb == e4m3::NOT_NUMBERS ? NAN : e4m3::up(kb);
