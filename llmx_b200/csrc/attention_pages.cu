@@ -143,10 +143,10 @@ FewPlan few_plan(int q_dtype, int cache_dtype, int requests, int max_rows, int m
     const bool types = (cache_dtype == LLMX_E4M3 && (q_dtype == LLMX_BF16 || q_dtype == LLMX_F32)) || (cache_dtype == LLMX_BF16 && q_dtype == LLMX_BF16);
     if (!types || (head_dim != 64 && head_dim != 128) || page_size % 16 || page_size > 512) return p;
     const long long pairs = (long long)max_rows * (heads / kv_heads);
-    // Over eight bits the warps' form is as fast up to 32 pairs and simpler to feed (us; warps against tcgen05 with tiles as high as the
-    // pairs ask for: 1 x 32,768 keys of 4 pairs 25.6 / 26.6, 8 x 8,192 32.6 / 34.3, 64 requests of 2 pairs 63 / 70, 8 x 4,096 of 32 pairs
-    // 33.2 / 34.4); from 33 on a tile's keys are turned into halves for too many warps (8 x 4,096 of 64 pairs 57.6 / 52.4, 1 x 8,191 of
-    // 252 54.3 / 43.6; 32 x 1,024 of 64 71 / 74).
+    // Over eight bits the warps' form is as fast up to 32 pairs and simpler to feed; from 33 on a tile's keys are turned into halves for too
+    // many warps.  In us, warps against tcgen05, each with tiles as high as the pairs ask for (the slower side of each, tcgen05's tiles of 16
+    // and 32 rows and the warps' of 64, is no longer built): 1 x 32,768 keys of 4 pairs 25.6 / 26.6, 8 x 8,192 32.6 / 34.3, 64 requests of 2
+    // pairs 63 / 70, 8 x 4,096 of 32 pairs 33.2 / 34.4; 8 x 4,096 of 64 pairs 57.6 / 52.4, 1 x 8,191 of 252 54.3 / 43.6, 32 x 1,024 of 64 71 / 74.
     p.tensor = head_dim == 128 && q_dtype == LLMX_BF16 && (cache_dtype == LLMX_BF16 || pairs > 32);
     // As few rows a tile as hold a request's: bfloat16, 8 x 4,096 keys, tiles of 16 / 32 / 64 rows: of 16 pairs 39 / 45 / 49 us, of 32 60 /
     // 46 / 51, of 64 106 / 72 / 54.

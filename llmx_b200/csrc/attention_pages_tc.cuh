@@ -10,8 +10,8 @@
 // nothing.  A softmax thread has one key and all rows, so that a key's power of two is its thread's own.
 //
 // Eight bits on both sides: a query is two codes that add up to it, q = (q1 + q2 / 32) 2^e (bfloat16 has 8 bits, a code 4: exact down
-// to 2^-22 of the row's largest), a weight three, w = w1 + w2 / 32 + w3 / 1024 (12 bits, down to 2^-20 of the largest): columns of their
-// own, whose sums are added up in 32 bits.  As in the warp form a value's power of two belongs to its key's weight; a row of zeros and a page
+// to 2^-22 of the row's largest), a weight, by then a half (11 bits), three, w = w1 + w2 / 32 + w3 / 1024 (down to 2^-20 of the largest):
+// columns of their own, whose sums are added up in 32 bits.  As in the warp form a value's power of two belongs to its key's weight; a row of zeros and a page
 // that is not there count with 2^-126.
 //
 //   warps 0, 10     page lookups and copies, STAGES tiles ahead, every other tile each: 16 keys and their values a copy (a warp issues
@@ -29,8 +29,8 @@
 // Work is cut evenly as in the warp form, one block an SM, tiles of 128 keys.
 //
 // Measured with the kernel that adds up (32 heads over 8): trees of 16 tokens for 8 requests after 4,096 keys of eight bits 52.5 us, one of 63 after
-// 8,191 of bfloat16 46, one token each after 8 x 8,191 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows takes 3,300 clocks: 500 until a unit
-// has begun, 650 to read scores, 800 for exponentials and weights, 1,000 to store these; the tensor pipe is 8 % busy, and two softmax warps a
+// 8,191 of bfloat16 46, one token each after 8 x 8,191 of bfloat16 60 (4.5 TB/s).  A tile of 64 rows over eight bits takes 3,300 clocks: 500 until a
+// unit has begun, 650 to read scores, 800 for exponentials and weights, 1,000 to store these, the rest between (barriers, sums); the tensor pipe is 8 % busy, and two softmax warps a
 // scheduler are what registers allow (four units of 16 rows, 96 registers a thread: 57 and 52 us).
 #pragma once
 #include "attention_pages_mma.cuh"

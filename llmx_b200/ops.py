@@ -1464,7 +1464,9 @@ def attention_quantized(q: torch.Tensor, cache: QuantizedPages, out: torch.Tenso
     Key t of a request lies in page block_tables[r, t // page size]; a page that is not in the cache reads as zeros.
     row_start, row_count, history int32 [requests] and block_tables int32 [requests, pages] on the device, as a step's metadata
     has them; `max_rows`, `max_context`: the most rows that a request brings and the most keys that one has, its own rows' among
-    them.  Rows of no request are left as they are."""
+    them.  Rows of no request are left as they are; requests have rows of their own.  Heads of 64 or 128 in pages of whole 16s up to 512
+    slots, rows on 16 bytes, run on matrix instructions (bfloat16 queries of a request's many rows, where `max_rows` allows them: weights
+    are rounded to bfloat16 there, else to half precision); other sizes take a general form, some hundred times slower."""
     _need(isinstance(cache, QuantizedPages), "attention_quantized: a cache in eight bits (QuantizedPages)")
     return _attention_pages("attention_quantized", q, cache, out, row_start, row_count, history, block_tables, None, heads, kv_heads, head_dim, window,
                             scale, max_rows, max_context)
@@ -1475,8 +1477,9 @@ def attention_tree(q: torch.Tensor, cache, out: torch.Tensor, row_start: torch.T
                    max_context: int) -> torch.Tensor:
     """`attention_quantized` for rows that are drafted tokens: a row sees its request's whole history, and key history[r] + j, that
     of the request's j-th row, where bit j % 32 of word j // 32 of its words in `tree` (int32 [rows, words], `tree_bits`) is set:
-    rows may see rows behind them, and not themselves; one that sees no key, or only keys with scores of -inf, is zeros.  `cache`: `QuantizedPages`, or bfloat16 or
-    float32 [pages, 2, kv_heads, page size, head_dim].  Where the drafted tokens' rotations stand is the queries' and keys' own
+    rows may see rows behind them, and not themselves; one that sees no key, or only keys with scores of -inf, is
+    zeros.  `cache`: `QuantizedPages`, or bfloat16 or float32 [pages, 2, kv_heads, page size, head_dim]; over bfloat16 weights are rounded to
+    that, and float32 queries over it and a float32 cache take the general form.  Where the drafted tokens' rotations stand is the queries' and keys' own
     business."""
     return _attention_pages("attention_tree", q, cache, out, row_start, row_count, history, block_tables, tree, heads, kv_heads, head_dim, None, scale,
                             max_rows, max_context)
