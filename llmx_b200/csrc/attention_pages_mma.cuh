@@ -18,7 +18,7 @@
 // set that maximum and leave small values no bits: it counts with 2^-127, as a page that is not there.  Queries in
 // 32 bits, and their weights, are two halves each.  Over bfloat16 pages queries, keys, values and weights are bfloat16.
 //
-// Measured with the kernel that adds up (32 heads of 128 over 8, bfloat16 queries): 8 x 8,192 keys 31.7 us, 4.3 TB/s (33 alone and cold: 244 registers,
+// Measured with the kernel that adds up (32 heads of 128 over 8, bfloat16 queries): 8 x 8,192 keys 31.7 us, 4.3 TB/s (32 alone and cold: 244 registers,
 // so eight warps an SM, 37 % of issue slots, tensor pipe 24 %: what bounds the tiles is the length of a warp's chain); 1 x 32,768 23.1 us.
 //
 // A row's head axis is walked in an order that lets a lane read its keys in 16-byte pieces: piece 4h + c of a row's bytes belongs to
