@@ -94,6 +94,9 @@ def _need_eight_bits(model, specs) -> None:
     if others or not any(isinstance(s, KVSpec) for s in specs):
         raise StepError("a cache in eight bits holds the keys and values of attention mixers alone"
                         + (f"; this model has {', '.join(others)}" if others else ""))
+    widest = max(s.head_dim for s in specs if isinstance(s, KVSpec))
+    if widest > 256:
+        raise StepError(f"a cache in eight bits holds heads of 256 values at most; this model has {widest}")
 
 
 ROOM_STEP = 2048           # a recording's room for context is a multiple of this

@@ -44,3 +44,18 @@ def test_pages_of_other_types_are_attended_under_a_tree_alone(cache, window):
     assert runtime.lib().llmx_pages_attention(packed) != 0 and "under a tree alone" in runtime.last_error()
     assert runtime.lib().llmx_pages_workspace(packed) == 0
     assert cache == ops.F32 or room(requests=2, rows=20, max_rows=10, cache=cache, tree_words=1) > 0
+
+
+# ---- engines ------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("width, refused", [(256, False), (264, True)])
+def test_an_engine_of_wide_heads_is_refused_before_its_first_step(width, refused):
+    from configs import TINY_E
+    from llmx_b200.engine.engine import StepError, _need_eight_bits
+    from llmx_b200.registry import architecture_of
+    entry = architecture_of(dict(TINY_E, head_dim=width))
+    model = entry.build(entry.config_cls.from_dict(dict(TINY_E, head_dim=width)))
+    if refused:
+        with pytest.raises(StepError, match="256 values at most"):
+            _need_eight_bits(model, model.cache_entry_specs())
+    else:
+        _need_eight_bits(model, model.cache_entry_specs())
